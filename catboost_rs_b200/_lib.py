@@ -7,7 +7,9 @@ is no CPU fallback.
 from __future__ import annotations
 
 import ctypes as C
+import importlib.util
 import os
+import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libcbgpu.so")
@@ -39,6 +41,25 @@ class BeginArgs(C.Structure):
     ]
 
 
+F64, F32, F16, BF16 = range(4)  # cbgpu_dtype
+
+
+class Logits(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("dtype", C.c_int32), ("n_classes", C.c_int32), ("n", C.c_int64),
+                ("row_stride", C.c_int64), ("class_stride", C.c_int64)]
+
+
+class Teacher(C.Structure):
+    _fields_ = [("index", C.c_void_p), ("value", C.c_void_p), ("tail", C.c_void_p), ("index_bytes", C.c_int32),
+                ("value_dtype", C.c_int32), ("k", C.c_int32)]
+
+
+class Sampling(C.Structure):
+    _fields_ = [("uniform", C.c_void_p), ("temperature_rows", C.c_void_p), ("top_p_rows", C.c_void_p),
+                ("min_p_rows", C.c_void_p), ("top_k_rows", C.c_void_p), ("temperature", C.c_double),
+                ("top_p", C.c_double), ("min_p", C.c_double), ("top_k", C.c_int32), ("uniform_dtype", C.c_int32)]
+
+
 EXPORTS = [
     "cbgpu_begin", "cbgpu_begin_raw", "cbgpu_grow_tree", "cbgpu_end", "cbgpu_stage_sample",
     "cbgpu_compute_gradients",
@@ -50,6 +71,7 @@ EXPORTS = [
     "cbgpu_select_borders", "cbgpu_apply_oblivious",
     "cbgpu_multi_begin_raw", "cbgpu_multi_begin_cat_raw", "cbgpu_multi_grow_tree", "cbgpu_multi_approx", "cbgpu_multi_end",
     "cbgpu_rank_begin_raw",
+    "cbgpu_top_logits", "cbgpu_distill", "cbgpu_sample_classes",
 ]
 
 _lib = None
@@ -63,6 +85,25 @@ class CbGpuError(RuntimeError):
         self.code = code
 
 
+def _preload_nccl():
+    """Load the NCCL that torch ships before libcbgpu.so asks for the system's: a process holds
+    one libnccl.so.2, and a torch imported later needs its own (newer) one."""
+    if "torch" in sys.modules:
+        return
+    try:
+        spec = importlib.util.find_spec("nvidia.nccl")
+    except (ImportError, ValueError):
+        return
+    for where in (spec.submodule_search_locations if spec else None) or ():
+        so = os.path.join(where, "lib", "libnccl.so.2")
+        if os.path.exists(so):
+            try:
+                C.CDLL(so)
+            except OSError:
+                pass
+            return
+
+
 def load(path: str = LIB_PATH):
     """Load libcbgpu.so and declare every exported signature."""
     global _lib
@@ -70,6 +111,7 @@ def load(path: str = LIB_PATH):
         return _lib
     if not os.path.exists(path):
         raise ImportError(f"{path} is missing: build it with `python -m catboost_rs_b200.build`")
+    _preload_nccl()
     L = C.CDLL(path)
     vp, i32, i64, u64, f64, f32 = C.c_void_p, C.c_int32, C.c_int64, C.c_uint64, C.c_double, C.c_float
     sig = {
@@ -105,6 +147,9 @@ def load(path: str = LIB_PATH):
         "cbgpu_rank_begin_raw": ([C.POINTER(BeginArgs), vp, i32, vp, vp, i64, C.POINTER(RankParams), vp, vp, vp,
                                   C.POINTER(vp)], C.c_int),
         "cbgpu_multi_end": ([vp], C.c_int),
+        "cbgpu_top_logits": ([C.POINTER(Logits), i32, f64, vp, vp, vp, vp], C.c_int),
+        "cbgpu_distill": ([C.POINTER(Logits), C.POINTER(Teacher), vp, f64, vp, vp, i64, i64, vp], C.c_int),
+        "cbgpu_sample_classes": ([C.POINTER(Logits), C.POINTER(Sampling), vp, vp], C.c_int),
         "cbgpu_nccl_unique_id": ([vp], C.c_int),
         "cbgpu_version": ([], C.c_char_p),
     }

@@ -503,6 +503,109 @@ CBGPU_API int cbgpu_apply_oblivious(const float* features_fm, int64_t n, int32_t
                                     const double* leaf_values, const uint32_t* tree_leaf_offsets, double bias,
                                     const uint8_t* nan_above, int32_t device, double* out);
 
+/* ---- class logits -------------------------------------------------------
+ *
+ * Operators on rows of class logits held on the DEVICE: a booster's
+ * multi-class approximants (CBGPU_F64, dim-major: row_stride 1, class_stride
+ * n) or the rows of a neural teacher or student (class_stride 1).  No
+ * counterpart in the reference, whose losses take labels, not another
+ * model's logits.
+ *
+ * Pointers are device pointers of the CURRENT device, owned by the caller;
+ * work is enqueued on `stream` (a cudaStream_t; NULL = the legacy default
+ * stream) and the call returns without waiting.  The calls allocate nothing,
+ * hold no state and share no workspace, so they may overlap on any streams
+ * and be captured into graphs.  Arithmetic and the "wide" outputs are f64 for
+ * CBGPU_F64 logits and f32 for the other types; sums are taken in 64 bits.
+ * Results do not depend on the launch or on timing.
+ * Classes are ordered by logit, larger first, equal logits (-0 == +0) by
+ * lower index, NaN last.  Limits: 1..262144 classes, n < 2^31 rows; n = 0 is
+ * a call that does nothing. */
+typedef enum { CBGPU_F64 = 0, CBGPU_F32 = 1, CBGPU_F16 = 2, CBGPU_BF16 = 3 } cbgpu_dtype;
+
+typedef struct {
+    const void* data;
+    int32_t dtype;        /* cbgpu_dtype */
+    int32_t n_classes;
+    int64_t n;            /* rows */
+    int64_t row_stride;   /* in elements, >= 0; any, also 0 */
+    int64_t class_stride;
+} cbgpu_logits;
+
+/* The k largest logits of every row in order, and the log-sum-exp of the
+ * others at a temperature: what cbgpu_distill takes as its teacher.
+ *  k            1..min(256, n_classes);
+ *  temperature  1e-6..1e6 (it enters the tail only);
+ *  value        [n][k] of the logits' dtype;  index [n][k];
+ *  tail         [n] wide: ln sum of exp(a_i / temperature) over the classes
+ *               not in the row's k; -inf where they are none or all masked
+ *               (-inf); NaN where the row holds a NaN; or NULL. */
+CBGPU_API int cbgpu_top_logits(const cbgpu_logits* logits, int32_t k, double temperature, void* value,
+                               int32_t* index, void* tail, void* stream);
+
+/* A teacher's rows: k logits with their classes, [n][k] each, and the
+ * log-sum-exp of its other classes at the temperature of the call. */
+typedef struct {
+    const void* index;    /* int32 or int64; an index outside 0..n_classes - 1 is no entry, of equal
+                             indices in a row the first counts */
+    const void* value;
+    const void* tail;     /* [n] wide, or NULL: the teacher is renormalised over its k classes */
+    int32_t index_bytes;  /* 4 or 8 */
+    int32_t value_dtype;  /* cbgpu_dtype */
+    int32_t k;            /* 1..256 */
+} cbgpu_teacher;
+
+/* Distillation from a teacher's top logits.  With p = softmax(a / T) of the
+ * student's row a, S the teacher's classes, q and Q its probabilities for
+ * each of S and for all others together (softmax over value / T and tail),
+ * P = sum of p outside S:
+ *   loss = w T^2 [ sum_S q ln(q / p) + Q ln(Q / P) ]       [n] wide
+ *   der1 = -d loss / d a = w T (q_i - p_i) in S,  -w T p_i (1 - Q / P) outside
+ * (the sign of cbgpu_compute_gradients' der1).
+ *  weight  [n] wide, or NULL = 1; a row of weight 0 gives loss 0 and der1 0
+ *          whatever it holds;
+ *  der1    of the logits' dtype with its own strides (no two elements may
+ *          share memory), or NULL for the loss alone; it may be the logits
+ *          themselves (same pointer and strides), else must not overlap any
+ *          other array of the call.
+ * A row whose classes are all masked (-inf), or whose teacher has no entry
+ * left, gives 0; NaN or +inf among a row's logits or entries gives NaN; a
+ * class the student masks but the teacher does not gives loss +inf. */
+CBGPU_API int cbgpu_distill(const cbgpu_logits* logits, const cbgpu_teacher* teacher, const void* weight,
+                            double temperature, void* loss, void* der1, int64_t der1_row_stride,
+                            int64_t der1_class_stride, void* stream);
+
+/* Settings of cbgpu_sample_classes; a *_rows array ([n], on the device)
+ * replaces the value beside it where it is not NULL. */
+typedef struct {
+    const void* uniform;           /* [n] the given random numbers, in [0, 1) */
+    const float* temperature_rows; /* <= 0 or NaN: the first class in order; above 1e6 counts as 1e6 */
+    const float* top_p_rows;       /* 1 and above or NaN: off */
+    const float* min_p_rows;       /* 0 and below or NaN: off; above 1 counts as 1 */
+    const int32_t* top_k_rows;     /* <= 0: off */
+    double temperature;            /* 0 (the first class in order) or 1e-6..1e6 */
+    double top_p;                  /* 0..1; 1 = off */
+    double min_p;                  /* 0..1; 0 = off */
+    int32_t top_k;                 /* >= 0; 0 = off */
+    int32_t uniform_dtype;         /* CBGPU_F32 or CBGPU_F64 */
+} cbgpu_sampling;
+
+/* One class a row, drawn from softmax(a / temperature) under filters, applied
+ * in this order (the first class in order always stays):
+ *   top_k  the first k classes in order stay;
+ *   top_p  in order, a class stays while the probability before it is below
+ *          top_p, of what top_k left;
+ *   min_p  a class stays while its probability is at least min_p times the
+ *          largest.
+ * Drawn is the first class by INDEX whose running sum of kept probabilities
+ * exceeds uniform times their sum.  Weights are held as integers of
+ * min(52, 62 - ceil(log2 n_classes)) bits, so the sums are exact; a class
+ * whose probability is below half of the last bit of the largest is never
+ * drawn.  Among +inf logits the draw is uniform.
+ *  index  [n]; -1 where the row holds a NaN or masks every class (-inf). */
+CBGPU_API int cbgpu_sample_classes(const cbgpu_logits* logits, const cbgpu_sampling* sampling, int32_t* index,
+                                   void* stream);
+
 /* NCCL unique id (128 bytes) for world_size > 1 sessions. */
 CBGPU_API int cbgpu_nccl_unique_id(uint8_t* out128);
 

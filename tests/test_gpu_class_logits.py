@@ -1,0 +1,466 @@
+"""Class-logit operators on the device against their plain 64-bit forms (logits_reference.py).
+
+Tolerances.  u is the unit roundoff of the arithmetic (2^-24 for 16- and 32-bit
+logits, 2^-53 for f64).  An exponential's argument (a - m) / T passes two
+rounded operations and a scale rounded once, so it is off by at most 3u times
+its size; with `reach` the largest such size that matters (beyond it the
+probability is below u) an exponential is off by 3u reach plus 2 ulp = 4u of its
+own, a probability (two of them) by 2 (3u reach + 4u) of itself.  Outputs add
+half a step of their type.  The logarithm of a sum is off by one such relative
+error, absolutely; a loss holds two of them and 3u of the scaled logits it
+subtracts.
+"""
+import numpy as np
+import pytest
+
+import catboost_rs_b200 as cb
+from tests import logits_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+DTYPES = {"f64": torch.float64, "f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+@pytest.fixture(scope="module", autouse=True)
+def cuda():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+
+
+def unit(dtype):
+    return 2.0 ** -53 if dtype == "f64" else 2.0 ** -24
+
+
+def rounding(dtype):
+    return torch.finfo(DTYPES[dtype]).eps / 2
+
+
+def host(x):
+    return x.detach().to("cpu").double().numpy()
+
+
+def make(n, V, dtype, layout, seed, masked=0.0, spread=2.5):
+    """Device logits with the layout asked for; ties are frequent in 16 bits."""
+    rs = np.random.RandomState(seed)
+    a = rs.standard_normal((n, V)) * spread
+    if V > 50:
+        a[np.arange(n)[:, None], rs.randint(0, V, (n, 4))] += rs.uniform(3, 9, (n, 4))
+    if masked:
+        a[rs.uniform(size=(n, V)) < masked] = -np.inf
+    return put(a, dtype, layout)
+
+
+def put(a, dtype, layout="rows"):
+    n, V = a.shape
+    t = torch.from_numpy(np.ascontiguousarray(a)).to(DTYPES[dtype]).cuda()
+    if layout == "rows":
+        return t
+    if layout == "dims":
+        return t.t().contiguous().t()
+    if layout == "offset":  # rows that start at no particular alignment, with room behind them
+        big = torch.full((n, V + 3), float("nan"), dtype=t.dtype, device="cuda")
+        big[:, 1:V + 1] = t
+        return big[:, 1:V + 1]
+    if layout == "strided":
+        big = torch.full((2 * n, 3 * V), float("nan"), dtype=t.dtype, device="cuda")
+        big[::2, ::3] = t
+        return big[::2, ::3]
+    raise ValueError(layout)
+
+
+SHAPES = [(1, 1), (5, 2), (300, 7), (70, 12), (33, 13), (40, 100), (9, 128), (21, 129), (10, 1000), (3, 1024),
+          (4, 1025), (3, 2048), (2, 4099), (2, 33000), (1, 131071), (1, 262144)]
+LAYOUTS = ["rows", "dims", "offset", "strided"]
+
+
+def grid(shapes=SHAPES):
+    """Every shape with every type; the layout and the mask go round."""
+    out = []
+    for s, (n, V) in enumerate(shapes):
+        for d, dtype in enumerate(DTYPES):
+            out.append((n, V, dtype, LAYOUTS[(s + d) % 4], [0.0, 0.3][(s + d // 2) % 2]))
+    return out
+
+
+# ---- top_logits ------------------------------------------------------------------
+
+def check_top(x, k, temperature, dtype):
+    got = cb.top_logits(x, k, temperature=temperature)
+    a = host(x)
+    u = unit(dtype)
+    idx, val, tail = got.index.cpu().numpy(), host(got.value), host(got.tail)
+    assert got.index.dtype == torch.int32 and got.value.dtype == x.dtype
+    for r in range(a.shape[0]):
+        wi, wv, wt = ref.top(a[r], k, temperature)
+        assert (idx[r] == wi).all(), (r, idx[r], wi)
+        assert np.array_equal(val[r], wv, equal_nan=True)
+        if np.isfinite(wt):
+            rest = np.delete(a[r], wi) / temperature
+            reach = min(np.max(rest) - np.min(rest[np.isfinite(rest)]), 40.0)
+            assert abs(tail[r] - wt) <= u * (3 * reach + 4) + 3 * u * abs(wt), (r, tail[r], wt)
+        else:
+            assert np.array_equal(tail[r], wt, equal_nan=True), (r, tail[r], wt)
+
+
+@pytest.mark.parametrize("n,V,dtype,layout,masked", grid())
+def test_top_logits(n, V, dtype, layout, masked):
+    x = make(n, V, dtype, layout, V + n, masked)
+    for k in sorted({1, min(V, 5), min(V, 64), min(V, 256)}):
+        check_top(x, k, 0.7, dtype)
+
+
+@pytest.mark.parametrize("V", [5, 60, 700, 5000])
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_top_logits_ties_masks_and_nan(V, dtype):
+    rows = [np.zeros(V), np.full(V, -np.inf), np.where(np.arange(V) % 2, -0.0, 0.0),
+            np.where(np.arange(V) % 3, 1.0, -np.inf), np.full(V, np.nan), np.arange(V) % 4 * 1.0]
+    one = np.linspace(3, -3, V)
+    one[V // 2] = np.nan
+    low = np.full(V, float(torch.finfo(DTYPES[dtype]).min))
+    low[V - 1] = 1.0
+    rows += [one, low, np.sort(np.arange(V) * 0.125)[::-1].copy()]
+    x = put(np.array(rows), dtype)
+    for k in {1, 3, min(V, 200)}:
+        check_top(x, k, 1.0, dtype)
+    got = cb.top_logits(x, 2, tail=False)
+    assert got.tail is None
+
+
+# ---- distillation -------------------------------------------------------------------
+
+def check_distill(x, teacher, weight, temperature, dtype, out=None):
+    u, V = unit(dtype), x.shape[1]
+    a = host(x)
+    loss_only = host(cb.distill_loss(x, teacher, weight=weight, temperature=temperature))
+    got = cb.distill_derivatives(x, teacher, weight=weight, temperature=temperature, out=out)
+    assert got.der1.dtype == x.dtype and got.der1.shape == x.shape
+    loss, der1 = host(got.loss), host(got.der1)
+    idx, val = teacher.index.cpu().numpy(), host(teacher.value)
+    tail = np.full(len(a), -np.inf) if teacher.tail is None else host(teacher.tail)
+    w = np.ones(len(a)) if weight is None else host(weight)
+    small = float(torch.finfo(x.dtype).smallest_normal) * float(torch.finfo(x.dtype).eps)
+    for r in range(len(a)):
+        wl, wd, p, q = ref.distill(a[r], idx[r], val[r], tail[r], w[r], temperature)
+        scaled = np.concatenate([a[r], val[r], [0.0]]) / temperature
+        scaled = np.concatenate([scaled[np.isfinite(scaled)], tail[r:r + 1][np.isfinite(tail[r:r + 1])]])
+        size = np.abs(scaled).max()
+        reach = min(scaled.max() - scaled.min(), 40.0)
+        rel = 2 * u * (3 * reach + 4)
+        wt2 = abs(w[r]) * temperature * temperature
+        for g in (loss[r], loss_only[r]):
+            if np.isfinite(wl):
+                assert abs(g - wl) <= wt2 * (2 * rel + 6 * u * size) + 4 * u * abs(wl), (r, g, wl)
+            else:
+                assert np.array_equal(g, wl, equal_nan=True), (r, g, wl)
+        if np.isnan(wd).any():
+            assert np.isnan(der1[r]).all()
+            continue
+        bound = abs(w[r]) * temperature * rel * 2 * (p + q) + rounding(dtype) * np.abs(wd) + small
+        off = np.abs(der1[r] - wd) - bound
+        assert off.max() <= 0, (r, int(off.argmax()), der1[r][off.argmax()], wd[off.argmax()])
+    return got
+
+
+def make_teacher(n, V, k, dtype, seed, tail, masked=0.0, int64=False, temperature=1.0):
+    z = make(n, V, dtype, "rows", seed, masked)
+    t = cb.top_logits(z, min(k, V), temperature=temperature)
+    index = t.index.long() if int64 else t.index
+    return cb.TopLogits(index, t.value, t.tail if tail else None)
+
+
+@pytest.mark.parametrize("n,V,dtype,layout,masked", grid())
+def test_distill(n, V, dtype, layout, masked):
+    # a class that only the student masks gives +inf: the masks are the teacher's, and half of
+    # the shapes have them
+    x = make(n, V, dtype, layout, V + n, 0.0)
+    wide = torch.float64 if dtype == "f64" else torch.float32
+    weight = torch.rand((n,), dtype=wide, device="cuda", generator=torch.Generator("cuda").manual_seed(V)) + 0.5
+    for k, tail, w, temperature in ((1, True, None, 1.0), (16, False, weight, 2.0), (256, True, weight, 0.7)):
+        check_distill(x, make_teacher(n, V, k, dtype, V + 7, tail, masked, k == 16, temperature), w, temperature,
+                      dtype)
+
+
+@pytest.mark.parametrize("V", [6, 60, 900, 6000])
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_distill_edges(V, dtype):
+    wide = torch.float64 if dtype == "f64" else torch.float32
+    rs = np.random.RandomState(V)
+    ninf, nan, inf = -np.inf, np.nan, np.inf
+    rows, idx, val, tail, w = [], [], [], [], []
+
+    def add(row, i, z, t=ninf, weight=1.0):
+        i = list(i) + [-1] * (5 - len(i))
+        z = list(z) + [0.0] * (5 - len(z))
+        rows.append(row), idx.append(i), val.append(z), tail.append(t), w.append(weight)
+
+    plain = rs.randn(V)
+    add(plain, [0, 1], [1, 2])                                    # entries missing
+    add(plain, [], [])                                            # no entry at all
+    add(plain, [], [], 0.5)                                       # the others only: loss 0
+    add(plain, [3, 3, 3], [1, 7, nan], 0.2)                       # the same index: the first counts
+    add(plain, [1, V, -5, V + 100, 2], [1, 9, 9, 9, 2], 0.1)      # indices outside
+    add(np.full(V, ninf), [1], [1.0], 0.1)                        # every class masked
+    add(np.full(V, nan), [1], [1.0], 0.1, 0.0)                    # weight 0: not read
+    add(np.full(V, nan), [1], [1.0], 0.1)
+    add(np.where(np.arange(V) == 2, nan, plain), [1], [1.0])
+    add(np.where(np.arange(V) == 2, inf, plain), [1], [1.0])
+    add(np.where(np.arange(V) == 2, ninf, plain), [1, 2], [1.0, 1.0])   # the student masks an entry: +inf
+    add(np.where(np.arange(V) == 2, ninf, plain), [1, 2], [1.0, ninf])  # both do
+    add(np.where(np.arange(V) == 0, 1.0, ninf), [0], [1.0], 0.3)  # the student masks all others: +inf
+    add(np.where(np.arange(V) == 0, 1.0, ninf), [0], [1.0])       # both do: loss 0
+    add(plain, [1], [nan])
+    add(plain, [1], [1.0], nan)
+    add(plain, [1], [inf])
+    add(plain, [0, 1, 2], [ninf, ninf, ninf])                     # entries of no weight
+    add(np.full(V, float(torch.finfo(DTYPES[dtype]).min)), [0, 4], [1.0, 2.0], 0.5)  # masked by the lowest value
+    add(np.zeros(V), [4, 0], [0.0, 0.0], 0.5, -2.0)
+    for layout in ("rows", "dims"):
+        x = put(np.array(rows), dtype, layout)
+        t = cb.TopLogits(torch.tensor(idx, dtype=torch.int32, device="cuda"),
+                         torch.tensor(val, dtype=DTYPES[dtype], device="cuda"),
+                         torch.tensor(tail, dtype=wide, device="cuda"))
+        check_distill(x, t, torch.tensor(w, dtype=wide, device="cuda"), 1.0, dtype)
+
+
+@pytest.mark.parametrize("V", [10, 100, 1000, 5000])
+@pytest.mark.parametrize("dtype", ["f64", "bf16"])
+def test_distill_out(V, dtype):
+    n = 37
+    x = make(n, V, dtype, "rows", 3)
+    t = make_teacher(n, V, 8, dtype, 4, True)
+    want = check_distill(x, t, None, 1.0, dtype).der1
+    # a strided view: what lies between and behind its rows stays
+    big = torch.full((n + 2, 2 * V + 5), 7.0, dtype=x.dtype, device="cuda")
+    view = big[1:n + 1, 2:2 + 2 * V:2]
+    got = cb.distill_derivatives(x, t, out=view)
+    assert got.der1.data_ptr() == view.data_ptr() and torch.equal(view, want)
+    view.fill_(7.0)
+    assert (big == 7.0).all()
+    dims = torch.empty((V, n), dtype=x.dtype, device="cuda").t()
+    assert torch.equal(cb.distill_derivatives(x, t, out=dims).der1, want)
+    # in place, for each layout
+    for layout in LAYOUTS:
+        y = put(host(x), dtype, layout)
+        assert torch.equal(cb.distill_derivatives(y, t, out=y).der1, want)
+        assert torch.equal(y, want)
+    # rows that share memory can be read
+    one = x[:1].expand(n, V)
+    assert torch.equal(cb.distill_derivatives(one, t).der1, cb.distill_derivatives(one.contiguous(), t).der1)
+
+
+def test_distill_teacher_types_mix():
+    x = make(6, 50, "bf16", "rows", 1)
+    for vd in DTYPES.values():
+        t = cb.TopLogits(torch.arange(18, device="cuda").view(6, 3), torch.randn((6, 3), device="cuda").to(vd))
+        check_distill(x, t, None, 1.0, "bf16")
+        wide = cb.TopLogits(t.index[:, ::2], t.value[:, ::2], torch.zeros((12,), device="cuda")[::2])
+        check_distill(x, wide, None, 1.0, "bf16")  # operands that are not contiguous
+
+
+def test_der1_is_minus_the_gradient_by_differences():
+    n, V, k, h = 3, 1500, 9, 1e-4
+    for V in (11, 1500):
+        x = make(n, V, "f64", "rows", 8)
+        t = make_teacher(n, V, k, "f64", 9, True)
+        der1 = host(cb.distill_derivatives(x, t, temperature=1.5).der1)
+        probe = list(range(4)) + [int(i) for i in t.index[0, :4]] + [V - 1]
+        for i in probe:
+            up, dn = x.clone(), x.clone()
+            up[:, i] += h
+            dn[:, i] -= h
+            num = host(cb.distill_loss(up, t, temperature=1.5) - cb.distill_loss(dn, t, temperature=1.5)) / (2 * h)
+            assert np.abs(der1[:, i] + num).max() < 1e-7  # third derivative h^2 / 6 < 1e-8; 1e-15 / h
+
+
+# ---- sampling ----------------------------------------------------------------------
+
+SETTINGS = [dict(), dict(top_k=1), dict(top_k=5), dict(top_p=0.0), dict(top_p=0.3), dict(top_p=0.9),
+            dict(min_p=0.1), dict(min_p=1.0), dict(top_k=300, top_p=0.95, min_p=0.01), dict(temperature=0.0),
+            dict(temperature=0.3, top_p=0.8), dict(temperature=5.0, top_k=70, top_p=0.99)]
+
+
+def check_sample(x, u, **kw):
+    got = cb.sample_classes(x, u, **kw)
+    assert got.dtype == torch.int32
+    a, uh = host(x), host(u)
+    full = dict(temperature=1.0, top_k=0, top_p=1.0, min_p=0.0)
+    full.update(kw)
+    full = {k: (host(v) if isinstance(v, torch.Tensor) else np.full(len(a), v)) for k, v in full.items()}
+    want = [ref.sample(a[r], uh[r], full["temperature"][r], int(full["top_k"][r]), full["top_p"][r], full["min_p"][r])
+            for r in range(len(a))]
+    assert got.cpu().tolist() == [int(v) for v in want], kw
+
+
+@pytest.mark.parametrize("n,V,dtype,layout,masked", grid())
+def test_sample_classes(n, V, dtype, layout, masked):
+    x = make(n, V, dtype, layout, V + n, masked)
+    if V == 1:
+        x = put(np.zeros((n, 1)), dtype)
+    gen = torch.Generator("cuda").manual_seed(V)
+    for i, kw in enumerate(SETTINGS if V < 30000 else SETTINGS[V % 2::3]):
+        u = torch.rand((n,), generator=gen, device="cuda", dtype=torch.float64 if i % 2 else torch.float32)
+        check_sample(x, u, **kw)
+
+
+@pytest.mark.parametrize("V", [8, 90, 1000, 9000])
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_sample_edges(V, dtype):
+    nan, inf = np.nan, np.inf
+    flat = np.zeros(V)
+    lone = np.full(V, -inf)
+    lone[V // 3] = -7.0
+    bad = np.random.RandomState(0).randn(V)
+    bad[V - 1] = nan
+    infs = np.random.RandomState(1).randn(V)
+    infs[[1, V - 2]] = inf
+    low = np.full(V, float(torch.finfo(DTYPES[dtype]).min))
+    low[2] = 0.0
+    steps = -(np.arange(V) % 5) * 1.0
+    one = np.full(V, -30.0)
+    one[V // 2] = 3.0
+    x = put(np.array([flat, lone, bad, infs, low, steps, one, np.full(V, -inf), np.full(V, nan)]), dtype)
+    n = x.shape[0]
+    for u0 in (0.0, 0.37, 0.75, float(np.nextafter(np.float32(1), np.float32(0)))):
+        u = torch.full((n,), u0, device="cuda")
+        for kw in SETTINGS:
+            check_sample(x, u, **kw)
+
+
+def test_sample_per_row_settings_and_strange_numbers():
+    n, V = 64, 300
+    x = make(n, V, "f32", "rows", 5)
+    u = torch.rand((n,), generator=torch.Generator("cuda").manual_seed(1), device="cuda")
+    rs = np.random.RandomState(2)
+    t = torch.from_numpy(rs.choice([0.0, 0.5, 1.0, 2.0, -1.0], n).astype(np.float32)).cuda()
+    k = torch.from_numpy(rs.choice([-3, 0, 1, 7, 299, 300, 1000], n).astype(np.int32)).cuda()
+    p = torch.from_numpy(rs.choice([0.0, 0.5, 0.95, 1.0, 2.0], n).astype(np.float32)).cuda()
+    m = torch.from_numpy(rs.choice([-1.0, 0.0, 0.05, 1.0, 3.0], n).astype(np.float32)).cuda()
+    check_sample(x, u, temperature=t, top_k=k, top_p=p, min_p=m)
+    # numbers outside [0, 1) draw the first or the last class that stays
+    out = cb.sample_classes(x[:3], torch.tensor([-1.0, float("nan"), 1.0], device="cuda"))
+    assert out.cpu().tolist()[:2] == [0, 0] and 0 <= int(out[2]) < V
+    nan = torch.full((n,), float("nan"), device="cuda")
+    assert torch.equal(cb.sample_classes(x, u, top_p=nan, min_p=nan), cb.sample_classes(x, u))
+    assert torch.equal(cb.sample_classes(x, u, temperature=nan), cb.sample_classes(x, u, temperature=0.0))
+
+
+def test_sampling_frequencies_follow_the_softmax():
+    # evenly spaced numbers: each class is drawn its share of them, to one draw at each border
+    n, V = 20000, 23
+    row = make(1, V, "f32", "rows", 11)
+    u = (torch.arange(n, device="cuda", dtype=torch.float64) + 0.5) / n
+    got = np.bincount(cb.sample_classes(row.expand(n, V), u).cpu().numpy(), minlength=V) / n
+    p = torch.softmax(row.double(), 1)[0].cpu().numpy()
+    assert np.abs(got - p).max() <= 1.5 / n
+
+
+# ---- how they are called ---------------------------------------------------------------
+
+def batch(V, dtype="bf16", n=130):
+    x = make(n, V, dtype, "rows", 1)
+    t = cb.top_logits(make(n, V, dtype, "rows", 2), 8)
+    return x, t, torch.rand((n,), generator=torch.Generator("cuda").manual_seed(3), device="cuda")
+
+
+@pytest.mark.parametrize("V", [10, 100, 1000, 40000])
+def test_same_results_again_on_another_stream_and_in_a_graph(V):
+    x, t, u = batch(V)
+
+    def call():
+        d = cb.distill_derivatives(x, t, temperature=2.0)
+        top = cb.top_logits(x, 6)
+        return d.loss, d.der1, top.index, top.value, top.tail, cb.sample_classes(x, u, top_p=0.9, top_k=40)
+
+    want = [v.clone() for v in call()]
+    assert all(torch.equal(a, b) for a, b in zip(call(), want))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = call()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            held = call()
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for v in held:
+        v.zero_()
+    g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(held, want))
+    # new inputs through the same graph
+    x.copy_(x.flip(0))
+    g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(held, [v.clone() for v in call()]))
+
+
+def test_empty_batches_and_refusals():
+    x = torch.empty((0, 9), device="cuda")
+    assert cb.top_logits(x, 3).index.shape == (0, 3)
+    t = cb.TopLogits(torch.empty((0, 3), dtype=torch.int32, device="cuda"), torch.empty((0, 3), device="cuda"))
+    assert cb.distill_derivatives(x, t).der1.shape == (0, 9)
+    assert cb.sample_classes(x, torch.empty((0,), device="cuda")).shape == (0,)
+    x = torch.zeros((4, 9), device="cuda")
+    t = cb.TopLogits(torch.zeros((4, 3), dtype=torch.int32, device="cuda"), torch.zeros((4, 3), device="cuda"))
+    u = torch.zeros((4,), device="cuda")
+    big = torch.zeros((8, 9), device="cuda")
+    bad = [lambda: cb.top_logits(x, 10), lambda: cb.top_logits(x, 0), lambda: cb.top_logits(x, 1, temperature=0.0),
+           lambda: cb.distill_loss(x, (t.index, t.value)), lambda: cb.distill_loss(x[:3], t),
+           lambda: cb.distill_loss(x, cb.TopLogits(t.index.short(), t.value)),
+           lambda: cb.distill_loss(x, cb.TopLogits(t.index, t.value.cpu())),
+           lambda: cb.distill_loss(x, cb.TopLogits(t.index, t.value[:, :2])),
+           lambda: cb.distill_loss(x, cb.TopLogits(t.index, t.value, u.double())),
+           lambda: cb.distill_loss(x, t, weight=u.double()), lambda: cb.distill_loss(x, t, weight=u[:3]),
+           lambda: cb.distill_derivatives(x, t, out=x.half()), lambda: cb.distill_derivatives(x, t, out=x[:3]),
+           lambda: cb.distill_derivatives(x, t, out=x[:1].expand(4, 9)),
+           lambda: cb.distill_derivatives(big[:4], t, out=big[1:5]),
+           lambda: cb.sample_classes(x, u.half()), lambda: cb.sample_classes(x, u[:2]),
+           lambda: cb.sample_classes(x, u.cpu()), lambda: cb.sample_classes(x, u, temperature=-1.0),
+           lambda: cb.sample_classes(x, u, top_p=1.1), lambda: cb.sample_classes(x, u, min_p=float("nan")),
+           lambda: cb.sample_classes(x, u, top_k=-1), lambda: cb.sample_classes(x, u, top_k=u),
+           lambda: cb.top_logits(torch.zeros((2, 262145), device="cuda"), 1)]
+    for call in bad:
+        with pytest.raises(cb.CbGpuError):
+            call()
+
+
+def test_rows_behind_32_bit_offsets():
+    # the last rows start beyond 2^32 elements
+    n, V = 3, 2000
+    store = torch.empty(((1 << 32) + 4096,), dtype=torch.bfloat16, device="cuda")
+    x = torch.as_strided(store, (n, V), (1 << 31, 1))
+    y = make(n, V, "bf16", "rows", 4)
+    x.copy_(y)
+    t = make_teacher(n, V, 8, "bf16", 5, True)
+    u = torch.rand((n,), device="cuda")
+    assert torch.equal(cb.distill_derivatives(x, t, out=x.clone()).der1, cb.distill_derivatives(y, t).der1)
+    assert torch.equal(cb.top_logits(x, 9).index, cb.top_logits(y, 9).index)
+    assert torch.equal(cb.sample_classes(x, u), cb.sample_classes(y, u))
+    want = cb.distill_derivatives(y, t).der1
+    assert torch.equal(cb.distill_derivatives(x, t, out=x).der1, want)
+
+
+def test_from_a_teachers_rows_to_drawn_labels():
+    """The operators as they are used together: a teacher's rows are reduced to their top logits, a
+    student's rows follow der1 towards them, labels are drawn from the student."""
+    n, V = 500, 3000
+    teacher = make(n, V, "f32", "rows", 21, spread=1.0)
+    top = cb.top_logits(teacher, 32)
+    student = torch.zeros((n, V), device="cuda")
+    buf = torch.empty_like(student)
+    # at the teacher's own logits the loss is 0 and der1 vanishes, to rounding
+    at = cb.distill_derivatives(teacher, top)
+    assert float(at.loss.abs().max()) < 1e-5 and float(at.der1.abs().max()) < 1e-5
+    for _ in range(3):
+        before = student.clone()
+        d = cb.distill_derivatives(student, top, out=buf)
+        student += 5.0 * d.der1
+        # the step is uphill in -loss: the loss' derivative along it is -|der1|^2 < 0
+        eps = 1e-2
+        moved = cb.distill_loss(before + eps * d.der1, top)
+        assert bool((moved < d.loss).all())
+    u = torch.rand((n,), generator=torch.Generator("cuda").manual_seed(5), device="cuda")
+    labels = cb.sample_classes(student, u, top_k=8)
+    best = cb.top_logits(student, 8).index
+    assert bool((best == labels[:, None]).any(dim=1).all())
