@@ -1,0 +1,473 @@
+// logits_distill.cu -- cbgpu_distill: the Kullback-Leibler loss of a student's rows against a teacher's
+// top logits, and its derivative.
+#include <type_traits>
+
+#include "logits.cuh"
+
+namespace {
+
+// ---- distillation ------------------------------------------------------------------
+//
+// Row a[V], temperature T, weight w; the teacher's buckets are its k top
+// classes (their distinct valid indices S, the first entry of an index
+// counting) and all others together (tail = their log-sum-exp at T):
+//   q, Q  = softmax over (z_j / T, tail);  p = softmax(a / T);  P = sum of p outside S
+//   loss  = w T^2 [ sum_S q ln(q / p) + Q ln(Q / P) ]
+//   der1  = -d loss / d a = w T (q_i - p_i) in S,  -w T p_i (1 - Q / P) outside.
+// With e_i = exp((a_i - m) / T), s their sum, s_t the sum outside S, r_j the
+// teacher's exponentials and R their sum, the loss is
+//   w T^2 [ (sum r_j (z_j - z_max - a_j + m) / T + r_t (tail - z_max / T - ln s_t)) / R - ln R + ln s ]:
+// no difference of logarithms of rounded sums but ln s - ln R, both taken in 64 bits.
+
+template <typename C>
+struct RowOut {  // what turns a row's logits into its loss and derivative
+    double loss;
+    C c_top, c_rest, q_scale;  // der1 = q_scale * r_i - c_top * e_i in S, -c_rest * e_i outside
+    bool zero;
+};
+
+template <typename C>
+__device__ __forceinline__ RowOut<C> distill_finish(double w, double t, double s_top, double s_rest, double r_sum,
+                                                    double r_tail, double tail_rel, double cross) {
+    RowOut<C> o{};
+    const double s = s_top + s_rest;
+    o.zero = s == 0.0 || r_sum == 0.0;  // every class masked (m is 0 then), or a teacher without an entry
+    if (o.zero) return o;
+    double kl = cross;
+    if (r_tail > 0.0 || r_tail != r_tail) kl += r_tail * (tail_rel - log(s_rest));
+    o.loss = w * t * t * (kl / r_sum - log(r_sum) + log(s));
+    const double wt = w * t;
+    o.q_scale = (C)(wt / r_sum);
+    o.c_top = (C)(wt / s);
+    const double q = r_tail / r_sum;
+    o.c_rest = (C)(wt * (1.0 / s - (q != 0.0 && s_rest != 0.0 ? q / s_rest : (q != q ? q : 0.0))));
+    return o;
+}
+
+constexpr uint32_t kAbsent32 = 0xffffffffu;  // a NaN no arithmetic gives
+constexpr u64 kAbsent64 = ~0ull;
+__device__ __forceinline__ bool is_absent(float v) { return __float_as_uint(v) == kAbsent32; }
+__device__ __forceinline__ bool is_absent(double v) { return (u64)__double_as_longlong(v) == kAbsent64; }
+__device__ __forceinline__ void set_absent(float* p) { *(uint32_t*)p = kAbsent32; }
+__device__ __forceinline__ void set_absent(double* p) { *(u64*)p = kAbsent64; }
+__device__ __forceinline__ float plain_nan(float v) { return v != v ? __int_as_float(0x7fc00000) : v; }
+__device__ __forceinline__ double plain_nan(double v) {
+    return v != v ? __longlong_as_double(0x7ff8000000000000ll) : v;
+}
+
+// tgt[i] = the teacher's logit of class i, or absent.
+template <typename T, int G>
+__global__ void __launch_bounds__(kLgThreads)
+lg_distill_narrow_kernel(Rows<T> x, TeacherArgs tc, const typename Num<T>::C* __restrict__ tail,
+                         const typename Num<T>::C* __restrict__ weight, double temp, Scale<typename Num<T>::C> sc,
+                         int tile, int pitch, typename Num<T>::C* __restrict__ loss, T* der1, int64_t drs,
+                         int64_t dcs) {
+    typedef typename Num<T>::C C;
+    extern __shared__ __align__(16) unsigned char lg_smem[];
+    C* tgt_all = reinterpret_cast<C*>(lg_smem);
+    T* s = reinterpret_cast<T*>(tgt_all + (size_t)tile * pitch);
+    const int64_t r0 = (int64_t)blockIdx.x * tile;
+    const int rows = (int)(x.n - r0 < tile ? x.n - r0 : tile);
+    const int V = x.V;
+    tile_copy<T, false>(s, pitch, rows, V, const_cast<T*>(x.data) + r0 * x.row_stride, x.row_stride, x.class_stride);
+    __syncthreads();
+    const LaneTeam<G> t;
+    for (int r = threadIdx.x / G; r < rows; r += kLgThreads / G) {
+        T* row = s + (size_t)r * pitch;
+        C* tgt = tgt_all + (size_t)r * pitch;
+        const double w = weight ? (double)weight[r0 + r] : 1.0;
+        for (int i = t.rank; i < V; i += G) set_absent(&tgt[i]);
+        t.sync();
+        for (int j0 = 0; j0 < tc.k && w != 0.0; j0 += G) {
+            const int j = j0 + t.rank;
+            const int64_t at = (r0 + r) * tc.k + j;
+            const int64_t idx = j < tc.k ? tc.idx(at) : -1;
+            bool take = idx >= 0 && idx < V;
+            if (G > 1) {  // of equal indices in this step the first counts
+                const unsigned same = __match_any_sync(t.mask, take ? (int)idx : -1 - t.rank);
+                take = take && (__ffs(same) - 1) == (int)(threadIdx.x & 31);
+            }
+            if (take && is_absent(tgt[idx])) tgt[idx] = plain_nan((C)load_any(tc.value, tc.value_dtype, at));
+            t.sync();
+        }
+        C m = -lg_inf(C()), zm = -lg_inf(C());
+        for (int i = t.rank; i < V; i += G) {
+            m = OpMax()(m, to_c(row[i]));
+            if (!is_absent(tgt[i])) zm = OpMax()(zm, tgt[i]);
+        }
+        m = floor_max(t.reduce(m, OpMax()));
+        zm = t.reduce(zm, OpMax());
+        const double tl = tail ? (double)tail[r0 + r] : -lg_inf(0.0);
+        const double z_max = floor_max(fmax((double)zm * sc.inv_t, tl));
+        double s_top = 0.0, s_rest = 0.0, r_sum = 0.0, cross = 0.0;
+        for (int i = t.rank; i < V; i += G) {
+            const C a = to_c(row[i]);
+            const double e = (double)lg_exp(a - m, sc.c);
+            const C z = tgt[i];
+            if (is_absent(z)) {
+                s_rest += e;
+                continue;
+            }
+            s_top += e;
+            const double d = (double)z * sc.inv_t - z_max;
+            const double rj = exp(d);
+            r_sum += rj;
+            if (rj != 0.0) cross += rj * (d - ((double)a - (double)m) * sc.inv_t);
+        }
+        s_top = t.reduce(s_top, OpSum());
+        s_rest = t.reduce(s_rest, OpSum());
+        r_sum = t.reduce(r_sum, OpSum());
+        cross = t.reduce(cross, OpSum());
+        const double r_tail = exp(tl - z_max);
+        RowOut<C> o = distill_finish<C>(w, temp, s_top, s_rest, r_sum + r_tail, r_tail, tl - z_max, cross);
+        if (w == 0.0) {
+            o = RowOut<C>{};
+            o.zero = true;
+        }
+        if (t.rank == 0) loss[r0 + r] = (C)o.loss;
+        if (der1)
+            for (int i = t.rank; i < V; i += G) {
+                C d = 0;
+                if (!o.zero) {
+                    const C e = lg_exp(to_c(row[i]) - m, sc.c);
+                    const C z = tgt[i];
+                    d = is_absent(z) ? -o.c_rest * e
+                                     : o.q_scale * (C)exp((double)z * sc.inv_t - z_max) - o.c_top * e;
+                }
+                row[i] = from_c<T>(d);
+            }
+    }
+    if (der1) {
+        __syncthreads();
+        tile_copy<T, true>(s, pitch, rows, V, der1 + r0 * drs, drs, dcs);
+    }
+}
+
+// Wide: a block takes the entries whose classes lie in its part of the row (one
+// thread an entry), puts -inf in their place and sums the rest; the blocks
+// of the cluster exchange their maxima and sums once through each other's
+// shared memory, then each writes its part of der1.  der1 may be the logits'
+// own memory: all reads are before the exchange.
+template <typename C>
+struct DistillPart {  // sums relative to the block's own maxima: m of its logits, z of its entries' z / T
+    double s_rest, s_top, r_sum, cross;
+    C m, z;
+};
+
+constexpr int kClaims = 1024;  // places where entries claim their index
+
+template <typename C>
+struct DistillJoin {  // for the second pass, from the joined parts
+    C base, c_rest, q_scale, c_top;  // an entry: der1 = q_scale * r - c_top * e, both relative to this block's maxima
+    bool zero;
+};
+
+__device__ __forceinline__ float part_exp(float x) { return __expf(x); }
+__device__ __forceinline__ double part_exp(double x) { return exp(x); }
+
+// A warp joins the parts, a lane a part.  The second pass waits for this, so it is in C.
+template <typename C>
+__device__ DistillJoin<C> distill_join(const DistillPart<C>& p, int rank, int blocks, C w, C tl, const Scale<C>& sc) {
+    const Base<C> base(floor_max(warp_max(p.m)), sc);
+    const C z_max = floor_max(OpMax()(warp_max(p.z), tl));
+    const C f = Base<C>(floor_max(p.m), sc).shift(base);
+    const C g = part_exp(floor_max(p.z) - z_max), r_tail = part_exp(tl - z_max);
+    const C s_rest = warp_sum(p.s_rest == 0.0 ? C(0) : (C)p.s_rest * f, blocks);
+    const C s = s_rest + warp_sum(p.s_top == 0.0 ? C(0) : (C)p.s_top * f, blocks);
+    const C r_sum = r_tail + warp_sum(p.r_sum == 0.0 ? C(0) : (C)p.r_sum * g, blocks);
+    const C q = r_tail / r_sum, per_s = C(1) / s;
+    DistillJoin<C> j;
+    j.base = base.m;
+    j.zero = s == C(0) || r_sum == C(0);  // every class masked, or a teacher without an entry
+    j.c_rest = w * (q != q ? q : (q != C(0) && s_rest != C(0) ? per_s - q / s_rest : per_s));
+    j.q_scale = __shfl_sync(0xffffffffu, w / r_sum * g, rank);
+    j.c_top = __shfl_sync(0xffffffffu, w * per_s * f, rank);
+    return j;
+}
+
+// The loss from the parts, in 64 bits; nothing waits for it.
+template <typename C>
+__device__ double distill_loss(const DistillPart<C>& p, int blocks, double w, double t, double tl, const Scale<C>& sc) {
+    const Base<C> base(floor_max(warp_max(p.m)), sc);
+    const double z_max = floor_max(fmax((double)warp_max(p.z), tl));
+    const double ln_f = Base<C>(floor_max(p.m), sc).ln_shift(base), f = exp(ln_f);
+    const double ln_g = (double)floor_max(p.z) - z_max, g = exp(ln_g);
+    const double s_rest = warp_sum(p.s_rest == 0.0 ? 0.0 : p.s_rest * f, blocks);
+    const double s_top = warp_sum(p.s_top == 0.0 ? 0.0 : p.s_top * f, blocks);
+    const double r_sum = warp_sum(p.r_sum == 0.0 ? 0.0 : p.r_sum * g, blocks);
+    const double cross = warp_sum(p.r_sum == 0.0 ? 0.0 : g * (p.cross + p.r_sum * (ln_g - ln_f)), blocks);
+    const double r_tail = exp(tl - z_max);
+    return distill_finish<double>(w, t, s_top, s_rest, r_sum + r_tail, r_tail, tl - z_max, cross).loss;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kLgThreads)
+lg_distill_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, TeacherArgs tc, const typename Num<T>::C* __restrict__ tail,
+                       const typename Num<T>::C* __restrict__ weight, double temp, Scale<typename Num<T>::C> sc,
+                       typename Num<T>::C* __restrict__ loss, T* der1, int64_t drs, int64_t dcs) {
+    typedef typename Num<T>::C C;
+    constexpr int VE = WideRow<T>::VE;
+    extern __shared__ __align__(16) unsigned char lg_smem[];
+    __shared__ __align__(16) C red_max[2][kLgWarps];
+    __shared__ union {
+        int claim[kClaims];
+        double red[4][kLgThreads];  // s_rest, s_top, r_sum, cross of every thread
+    } u;
+    __shared__ int s_idx[kLgMaxTop];
+    __shared__ DistillPart<C> parts[16];
+    __shared__ DistillJoin<C> join;
+    __shared__ int s_next;
+    uint4* s = reinterpret_cast<uint4*>(lg_smem);
+    T* se = reinterpret_cast<T*>(s);
+    auto cluster = cooperative_groups::this_cluster();
+    const int rank = (int)cluster.block_rank(), blocks = (int)cluster.num_blocks(), k = tc.k;
+    const int tid = threadIdx.x, lane = tid & 31, warp_id = tid >> 5;
+    const int64_t r = row0 + (int64_t)(blockIdx.x / (unsigned)blocks);
+    const WideRow<T> w(x, r, rank, per);
+    T* out = der1 ? der1 + r * drs : nullptr;
+    // 16-byte stores where der1's row lies to the 16-byte boundaries as the logits' row does
+    const bool vec_out = dcs == 1 && w.cs == 1 && (((uintptr_t)out - (uintptr_t)w.head * sizeof(T)) & 15) == 0;
+    auto put = [&](int v, const C(&d)[VE]) {
+        const int i = w.first(v);
+        for (int j = 0; j < VE; ++j)
+            if (i + j >= 0 && i + j < w.V) out[(int64_t)(i + j) * dcs] = from_c<T>(d[j]);
+    };
+    if (blocks > 1) cluster_arrive<false>();
+
+    static_assert(kLgThreads >= kLgMaxTop, "one thread an entry");
+    // the row's own numbers are asked for before its logits and used after them
+    const C wt = weight ? weight[r] : C(1), tl = tail ? tail[r] : -lg_inf(C());
+    u64 i_bits = 0, z_bits = 0;
+    if (tid < k) {
+        i_bits = tc.idx_bits(r * k + tid);
+        z_bits = load_bits(tc.value, tc.value_dtype, r * k + tid);
+    }
+    if (r + ahead < x.n) {
+        if (tid == kLgThreads - 1) WideRow<T>(x, r + ahead, rank, per).prefetch();
+        if (tid < k && (tid & 15) == 0) tc.prefetch((r + ahead) * k + tid);
+    }
+    for (int i = tid; i < kClaims; i += kLgThreads) u.claim[i] = kLgMaxTop;
+    if (tid == 0) s_next = 0;
+    VecMax<T> most;
+    w.load(s, [&](const uint4& q) { most(q); });
+    if (wt == C(0)) {  // the same for all blocks of the cluster
+        if (tid == 0 && rank == 0) loss[r] = 0;
+        const C zero[VE] = {};
+        if (out)
+            for (int v = tid; v < w.nv; v += kLgThreads) put(v, zero);
+        if (blocks > 1) cluster_wait();
+        return;
+    }
+    const int64_t idx = tid < k ? tc.of_idx_bits(i_bits) : -1;
+    double z = tid < k ? (double)(C)of_bits(z_bits, tc.value_dtype) * sc.inv_t : -lg_inf(0.0);
+    const int own = idx >= 0 && idx < w.V ? (int)idx : -1;  // the class of this thread's entry
+    if (tid < k) s_idx[tid] = own;
+    __syncthreads();
+    int at = own >= 0 ? w.slot(own) : -1;  // its place, if the class is in this block's part
+    if (at >= 0) atomicMin(&u.claim[own % kClaims], tid);
+    __syncthreads();
+    if (warp_id * 32 < k) {
+        // of equal indices the first counts: who holds its claim is the first of its index; for the
+        // others (equal indices, or two that share a claim) the warp looks through the entries before
+        unsigned late = __ballot_sync(0xffffffffu, at >= 0 && u.claim[own % kClaims] != tid);
+        for (; late; late &= late - 1) {
+            const int l = __ffs(late) - 1, who = warp_id * 32 + l;
+            const int mine = __shfl_sync(0xffffffffu, own, l);
+            bool again = false;
+            for (int j = lane; j < who; j += 32) again |= s_idx[j] == mine;
+            if (__any_sync(0xffffffffu, again) && lane == l) at = -1;
+        }
+    }
+    C a_own = -lg_inf(C());
+    if (at >= 0) {
+        a_own = to_c(se[at]);
+        se[at] = from_c<T>(-lg_inf(C()));
+    } else {
+        z = -lg_inf(0.0);
+    }
+    {
+        const C m = warp_max(OpMax()(most.get(), a_own)), zm = warp_id * 32 < k ? warp_max((C)z) : -lg_inf(C());
+        if (lane == 0) red_max[0][warp_id] = m, red_max[1][warp_id] = zm;
+    }
+    __syncthreads();
+    C top[2] = {red_max[0][0], red_max[1][0]};
+#pragma unroll
+    for (int i = 1; i < kLgWarps; ++i) {
+        top[0] = OpMax()(top[0], red_max[0][i]);
+        top[1] = OpMax()(top[1], red_max[1][i]);
+    }
+    const Base<C> here(floor_max(top[0]), sc);
+    const double z_here = (double)floor_max(top[1]);
+
+    double sum[4] = {0.0, 0.0, 0.0, 0.0};  // s_rest, s_top, r_sum, cross
+    auto add = [&](auto huge) {
+#pragma unroll 4
+        for (int v = tid; v < w.nv; v += kLgThreads) {
+            C a[VE];
+            unpack(s[v], a, T());
+            here.template exps<decltype(huge)::value>(a);
+            sum[0] += Base<C>::total(a);
+        }
+    };
+    if (here.huge) add(std::true_type());
+    else add(std::false_type());
+    if (at >= 0) {
+        sum[1] = (double)here.exp(a_own);
+        sum[2] = exp(z - z_here);
+        if (sum[2] != 0.0) sum[3] = sum[2] * (z - z_here - here.ln(a_own));
+    }
+    const double e_own = sum[1], r_own = sum[2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u.red[i][tid] = sum[i];
+    __syncthreads();
+    // a warp for each of the four sums, which it gives to all blocks of the cluster
+    if (blocks > 1) cluster_wait();  // every block runs: its shared memory can be written
+    if (warp_id < 4) {
+        double v = 0.0;
+#pragma unroll
+        for (int i = 0; i < kLgWarps; ++i) v += u.red[warp_id][lane + 32 * i];
+        v = warp_sum(v, 32);
+        if (lane < blocks) {
+            DistillPart<C>* to = cluster.map_shared_rank(&parts[rank], lane);
+            if (warp_id == 0) to->s_rest = v, to->m = top[0], to->z = top[1];
+            else if (warp_id == 1) to->s_top = v;
+            else if (warp_id == 2) to->r_sum = v;
+            else to->cross = v;
+        }
+    }
+    if (blocks > 1) {
+        if (warp_id < 4) cluster_arrive<true>();
+        else cluster_arrive<false>();
+        cluster_wait();
+    } else {
+        __syncthreads();
+    }
+    DistillPart<C> p{0.0, 0.0, 0.0, 0.0, -lg_inf(C()), -lg_inf(C())};
+    if (lane < blocks) p = parts[lane];
+    if (out) {  // one warp works out what the second pass needs
+        if (warp_id == 0) {
+            const DistillJoin<C> j = distill_join<C>(p, rank, blocks, (C)((double)wt * temp), tl, sc);
+            if (lane == 0) join = j;
+        }
+        __syncthreads();
+    }
+    if (warp_id == kLgWarps - 1 && rank == 0) {  // and another the loss, while the others are at the second pass
+        const double v = distill_loss<C>(p, blocks, (double)wt, temp, (double)tl, sc);
+        if (lane == 0) loss[r] = (C)v;
+    }
+    if (!out) return;
+    const Base<C> base(join.base, sc);
+    auto write = [&](auto huge) {
+        const C c = join.zero ? C(0) : -join.c_rest;
+        auto der = [&](int v, C(&a)[VE]) {
+            unpack(s[v], a, T());
+            base.template exps<decltype(huge)::value>(a);
+            Base<C>::times(a, c);
+        };
+        if (vec_out) {
+            uint4* g = reinterpret_cast<uint4*>(out + ((int64_t)w.v0 * VE - w.head));
+            const int lo = w.whole_lo(), hi = w.whole_hi();
+            constexpr int kRun = 4;  // warps take runs of vectors as they come, since one is late by the loss
+            for (;;) {
+                int v = 0;
+                if (lane == 0) v = atomicAdd(&s_next, kRun * 32);
+                v = lo + __shfl_sync(0xffffffffu, v, 0);
+                if (v >= hi) break;
+                v += lane;
+                if (v - lane + kRun * 32 <= hi) {
+#pragma unroll
+                    for (int u = 0; u < kRun; ++u) {
+                        C a[VE];
+                        der(v + 32 * u, a);
+                        __stcs(g + v + 32 * u, pack(a, T()));
+                    }
+                } else {
+                    for (; v < hi; v += 32) {
+                        C a[VE];
+                        der(v, a);
+                        __stcs(g + v, pack(a, T()));
+                    }
+                }
+            }
+            w.ends([&](int v) {
+                C a[VE];
+                der(v, a);
+                put(v, a);
+            });
+        } else {
+            for (int v = tid; v < w.nv; v += kLgThreads) {
+                C a[VE];
+                der(v, a);
+                put(v, a);
+            }
+        }
+    };
+    if (base.huge) write(std::true_type());
+    else write(std::false_type());
+    __syncthreads();  // the entries' classes over the zeros just written
+    if (at >= 0)
+        out[(int64_t)own * dcs] = from_c<T>(join.zero ? C(0) : join.q_scale * (C)r_own - join.c_top * (C)e_own);
+}
+
+template <typename T>
+int run_distill(const cbgpu_logits* x, const cbgpu_teacher* tc, const void* weight, double temp, void* loss, void* der1,
+                int64_t drs, int64_t dcs, cudaStream_t st) {
+    typedef typename Num<T>::C C;
+    const char* who = "distill";
+    const Rows<T> rows = rows_of<T>(x);
+    const Scale<C> sc(temp);
+    const TeacherArgs ta{tc->index, tc->value, tc->index_bytes, tc->value_dtype, tc->k};
+    if (rows.V > kLgNarrow) {
+        const Wide w = wide_shape<T>(rows.n, rows.V);
+        return lg_launch_wide(who, lg_distill_wide_kernel<T>, rows.n, w, w.smem, st, w.ahead, rows, ta, (const C*)tc->tail,
+                              (const C*)weight, temp, sc, (C*)loss, (T*)der1, drs, dcs);
+    }
+    auto narrow = [&](auto kernel, int lanes) {
+        const Tile t =
+            narrow_tile(rows.V, sizeof(T) + sizeof(C), kLgThreads / lanes, rows.class_stride <= rows.row_stride);
+        return lg_launch(who, kernel, tiles_of(rows.n, t.rows), t.smem, st, rows, ta, (const C*)tc->tail,
+                         (const C*)weight, temp, sc, t.rows, t.pitch, (C*)loss, (T*)der1, drs, dcs);
+    };
+    return by_lanes(rows.V, [&] { return narrow(lg_distill_narrow_kernel<T, 1>, 1); },
+                    [&] { return narrow(lg_distill_narrow_kernel<T, 8>, 8); },
+                    [&] { return narrow(lg_distill_narrow_kernel<T, 32>, 32); });
+}
+
+}  // namespace
+
+int cbgpu_distill(const cbgpu_logits* x, const cbgpu_teacher* t, const void* weight, double temperature, void* loss,
+                  void* der1, int64_t der1_row_stride, int64_t der1_class_stride, void* stream) {
+    int rc = check_logits("distill", x);
+    if (rc) return rc;
+    if (!t) return lfail(CBGPU_ERR_INVALID, "distill: teacher is NULL");
+    if (t->k < 1 || t->k > kLgMaxTop)
+        return lfail(CBGPU_ERR_INVALID, "distill: k = %d is outside 1..%d", t->k, kLgMaxTop);
+    if (t->index_bytes != 4 && t->index_bytes != 8)
+        return lfail(CBGPU_ERR_INVALID, "distill: index_bytes must be 4 or 8");
+    if (t->value_dtype < CBGPU_F64 || t->value_dtype > CBGPU_BF16)
+        return lfail(CBGPU_ERR_INVALID, "distill: value_dtype %d is not one of the cbgpu_dtype values", t->value_dtype);
+    if ((rc = check_temperature("distill", temperature, false))) return rc;
+    if (x->n == 0) return CBGPU_OK;
+    if (!t->index || !t->value || !loss) return lfail(CBGPU_ERR_INVALID, "distill: index, value or loss is NULL");
+    if (der1) {
+        const int64_t n = x->n, V = x->n_classes, rs = der1_row_stride, cs = der1_class_stride;
+        if (rs < 0 || cs < 0) return lfail(CBGPU_ERR_INVALID, "distill: negative strides");
+        const bool apart = (n == 1 && V == 1) || (n == 1 && cs >= 1) || (V == 1 && rs >= 1) ||
+                           (cs >= 1 && rs > cs * (V - 1)) || (rs >= 1 && cs > rs * (n - 1));
+        if (!apart) return lfail(CBGPU_ERR_INVALID, "distill: elements of der1 share memory");
+        const size_t es = dtype_size(x->dtype), wide = x->dtype == CBGPU_F64 ? 8 : 4;
+        if ((uintptr_t)der1 % es != 0) return lfail(CBGPU_ERR_INVALID, "distill: der1 is not aligned to its type");
+        const Span d = span_of(der1, es, n, (int)V, rs, cs);
+        const bool same = der1 == x->data && (n == 1 || rs == x->row_stride) && (V == 1 || cs == x->class_stride);
+        if (!same && d.meets(span_of(x->data, es, n, (int)V, x->row_stride, x->class_stride)))
+            return lfail(CBGPU_ERR_INVALID, "distill: der1 overlaps the logits without being them");
+        if (d.meets(span_of(t->index, (size_t)n * t->k * t->index_bytes)) ||
+            d.meets(span_of(t->value, (size_t)n * t->k * dtype_size(t->value_dtype))) ||
+            d.meets(span_of(t->tail, (size_t)n * wide)) || d.meets(span_of(weight, (size_t)n * wide)) ||
+            d.meets(span_of(loss, (size_t)n * wide)))
+            return lfail(CBGPU_ERR_INVALID, "distill: der1 overlaps the teacher, the weights or the loss");
+    }
+    return LG_BY_DTYPE(x->dtype, run_distill, x, t, weight, temperature, loss, der1, der1_row_stride,
+                       der1_class_stride, (cudaStream_t)stream);
+}
+

@@ -517,7 +517,8 @@ CBGPU_API int cbgpu_apply_oblivious(const float* features_fm, int64_t n, int32_t
  * hold no state and share no workspace, so they may overlap on any streams
  * and be captured into graphs.  Arithmetic and the "wide" outputs are f64 for
  * CBGPU_F64 logits and f32 for the other types; sums are taken in 64 bits.
- * Results do not depend on the launch or on timing.
+ * The same call gives the same bits again; rows in another layout may be
+ * summed in another grouping (the last bits of loss, der1 and tail).
  * Classes are ordered by logit, larger first, equal logits (-0 == +0) by
  * lower index, NaN last.  Limits: 1..262144 classes, n < 2^31 rows; n = 0 is
  * a call that does nothing. */
