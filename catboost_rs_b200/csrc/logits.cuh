@@ -459,6 +459,42 @@ struct VecMax<__nv_bfloat16> : PairMax<__nv_bfloat162> {
     __device__ float get() const { return fmaxf(__low2float(m), __high2float(m)); }
 };
 
+// The same, but a NaN stays.
+template <typename T>
+struct VecMaxNan {
+    typename Num<T>::C m = -lg_inf(typename Num<T>::C());
+    __device__ static float both(float a, float b) {
+        float r;
+        asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+        return r;
+    }
+    __device__ static double both(double a, double b) { return a != a ? a : (b != b ? b : fmax(a, b)); }
+    __device__ void operator()(const uint4& q) {
+        typename Num<T>::C a[16 / sizeof(T)];
+        unpack(q, a, T());
+#pragma unroll
+        for (int j = 0; j < 16 / (int)sizeof(T); ++j) m = both(m, a[j]);
+    }
+    __device__ typename Num<T>::C get() const { return m; }
+};
+template <typename H2>
+struct PairMaxNan {
+    H2 m;
+    __device__ void operator()(const uint4& q) {
+        const H2* h = reinterpret_cast<const H2*>(&q);
+        m = __hmax2_nan(m, __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3])));
+    }
+    __device__ float get() const { return VecMaxNan<float>::both(__low2float(m), __high2float(m)); }
+};
+template <>
+struct VecMaxNan<__half> : PairMaxNan<__half2> {
+    __device__ VecMaxNan() { m = __float2half2_rn(-lg_inf(0.0f)); }
+};
+template <>
+struct VecMaxNan<__nv_bfloat16> : PairMaxNan<__nv_bfloat162> {
+    __device__ VecMaxNan() { m = __float2bfloat162_rn(-lg_inf(0.0f)); }
+};
+
 // Two f32 operations in one instruction.
 __device__ __forceinline__ u64 f2(float a, float b) {
     u64 r;
@@ -627,10 +663,21 @@ __device__ __forceinline__ void block_reduce(V (&v)[N], V (*scratch)[kLgWarps], 
 
 constexpr int kTopCap = 1024;  // classes the first block can collect
 
+constexpr int kBins = 1024;    // of the sampler's histogram, which lies where the list comes to lie
+struct SampleHist {
+    float mass[kBins];
+    uint32_t count[kBins];
+};
+
 template <typename Key>
 struct TopShared {
-    Key key[kTopCap];
-    uint32_t idx[kTopCap];
+    union {
+        struct {
+            Key key[kTopCap];
+            uint32_t idx[kTopCap];
+        };
+        SampleHist hist;
+    };
     uint32_t bound[16][2];  // of every block: its k-th and its ceil(k / blocks)-th largest thread maximum
     u64 part[2][16];        // sums that go round the cluster
     u64 warp_part[kLgWarps];
@@ -658,7 +705,20 @@ struct ClusterInfo {
     }
 };
 
-// Sum over the cluster of a value a thread, in every thread.  `turn` alternates between calls.
+// A value of each block's first thread, to sh.part[the turn before][block] of every block.  `turn`
+// alternates between calls.
+template <typename Sh>
+__device__ const u64* cluster_gather(const ClusterInfo& cl, Sh& sh, u64 v, int& turn) {
+    if ((int)threadIdx.x < 32) {
+        v = __shfl_sync(0xffffffffu, v, 0);
+        if ((int)threadIdx.x < cl.blocks) *cl.of(&sh.part[turn][cl.rank], (int)threadIdx.x) = v;
+    }
+    cl.sync();
+    turn ^= 1;
+    return sh.part[turn ^ 1];
+}
+
+// Sum over the cluster of a value a thread, in every thread.
 template <typename Sh>
 __device__ u64 cluster_total(const ClusterInfo& cl, Sh& sh, u64 v, int& turn) {
     v = warp_sum(v, 32);
@@ -748,8 +808,7 @@ __device__ void sort_list(TopShared<Key>& sh, int n) {
 // Collects the row's first k classes, and perhaps some after them, in the
 // first block's list (not sorted; returns how many, in every thread); they are
 // replaced by -inf in the row, and `rest` gets the largest of this thread's classes
-// that stay.  `mine`: the largest of this thread's classes.  The caller has arrived at the
-// cluster's barrier once (cluster_arrive, blocks > 1).
+// that stay.  `mine`: the largest of this thread's classes.  Every block of the cluster runs.
 template <typename T>
 __device__ int wide_top(const ClusterInfo& cl, TopShared<typename Num<T>::Key>& sh, const WideRow<T>& w, uint4* s,
                         typename Num<T>::C mine, int k, int& turn, typename Num<T>::C& rest) {
@@ -767,7 +826,6 @@ __device__ int wide_top(const ClusterInfo& cl, TopShared<typename Num<T>::Key>& 
     if (share == k) bs = bk;
     if (threadIdx.x == 0) sh.count = 0;
     if (cl.blocks > 1) {
-        cluster_wait();  // every block runs: its shared memory can be written
         if ((int)threadIdx.x < cl.blocks) {
             uint32_t* to = cl.of(&sh.bound[cl.rank][0], (int)threadIdx.x);
             to[0] = bk, to[1] = bs;

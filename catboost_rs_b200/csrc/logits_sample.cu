@@ -172,16 +172,387 @@ lg_sample_narrow_kernel(Rows<T> x, SampleArgs a, int shift, int tile, int pitch,
     }
 }
 
+// ---- wide rows -------------------------------------------------------------------------------
+//
+// top-k up to kLgMaxTop: the first block collects the first k classes and does the rest alone.
+// Else each class that can be drawn is weighed once or twice.  Where top-p or a larger
+// top-k cuts, a histogram over the logits (counts, and masses in f32) shows in which bin the cut lies;
+// the bin's classes are collected and sorted, and the cut is then taken with
+// exact masses, which also show whether the bin was the right one.
+
+template <typename T>
+struct Weigh {
+    typedef typename Num<T>::C C;
+    typedef typename Num<T>::Key Key;
+    C m;
+    double inv_t, scale, min_p;
+    Ranked<Key> last;  // the last class that stays
+    bool cut;
+    __device__ double share(C a) const { return a == m ? 1.0 : exp(((double)a - (double)m) * inv_t); }
+    // rint(e 2^s) through the lowest bits of 2^52 + e 2^s
+    __device__ u64 whole(double e) const {
+        return (u64)__double_as_longlong(fma(e, scale, 4503599627370496.0)) - 0x4330000000000000ull;
+    }
+    __device__ u64 mass(C a) const { return whole(share(a)); }
+    __device__ bool stays(int i, C a) const {
+        const Key k = key_of(a);
+        return !cut || k > last.key || (k == last.key && (uint32_t)i <= last.idx);
+    }
+    __device__ u64 operator()(int i, C a) const {
+        if (!stays(i, a)) return 0;
+        const double e = share(a);
+        return e < min_p ? 0 : whole(e);
+    }
+};
+
+constexpr int kSegments = 8192 / 32 + 1;  // of 32 vectors; the largest row's blocks hold 8192
+
+// Exclusive scan of a value a thread over the block.
+__device__ __forceinline__ u64 block_exscan(u64 v, u64 (&warp_part)[kLgWarps]) {
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+    u64 inc = v;
+    for (int o = 1; o < 32; o <<= 1) {
+        const u64 t = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += t;
+    }
+    if (lane == 31) warp_part[wid] = inc;
+    __syncthreads();
+    u64 base = 0;
+    for (int i = 0; i < wid; ++i) base += warp_part[i];
+    __syncthreads();
+    return base + inc - v;
+}
+
+__device__ __forceinline__ u64 block_total(u64 v, u64 (&warp_part)[kLgWarps]) {
+    v = warp_sum(v, 32);
+    if ((threadIdx.x & 31) == 0) warp_part[threadIdx.x >> 5] = v;
+    __syncthreads();
+    u64 t = 0;
+    for (int i = 0; i < kLgWarps; ++i) t += warp_part[i];
+    __syncthreads();
+    return t;
+}
+
+// Draws from the classes that stay; every block of the cluster, one of them writes.
+template <typename T, typename Sh>
+__device__ void wide_draw(const ClusterInfo& cl, Sh& sh, u64* seg, const WideRow<T>& w, const uint4* s,
+                          const Weigh<T>& weigh, double u, int& turn, int32_t* index) {
+    constexpr int VE = WideRow<T>::VE;
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+    auto lane_mass = [&](int v) {
+        u64 own = 0;
+        if (v < w.nv) {
+            typename Num<T>::C a[VE];
+            unpack(s[v], a, T());
+#pragma unroll
+            for (int j = 0; j < VE; ++j) own += weigh(w.first(v) + j, a[j]);
+        }
+        return own;
+    };
+    const int segs = w.nv > 0 ? (w.nv + 31) / 32 : 0;
+    for (int g = wid; g < segs; g += kLgWarps) {
+        const u64 sum = warp_sum(lane_mass(g * 32 + lane), 32);
+        if (lane == 0) seg[g] = sum;
+    }
+    __syncthreads();
+    // a run of segments a thread
+    const int per = (segs + kLgThreads - 1) / kLgThreads, g0 = (int)threadIdx.x * per;
+    u64 own = 0;
+    for (int g = g0; g < g0 + per && g < segs; ++g) own += seg[g];
+    u64 upto = block_exscan(own, sh.warp_part);
+    const u64* of = cluster_gather(cl, sh, block_total(own, sh.warp_part), turn);
+    u64 total = 0, before = 0;
+    for (int b = 0; b < cl.blocks; ++b) {
+        if (b == cl.rank) before = total;
+        total += of[b];
+    }
+    const u64 target = draw_target(u, total);
+    __shared__ int s_seg;
+    __shared__ u64 s_upto;
+    if (threadIdx.x == 0) s_seg = -1;
+    __syncthreads();
+    upto += before;
+    if (upto < target && upto + own >= target)
+        for (int g = g0;; ++g) {
+            if (upto + seg[g] >= target) {
+                s_seg = g, s_upto = upto;
+                break;
+            }
+            upto += seg[g];
+        }
+    __syncthreads();
+    if (s_seg < 0 || wid != 0) return;
+    const int v = s_seg * 32 + lane;
+    const u64 mine = lane_mass(v);
+    u64 inc = mine;
+    for (int o = 1; o < 32; o <<= 1) {
+        const u64 t = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += t;
+    }
+    u64 sum = s_upto + inc - mine;
+    if (sum < target && sum + mine >= target) {
+        typename Num<T>::C a[VE];
+        unpack(s[v], a, T());
+#pragma unroll
+        for (int j = 0; j < VE; ++j) {
+            const u64 next = sum + weigh(w.first(v) + j, a[j]);
+            if (sum < target && next >= target) *index = w.first(v) + j;
+            sum = next;
+        }
+    }
+}
+
+// The draw from the first block's sorted list of k <= kLgThreads classes: a thread a class.
+template <typename T, typename Sh>
+__device__ void list_draw(Sh& sh, int k, const Weigh<T>& weigh, const RowSampling& rs, u64* w_of, int32_t* index) {
+    typedef typename Num<T>::C C;
+    const int j = threadIdx.x;
+    const double e = j < k ? weigh.share((C)of_key(sh.key[j])) : 0.0;
+    u64 own = j < k ? weigh.whole(e) : 0;
+    if (rs.top_p < 1.0) {
+        const u64 before = block_exscan(own, sh.warp_part);
+        if (before >= mass_part(rs.top_p, block_total(own, sh.warp_part))) own = 0;
+    }
+    if (e < rs.min_p) own = 0;
+    const u64 target = draw_target(rs.u, block_total(own, sh.warp_part));
+    w_of[j] = own;
+    __syncthreads();
+    if (own == 0) return;
+    u64 upto = 0;  // of the kept classes before this one by index
+    for (int i = 0; i < k; ++i) upto += sh.idx[i] < sh.idx[j] ? w_of[i] : 0;
+    if (upto < target && upto + own >= target) *index = (int32_t)sh.idx[j];
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kLgThreads)
-lg_sample_wide_kernel(Rows<T> x, SampleArgs a, int shift, int32_t* __restrict__ index) {
-    __shared__ u64 scratch[kLgThreads / 32 + 1];
-    const BlockTeam t(scratch);
-    const int64_t r = blockIdx.x;
-    const T* row = x.data + r * x.row_stride;
-    const int64_t cs = x.class_stride;
-    const int got = sample_row<T>(t, [&](int i) { return row[(int64_t)i * cs]; }, x.V, shift, row_sampling(a, r, x.V));
-    if (t.rank == 0) index[r] = got;
+lg_sample_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, SampleArgs a, int shift,
+                      int32_t* __restrict__ index) {
+    typedef typename Num<T>::C C;
+    typedef typename Num<T>::Key Key;
+    extern __shared__ __align__(16) unsigned char lg_smem[];
+    __shared__ TopShared<Key> sh;
+    __shared__ u64 seg[kSegments];
+    static_assert(kSegments >= kLgThreads, "list_draw's masses");
+    __shared__ C red_max[1][kLgWarps];
+    __shared__ Ranked<Key> s_cut;
+    uint4* s = reinterpret_cast<uint4*>(lg_smem);
+    const ClusterInfo cl;
+    const int tid = threadIdx.x;
+    const int64_t r = row0 + (int64_t)(blockIdx.x / (unsigned)cl.blocks);
+    const WideRow<T> w(x, r, cl.rank, per);
+    if (cl.blocks > 1) cluster_arrive<false>();
+    if (tid == 0 && r + ahead < x.n) WideRow<T>(x, r + ahead, cl.rank, per).prefetch();
+    VecMaxNan<T> most;
+    w.load(s, [&](const uint4& q) { most(q); });
+    const RowSampling rs = row_sampling(a, r, x.V);
+    const C mine = most.get();
+    C m[1] = {mine};
+    block_reduce(m, red_max, [](C p, C q) { return VecMaxNan<C>::both(p, q); });
+    if (cl.blocks > 1) cluster_wait();  // every block runs: its shared memory can be written
+    int turn = 0;
+    {
+        const u64* of = cluster_gather(cl, sh, (u64)__double_as_longlong((double)m[0]), turn);
+        for (int b = 0; b < cl.blocks; ++b) m[0] = VecMaxNan<C>::both(m[0], (C)__longlong_as_double((long long)of[b]));
+    }
+    int32_t* out = index + r;
+    if (m[0] != m[0] || m[0] == -lg_inf(C())) {  // a NaN, or every class masked
+        if (cl.rank == 0 && tid == 0) *out = -1;
+        return;
+    }
+    if (rs.greedy) {
+        uint32_t at = 0xffffffffu;
+        each_class(w, s, [&](int i, C v, int) { at = v == m[0] && (uint32_t)i < at ? (uint32_t)i : at; });
+        at = __reduce_min_sync(0xffffffffu, at);
+        if (tid == 0) sh.count = 0x7fffffff;
+        __syncthreads();
+        if ((tid & 31) == 0) atomicMin(&sh.count, (int)(at & 0x7fffffffu));
+        __syncthreads();
+        const u64* of = cluster_gather(cl, sh, (u64)sh.count, turn);
+        u64 first = of[0];
+        for (int b = 1; b < cl.blocks; ++b) first = first < of[b] ? first : of[b];
+        if (cl.rank == 0 && tid == 0) *out = (int32_t)first;
+        return;
+    }
+    Weigh<T> weigh{m[0], rs.inv_t, __longlong_as_double((long long)(1023 + shift) << 52), 0.0,
+                   Ranked<Key>{0, 0xffffffffu}, false};
+    if (rs.top_k <= kLgMaxTop) {
+        C rest;
+        const int n = wide_top(cl, sh, w, s, mine, rs.top_k, turn, rest);
+        if (cl.blocks > 1) cl.sync();  // no block leaves while another reads its shared memory
+        if (cl.rank != 0) return;
+        __syncthreads();
+        sort_list(sh, n);
+        list_draw<T>(sh, rs.top_k, weigh, rs, seg, out);
+        return;
+    }
+    if (rs.top_k < x.V || rs.top_p < 1.0) {
+        const bool by_count = rs.top_k < x.V, by_mass = rs.top_p < 1.0;
+        // behind it a weight is below a quarter of the last bit: 0
+        const float reach = (float)((double)(shift + 2) * 0.6931471805599453 / rs.inv_t);
+        C low = lg_inf(C());
+        each_class(w, s, [&](int, C v, int) { low = v < low && v != -lg_inf(C()) ? v : low; });
+        C neg[1] = {-low};
+        block_reduce(neg, red_max, OpMax());
+        {
+            const u64* of = cluster_gather(cl, sh, (u64)__double_as_longlong((double)neg[0]), turn);
+            for (int b = 0; b < cl.blocks; ++b) neg[0] = OpMax()(neg[0], (C)__longlong_as_double((long long)of[b]));
+        }
+        const float range = fminf((float)(m[0] + neg[0]), reach);
+        const float per_bin = range > 0.0f && range < lg_inf(0.0f) ? (float)(kBins - 1) / range : 0.0f;
+        auto bin_of = [&](C v) {  // larger logits have lower bins
+            const float d = v == m[0] ? 0.0f : (float)(m[0] - v) * per_bin;
+            return d < (float)(kBins - 1) ? (int)d : kBins - 1;
+        };
+        for (int i = tid; i < kBins; i += kLgThreads) sh.hist.mass[i] = 0.0f, sh.hist.count[i] = 0u;
+        __syncthreads();
+        const float c = (float)(rs.inv_t * 1.4426950408889634);
+        each_class(w, s, [&](int, C v, int) {
+            const int b = bin_of(v);
+            if (by_mass) atomicAdd(&sh.hist.mass[b], v == m[0] ? 1.0f : ex2((float)(v - m[0]) * c));
+            if (by_count) atomicAdd(&sh.hist.count[b], 1u);
+        });
+        cl.sync();
+        // every thread sums kBins / kLgThreads bins over the blocks, in the blocks' order
+        constexpr int kPer = kBins / kLgThreads;
+        double mass_own = 0.0, mass_bin[kPer];
+        u64 count_own = 0, count_bin[kPer];
+        for (int j = 0; j < kPer; ++j) {
+            float f = 0.0f;
+            u64 n = 0;
+            for (int b = 0; b < cl.blocks; ++b) {
+                const SampleHist* h = cl.of(&sh.hist, b);
+                f += h->mass[tid * kPer + j];
+                n += h->count[tid * kPer + j];
+            }
+            mass_bin[j] = (double)f, mass_own += mass_bin[j];
+            count_bin[j] = n, count_own += n;
+        }
+        // masses as integers: the scan below serves both (rounded alike in every block)
+        u64 mass_int = (u64)(mass_own * 1048576.0);
+        const u64 mass_upto = block_exscan(mass_int, sh.warp_part), count_upto = block_exscan(count_own, sh.warp_part);
+        cl.sync();  // the histograms are read: the list can take their place
+        __shared__ int s_bin;
+        __shared__ u64 s_above, s_mass;
+        auto push = [&](int i, C v) {
+            TopShared<Key>* first = cl.of(&sh, 0);
+            const int p = atomicAdd(&first->count, 1);
+            if (p < kTopCap) first->key[p] = key_of(v), first->idx[p] = (uint32_t)i;
+        };
+        auto restart = [&] {  // an empty list; also ends what read the last one
+            if (cl.rank == 0 && tid == 0) sh.count = 0;
+            cl.sync();
+        };
+        auto give_cut = [&](const Ranked<Key>& cut) {  // by one thread of the first block
+            for (int b = 0; b < cl.blocks; ++b) *cl.of(&s_cut, b) = cut;
+        };
+        if (by_count) {
+            const u64 k = (u64)rs.top_k;
+            if (count_upto < k && count_upto + count_own >= k) {
+                u64 above = count_upto;
+                int j = 0;
+                while (above + count_bin[j] < k) above += count_bin[j++];
+                double upto = (double)mass_upto;
+                for (int i = 0; i <= j; ++i) upto += mass_bin[i] * 1048576.0;
+                s_bin = tid * kPer + j, s_above = above, s_mass = (u64)upto;
+            }
+            __syncthreads();
+            const int bin = s_bin;
+            const u64 above = s_above;
+            weigh.cut = bin < kBins - 1 || range < reach;  // else what is cut weighs nothing
+            restart();
+            if (weigh.cut)
+                each_class(w, s, [&](int i, C v, int) {
+                    if (bin_of(v) == bin) push(i, v);
+                });
+            cl.sync();
+            const int n = cl.of(&sh, 0)->count;
+            if (!weigh.cut) {
+            } else if (n <= kTopCap) {
+                if (cl.rank == 0) {
+                    sort_list(sh, n);
+                    const int j = (int)(k - above) - 1;
+                    if (tid == 0) give_cut(Ranked<Key>{sh.key[j], sh.idx[j]});
+                }
+                cl.sync();
+                weigh.last = s_cut;
+            } else {
+                weigh.last = cluster_select(cl, sh, w, s, k, turn, [](int, C, Key) { return 1ull; });
+            }
+        }
+        if (by_mass) {
+            __syncthreads();
+            if (!by_count && tid == kLgThreads - 1) s_mass = mass_upto + mass_int;
+            if (tid == 0) s_bin = 0;
+            __syncthreads();
+            {
+                const u64 goal = (u64)(rs.top_p * (double)s_mass);
+                if (mass_upto < goal && mass_upto + mass_int >= goal) {
+                    double upto = (double)mass_upto;
+                    int j = 0;
+                    while (j + 1 < kPer && upto + mass_bin[j] * 1048576.0 < (double)goal) upto += mass_bin[j++] * 1048576.0;
+                    s_bin = tid * kPer + j;
+                }
+            }
+            __syncthreads();
+            int bin = s_bin, lo = -1, hi = kBins, step = 1;  // the cut's bin is in (lo, hi)
+            for (;;) {
+                restart();
+                u64 above = 0, within = 0, total = 0;
+                each_class(w, s, [&](int i, C v, int) {
+                    if (!weigh.stays(i, v)) return;
+                    const u64 f = weigh.mass(v);
+                    const int b = bin_of(v);
+                    total += f;
+                    above += b < bin ? f : 0;
+                    if (b == bin) {
+                        within += f;
+                        push(i, v);
+                    }
+                });
+                total = cluster_total(cl, sh, total, turn);
+                above = cluster_total(cl, sh, above, turn);
+                within = cluster_total(cl, sh, within, turn);
+                const u64 goal = mass_part(rs.top_p, total);
+                if (above >= goal || above + within < goal) {  // the f32 masses were a little off: a bin near
+                    if (above >= goal) hi = bin, bin = bin - step > lo ? bin - step : lo + 1;
+                    else lo = bin, bin = bin + step < hi ? bin + step : hi - 1;
+                    step *= 2;
+                    continue;
+                }
+                const int n = cl.of(&sh, 0)->count;
+                Ranked<Key> last;
+                if (n <= kTopCap) {
+                    if (cl.rank == 0) {
+                        sort_list(sh, n);
+                        // a run of the list a thread
+                        const int run = (n + kLgThreads - 1) / kLgThreads, j0 = tid * run;
+                        u64 own = 0;
+                        for (int j = j0; j < j0 + run && j < n; ++j) own += weigh.mass((C)of_key(sh.key[j]));
+                        u64 upto = above + block_exscan(own, sh.warp_part);
+                        if (upto < goal && upto + own >= goal)
+                            for (int j = j0;; ++j) {
+                                upto += weigh.mass((C)of_key(sh.key[j]));
+                                if (upto >= goal) {
+                                    give_cut(Ranked<Key>{sh.key[j], sh.idx[j]});
+                                    break;
+                                }
+                            }
+                    }
+                    cl.sync();
+                    last = s_cut;
+                } else {
+                    last = cluster_select(cl, sh, w, s, goal, turn, [&](int i, C v, Key) {
+                        return weigh.stays(i, v) ? weigh.mass(v) : 0ull;
+                    });
+                }
+                weigh.last = last;
+                weigh.cut = true;
+                break;
+            }
+        }
+    }
+    weigh.min_p = rs.min_p;
+    wide_draw(cl, sh, seg, w, s, weigh, rs.u, turn, out);
 }
 
 template <typename T>
@@ -193,8 +564,10 @@ int run_sample(const cbgpu_logits* x, const cbgpu_sampling* s, int32_t* index, c
     int bits = 0;
     while ((1 << bits) < rows.V) ++bits;
     const int shift = bits < 10 ? 52 : 62 - bits;  // at most what a 64-bit exponential holds
-    if (rows.V > kLgNarrow)
-        return lg_launch(who, lg_sample_wide_kernel<T>, (unsigned)rows.n, 0, st, rows, a, shift, index);
+    if (rows.V > kLgNarrow) {
+        const Wide w = wide_shape<T>(rows.n, rows.V);
+        return lg_launch_wide(who, lg_sample_wide_kernel<T>, rows.n, w, w.smem, st, w.ahead, rows, a, shift, index);
+    }
     auto narrow = [&](auto kernel, int lanes) {
         const Tile t = narrow_tile(rows.V, sizeof(T), kLgThreads / lanes, rows.class_stride <= rows.row_stride);
         return lg_launch(who, kernel, tiles_of(rows.n, t.rows), t.smem, st, rows, a, shift, t.rows, t.pitch, index);

@@ -94,6 +94,7 @@ lg_top_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, int k, Scale
     if (tid == 0 && r + ahead < x.n) WideRow<T>(x, r + ahead, cl.rank, per).prefetch();
     VecMax<T> most;
     w.load(s, [&](const uint4& q) { most(q); });
+    if (cl.blocks > 1) cluster_wait();  // every block runs
     int turn = 0;
     C rest;
     const int n = wide_top(cl, sh, w, s, most.get(), k, turn, rest);
