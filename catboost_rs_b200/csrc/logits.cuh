@@ -55,11 +55,25 @@ template <typename T>
 struct Num {  // 16- and 32-bit logits: arithmetic in f32, 32-bit order keys
     typedef float C;
     typedef uint32_t Key;
+    static constexpr int kKeyDrop = 0;  // low bits of a key that say nothing
+};
+template <>
+struct Num<__half> {
+    typedef float C;
+    typedef uint32_t Key;
+    static constexpr int kKeyDrop = 13;
+};
+template <>
+struct Num<__nv_bfloat16> {
+    typedef float C;
+    typedef uint32_t Key;
+    static constexpr int kKeyDrop = 16;
 };
 template <>
 struct Num<double> {
     typedef double C;
     typedef u64 Key;
+    static constexpr int kKeyDrop = 0;
 };
 
 __device__ __forceinline__ double to_c(double v) { return v; }
@@ -169,38 +183,10 @@ struct LaneTeam {
     }
 };
 
-struct BlockTeam {  // a whole block of kLgThreads
-    static constexpr int size = kLgThreads;
-    int rank;
-    u64* scratch;  // [kLgThreads / 32 + 1]
-    __device__ explicit BlockTeam(u64* s) : rank(threadIdx.x), scratch(s) {}
-    __device__ void sync() const { __syncthreads(); }
-    template <typename V, typename Op>
-    __device__ V reduce(V v, Op op) const {
-        static_assert(sizeof(V) <= sizeof(u64), "scratch word");
-        V* s = reinterpret_cast<V*>(scratch);
-        for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
-        if ((rank & 31) == 0) s[rank >> 5] = v;
-        __syncthreads();
-        V r = s[0];
-        for (int w = 1; w < size / 32; ++w) r = op(r, s[w]);
-        __syncthreads();
-        return r;
-    }
-    __device__ u64 exscan(u64 v) const {
-        u64 inc = v;
-        for (int o = 1; o < 32; o <<= 1) {
-            const u64 t = __shfl_up_sync(0xffffffffu, inc, o);
-            if ((rank & 31) >= o) inc += t;
-        }
-        if ((rank & 31) == 31) scratch[rank >> 5] = inc;
-        __syncthreads();
-        u64 base = 0;
-        for (int w = 0; w < (rank >> 5); ++w) base += scratch[w];
-        __syncthreads();
-        return base + inc - v;
-    }
-};
+template <int G>
+__device__ __forceinline__ int team_count(const LaneTeam<G>& t, int v) {
+    return G == 32 ? (int)__reduce_add_sync(0xffffffffu, (unsigned)v) : t.reduce(v, OpSum());
+}
 
 // ---- launch arguments ----------------------------------------------------------
 
@@ -250,27 +236,72 @@ struct SampleArgs {
     const int32_t* top_k_rows;
 };
 
-// Rows staged as [rows][V] in shared memory, `pitch` elements apart.  The
-// loop runs along the axis that is closer in memory.
-template <typename T, bool kStore>
-__device__ __forceinline__ void tile_copy(T* s, int pitch, int rows, int V, T* g, int64_t rs, int64_t cs) {
-    const uint32_t total = (uint32_t)rows * (uint32_t)V;
-    if (cs <= rs) {
-        for (uint32_t e = threadIdx.x; e < total; e += blockDim.x) {
-            const uint32_t r = e / (uint32_t)V, c = e - r * (uint32_t)V;
-            if (kStore) g[(int64_t)r * rs + (int64_t)c * cs] = s[r * pitch + c];
-            else s[r * pitch + c] = g[(int64_t)r * rs + (int64_t)c * cs];
+// ---- narrow rows ------------------------------------------------------------------------------
+//
+// A block stages a tile of rows in shared memory, `pitch` elements apart, and
+// gives each row to a team of G lanes; lane `rank` holds the classes
+// [rank * per, rank * per + per), per <= ITEMS, in registers.  G = 1 for up to 16 classes
+// (a booster's), 8 up to 128, 32 up to kLgNarrow: a lane then has work for each
+// instruction of a reduction over its team.  Rows that a thread has to itself and that lie class
+// by class in memory are read straight from there.
+template <typename T>
+struct TileIo {
+    int64_t rs, cs;
+    int V, rows, pitch;
+    bool flat;  // the tile is one run of memory: copied by 16 bytes
+    int shift;  // elements of shared memory before the first row, so that both sides lie alike to 16 bytes
+    __device__ TileIo(const T* g, int64_t rs_, int64_t cs_, int V_, int rows_)
+        : rs(rs_), cs(cs_), V(V_), rows(rows_) {
+        flat = (cs == 1 || V == 1) && rs == V;
+        pitch = flat ? V : (V | 1);
+        shift = flat ? (int)(((uintptr_t)g & 15) / sizeof(T)) : 0;
+    }
+    template <bool kStore>
+    __device__ void copy(T* s, T* g) const {
+        const uint32_t total = (uint32_t)rows * (uint32_t)V;
+        if (flat && (((uintptr_t)g ^ (uintptr_t)s) & 15) == 0) {
+            constexpr uint32_t VE = 16 / sizeof(T);
+            uint32_t head = (uint32_t)((16 - ((uintptr_t)g & 15)) & 15) / (uint32_t)sizeof(T);
+            head = head < total ? head : total;
+            const uint32_t vectors = (total - head) / VE, tail = head + vectors * VE;
+            uint4* gv = reinterpret_cast<uint4*>(g + head);
+            uint4* sv = reinterpret_cast<uint4*>(s + head);
+#pragma unroll 4
+            for (uint32_t v = threadIdx.x; v < vectors; v += kLgThreads) {
+                if (kStore) __stcs(gv + v, sv[v]);
+                else sv[v] = __ldcs(gv + v);
+            }
+            const uint32_t e = threadIdx.x < head ? threadIdx.x : tail + threadIdx.x - head;
+            if (threadIdx.x < head || e < total) {
+                if (kStore) g[e] = s[e];
+                else s[e] = g[e];
+            }
+            return;
         }
-    } else {
-        for (uint32_t e = threadIdx.x; e < total; e += blockDim.x) {
-            const uint32_t c = e / (uint32_t)rows, r = e - c * (uint32_t)rows;
-            if (kStore) g[(int64_t)r * rs + (int64_t)c * cs] = s[r * pitch + c];
-            else s[r * pitch + c] = g[(int64_t)r * rs + (int64_t)c * cs];
+        // along the axis that is closer in memory
+        const uint32_t inner = cs <= rs ? (uint32_t)V : (uint32_t)rows;
+        for (uint32_t e = threadIdx.x; e < total; e += kLgThreads) {
+            const uint32_t o = e / inner, i = e - o * inner;
+            const uint32_t r = cs <= rs ? o : i, c = cs <= rs ? i : o;
+            T* at = g + (int64_t)r * rs + (int64_t)c * cs;
+            if (kStore) *at = s[r * pitch + c];
+            else s[r * pitch + c] = *at;
         }
     }
-}
+};
 
-// ---- top logits ------------------------------------------------------------------
+// A lane's classes.
+template <int G, int ITEMS>
+struct Items {
+    int first, count;
+    template <typename Team>
+    __device__ Items(const Team& t, int V) {
+        const int per = (V + G - 1) / G;
+        first = t.rank * per;
+        count = V - first < per ? V - first : per;
+    }
+    __device__ bool has(int it) const { return it < count; }
+};
 
 template <typename Key>
 struct Ranked {  // a class in the operators' order
@@ -919,24 +950,20 @@ Rows<T> rows_of(const cbgpu_logits* x) {
 }
 
 struct Tile {
-    int rows, pitch;
+    int rows;
     size_t smem;
 };
-// Rows a narrow block stages: about 32 KB, at least one for each lane team.
-Tile narrow_tile(int V, size_t bytes_a_class, int teams, bool by_rows) {
-    Tile t;
-    t.pitch = by_rows ? V : (V | 1);  // an odd pitch for rows that are written class by class
-    const size_t row = (size_t)t.pitch * bytes_a_class;
-    size_t rows = 32768 / row;
+// Rows a narrow block stages: about 24 KB (8 blocks an SM), at least one for each lane team.
+Tile narrow_tile(int V, size_t bytes_a_class, int teams) {
+    const size_t row = (size_t)(V | 1) * bytes_a_class;
+    size_t rows = 24576 / row;
     rows = rows < (size_t)teams ? (size_t)teams : rows / teams * teams;
-    t.rows = (int)rows;
-    t.smem = (rows * row + 15) / 16 * 16;
-    return t;
+    return Tile{(int)rows, rows * row + 32};
 }
 
 template <typename K, typename... A>
 int lg_launch(const char* who, K kernel, unsigned grid, size_t smem, cudaStream_t st, A... args) {
-    if (smem > 48 * 1024) {
+    if (smem > 20 * 1024) {  // with the kernels' static arrays (up to 25 KB) above the 48 KB that need no asking
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return lfail(CBGPU_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
     }
@@ -998,12 +1025,6 @@ int lg_launch_wide(const char* who, K kernel, int64_t n, const Wide& w, size_t s
         return lfail(CBGPU_ERR_CUDA, "%s: launch failed: %s", who, cudaGetErrorString(e));
     }
     return CBGPU_OK;
-}
-
-// Lanes a narrow row: 1 up to 12 classes, 8 up to 128, else a warp.
-template <typename F1, typename F8, typename F32>
-int by_lanes(int V, F1 f1, F8 f8, F32 f32) {
-    return V <= 12 ? f1() : (V <= 128 ? f8() : f32());
 }
 
 unsigned tiles_of(int64_t n, int rows) { return (unsigned)((n + rows - 1) / rows); }

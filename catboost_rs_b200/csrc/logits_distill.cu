@@ -44,6 +44,9 @@ __device__ __forceinline__ RowOut<C> distill_finish(double w, double t, double s
     return o;
 }
 
+__device__ __forceinline__ float part_exp(float x) { return __expf(x); }
+__device__ __forceinline__ double part_exp(double x) { return exp(x); }
+
 constexpr uint32_t kAbsent32 = 0xffffffffu;  // a NaN no arithmetic gives
 constexpr u64 kAbsent64 = ~0ull;
 __device__ __forceinline__ bool is_absent(float v) { return __float_as_uint(v) == kAbsent32; }
@@ -55,30 +58,47 @@ __device__ __forceinline__ double plain_nan(double v) {
     return v != v ? __longlong_as_double(0x7ff8000000000000ll) : v;
 }
 
-// tgt[i] = the teacher's logit of class i, or absent.
-template <typename T, int G>
+// Narrow rows: the student's exponentials stay in registers; tgt[i] = the
+// teacher's logit of class i, or absent, and then its exponential.
+template <typename T, int G, int ITEMS>
 __global__ void __launch_bounds__(kLgThreads)
 lg_distill_narrow_kernel(Rows<T> x, TeacherArgs tc, const typename Num<T>::C* __restrict__ tail,
                          const typename Num<T>::C* __restrict__ weight, double temp, Scale<typename Num<T>::C> sc,
-                         int tile, int pitch, typename Num<T>::C* __restrict__ loss, T* der1, int64_t drs,
+                         int tile, int direct, typename Num<T>::C* __restrict__ loss, T* der1, int64_t drs,
                          int64_t dcs) {
     typedef typename Num<T>::C C;
     extern __shared__ __align__(16) unsigned char lg_smem[];
-    C* tgt_all = reinterpret_cast<C*>(lg_smem);
-    T* s = reinterpret_cast<T*>(tgt_all + (size_t)tile * pitch);
     const int64_t r0 = (int64_t)blockIdx.x * tile;
-    const int rows = (int)(x.n - r0 < tile ? x.n - r0 : tile);
-    const int V = x.V;
-    tile_copy<T, false>(s, pitch, rows, V, const_cast<T*>(x.data) + r0 * x.row_stride, x.row_stride, x.class_stride);
-    __syncthreads();
+    const int rows = (int)(x.n - r0 < tile ? x.n - r0 : tile), V = x.V;
+    const int tgt_pitch = V | 1;
+    C* tgt_all = reinterpret_cast<C*>(lg_smem);
+    T* g = const_cast<T*>(x.data) + r0 * x.row_stride;
+    const TileIo<T> io(g, x.row_stride, x.class_stride, V, rows);
+    T* s = reinterpret_cast<T*>(lg_smem + ((size_t)tile * tgt_pitch * sizeof(C) + 15) / 16 * 16) + io.shift;
+    if (!direct) {
+        io.template copy<false>(s, g);
+        __syncthreads();
+    }
     const LaneTeam<G> t;
+    const Items<G, ITEMS> mine(t, V);
     for (int r = threadIdx.x / G; r < rows; r += kLgThreads / G) {
-        T* row = s + (size_t)r * pitch;
-        C* tgt = tgt_all + (size_t)r * pitch;
+        T* row = s + (size_t)r * io.pitch;
+        C* tgt = tgt_all + (size_t)r * tgt_pitch;
+        C a[ITEMS];
+        if (direct) {
+            const T* from = g + r * x.row_stride;
+#pragma unroll
+            for (int it = 0; it < ITEMS; ++it)
+                a[it] = mine.has(it) ? to_c(from[(int64_t)(mine.first + it) * x.class_stride]) : -lg_inf(C());
+        } else {
+#pragma unroll
+            for (int it = 0; it < ITEMS; ++it) a[it] = mine.has(it) ? to_c(row[mine.first + it]) : -lg_inf(C());
+        }
         const double w = weight ? (double)weight[r0 + r] : 1.0;
+        const double tl = tail ? (double)tail[r0 + r] : -lg_inf(0.0);
         for (int i = t.rank; i < V; i += G) set_absent(&tgt[i]);
         t.sync();
-        for (int j0 = 0; j0 < tc.k && w != 0.0; j0 += G) {
+        for (int j0 = 0; j0 < tc.k; j0 += G) {
             const int j = j0 + t.rank;
             const int64_t at = (r0 + r) * tc.k + j;
             const int64_t idx = j < tc.k ? tc.idx(at) : -1;
@@ -91,31 +111,35 @@ lg_distill_narrow_kernel(Rows<T> x, TeacherArgs tc, const typename Num<T>::C* __
             t.sync();
         }
         C m = -lg_inf(C()), zm = -lg_inf(C());
-        for (int i = t.rank; i < V; i += G) {
-            m = OpMax()(m, to_c(row[i]));
-            if (!is_absent(tgt[i])) zm = OpMax()(zm, tgt[i]);
+        uint32_t top = 0;  // which of this lane's classes are entries
+#pragma unroll
+        for (int it = 0; it < ITEMS; ++it) {
+            m = OpMax()(m, a[it]);
+            if (!mine.has(it)) continue;
+            const C z = tgt[mine.first + it];
+            if (!is_absent(z)) top |= 1u << it, zm = OpMax()(zm, z);
         }
         m = floor_max(t.reduce(m, OpMax()));
         zm = t.reduce(zm, OpMax());
-        const double tl = tail ? (double)tail[r0 + r] : -lg_inf(0.0);
         const double z_max = floor_max(fmax((double)zm * sc.inv_t, tl));
-        double s_top = 0.0, s_rest = 0.0, r_sum = 0.0, cross = 0.0;
-        for (int i = t.rank; i < V; i += G) {
-            const C a = to_c(row[i]);
-            const double e = (double)lg_exp(a - m, sc.c);
-            const C z = tgt[i];
-            if (is_absent(z)) {
-                s_rest += e;
-                continue;
+        C sum_top = 0, sum_rest = 0;
+        double r_sum = 0.0, cross = 0.0;
+#pragma unroll
+        for (int it = 0; it < ITEMS; ++it) {
+            const C e = lg_exp(a[it] - m, sc.c);
+            if ((top >> it) & 1) {
+                sum_top += e;
+                const double d = (double)tgt[mine.first + it] * sc.inv_t - z_max;
+                const double rj = (double)part_exp((C)d);
+                r_sum += rj;
+                if (rj != 0.0) cross += rj * (d - ((double)a[it] - (double)m) * sc.inv_t);
+                tgt[mine.first + it] = (C)rj;
+            } else {
+                sum_rest += e;
             }
-            s_top += e;
-            const double d = (double)z * sc.inv_t - z_max;
-            const double rj = exp(d);
-            r_sum += rj;
-            if (rj != 0.0) cross += rj * (d - ((double)a - (double)m) * sc.inv_t);
+            a[it] = e;
         }
-        s_top = t.reduce(s_top, OpSum());
-        s_rest = t.reduce(s_rest, OpSum());
+        const double s_top = t.reduce((double)sum_top, OpSum()), s_rest = t.reduce((double)sum_rest, OpSum());
         r_sum = t.reduce(r_sum, OpSum());
         cross = t.reduce(cross, OpSum());
         const double r_tail = exp(tl - z_max);
@@ -125,21 +149,23 @@ lg_distill_narrow_kernel(Rows<T> x, TeacherArgs tc, const typename Num<T>::C* __
             o.zero = true;
         }
         if (t.rank == 0) loss[r0 + r] = (C)o.loss;
-        if (der1)
-            for (int i = t.rank; i < V; i += G) {
-                C d = 0;
-                if (!o.zero) {
-                    const C e = lg_exp(to_c(row[i]) - m, sc.c);
-                    const C z = tgt[i];
-                    d = is_absent(z) ? -o.c_rest * e
-                                     : o.q_scale * (C)exp((double)z * sc.inv_t - z_max) - o.c_top * e;
-                }
-                row[i] = from_c<T>(d);
-            }
+        if (!der1) continue;
+#pragma unroll
+        for (int it = 0; it < ITEMS; ++it) {
+            if (!mine.has(it)) continue;
+            C d = C(0);
+            if (!o.zero)
+                d = (top >> it) & 1 ? o.q_scale * tgt[mine.first + it] - o.c_top * a[it] : -o.c_rest * a[it];
+            if (direct) der1[(r0 + r) * drs + (int64_t)(mine.first + it) * dcs] = from_c<T>(d);
+            else row[mine.first + it] = from_c<T>(d);
+        }
     }
-    if (der1) {
+    if (der1 && !direct) {
         __syncthreads();
-        tile_copy<T, true>(s, pitch, rows, V, der1 + r0 * drs, drs, dcs);
+        TileIo<T> to = io;
+        to.rs = drs, to.cs = dcs;
+        to.flat = io.flat && (dcs == 1 || V == 1) && drs == V;
+        to.template copy<true>(s, der1 + r0 * drs);
     }
 }
 
@@ -161,9 +187,6 @@ struct DistillJoin {  // for the second pass, from the joined parts
     C base, c_rest, q_scale, c_top;  // an entry: der1 = q_scale * r - c_top * e, both relative to this block's maxima
     bool zero;
 };
-
-__device__ __forceinline__ float part_exp(float x) { return __expf(x); }
-__device__ __forceinline__ double part_exp(double x) { return exp(x); }
 
 // A warp joins the parts, a lane a part.  The second pass waits for this, so it is in C.
 template <typename C>
@@ -423,14 +446,16 @@ int run_distill(const cbgpu_logits* x, const cbgpu_teacher* tc, const void* weig
                               (const C*)weight, temp, sc, (C*)loss, (T*)der1, drs, dcs);
     }
     auto narrow = [&](auto kernel, int lanes) {
-        const Tile t =
-            narrow_tile(rows.V, sizeof(T) + sizeof(C), kLgThreads / lanes, rows.class_stride <= rows.row_stride);
+        const bool direct = lanes == 1 && rows.class_stride > rows.row_stride && (!der1 || dcs > drs);
+        Tile t = narrow_tile(rows.V, sizeof(T) + sizeof(C), kLgThreads / lanes);
+        if (direct) t = Tile{kLgThreads, (size_t)kLgThreads * (rows.V | 1) * sizeof(C) + 16};
         return lg_launch(who, kernel, tiles_of(rows.n, t.rows), t.smem, st, rows, ta, (const C*)tc->tail,
-                         (const C*)weight, temp, sc, t.rows, t.pitch, (C*)loss, (T*)der1, drs, dcs);
+                         (const C*)weight, temp, sc, t.rows, (int)direct, (C*)loss, (T*)der1, drs, dcs);
     };
-    return by_lanes(rows.V, [&] { return narrow(lg_distill_narrow_kernel<T, 1>, 1); },
-                    [&] { return narrow(lg_distill_narrow_kernel<T, 8>, 8); },
-                    [&] { return narrow(lg_distill_narrow_kernel<T, 32>, 32); });
+    if (rows.V <= 8) return narrow(lg_distill_narrow_kernel<T, 1, 8>, 1);
+    if (rows.V <= 16) return narrow(lg_distill_narrow_kernel<T, 1, 16>, 1);
+    if (rows.V <= 128) return narrow(lg_distill_narrow_kernel<T, 8, 16>, 8);
+    return narrow(lg_distill_narrow_kernel<T, 32, 32>, 32);
 }
 
 }  // namespace

@@ -55,119 +55,149 @@ __device__ __forceinline__ u64 draw_target(double u, u64 total) {
     return (down >= 64 ? hi >> (down - 64) : (hi << (64 - down)) | (lo >> down)) + 1ull;
 }
 
-// The last class of the shortest prefix (in order) whose metric reaches
-// `target`: bit by bit the largest key that still reaches it, then the
-// lowest index among that key's classes.  metric(i, key) is 0 for what is out already.
-template <typename Key, typename Team, typename Met, typename KeyAt>
-__device__ Ranked<Key> team_select(const Team& t, int V, u64 target, KeyAt key_at, Met metric) {
-    Key key = 0;
-    for (int b = (int)sizeof(Key) * 8 - 1; b >= 0; --b) {
-        const Key cand = key | ((Key)1 << b);
-        u64 f = 0;
-        for (int i = t.rank; i < V; i += t.size) {
-            const Key ki = key_at(i);
-            if (ki >= cand) f += metric(i, ki);
-        }
-        if (t.reduce(f, OpSum()) >= target) key = cand;
-    }
-    u64 above = 0;
-    for (int i = t.rank; i < V; i += t.size) {
-        const Key ki = key_at(i);
-        if (ki > key) above += metric(i, ki);
-    }
-    const u64 need = target - t.reduce(above, OpSum());
-    int bits = 0;
-    while ((1 << bits) < V) ++bits;
-    uint32_t idx = (1u << bits) - 1u;
-    for (int b = bits - 1; b >= 0; --b) {
-        const uint32_t cand = idx & ~(1u << b);
-        u64 f = 0;
-        for (int i = t.rank; i < V; i += t.size) {
-            const Key ki = key_at(i);
-            if (ki == key && (uint32_t)i <= cand) f += metric(i, ki);
-        }
-        if (t.reduce(f, OpSum()) >= need) idx = cand;
-    }
-    return Ranked<Key>{key, idx};
+// rint(e 2^s) through the lowest bits of 2^52 + e 2^s
+__device__ __forceinline__ u64 whole_mass(double e, double scale) {
+    return (u64)__double_as_longlong(fma(e, scale, 4503599627370496.0)) - 0x4330000000000000ull;
 }
 
-template <typename T, typename Team, typename Get>
-__device__ int sample_row(const Team& t, Get get, int V, int shift, const RowSampling& rs) {
+// Narrow rows: keys (0: none; 1: NaN) and masses in registers, the classes
+// that stay as bits.  A thread that has a row to itself counts for each class
+// what comes before it; a team finds the cut's key bit by bit.
+template <typename T, int G, int ITEMS>
+__device__ int sample_row(const LaneTeam<G>& t, const Items<G, ITEMS>& mine, const typename Num<T>::C (&a)[ITEMS], int V,
+                          double scale, const RowSampling& rs) {
     typedef typename Num<T>::C C;
     typedef typename Num<T>::Key Key;
+    constexpr int kBits = (int)sizeof(Key) * 8 - Num<T>::kKeyDrop;
+    Key key[ITEMS];
     C m = -lg_inf(C());
     int bad = 0;
-    for (int i = t.rank; i < V; i += t.size) {
-        const C a = to_c(get(i));
-        bad |= a != a;
-        m = OpMax()(m, a);
+#pragma unroll
+    for (int it = 0; it < ITEMS; ++it) {
+        key[it] = mine.has(it) ? (key_of(a[it]) >> Num<T>::kKeyDrop) + 1 : 0;
+        bad |= key[it] == 1;
+        if (mine.has(it)) m = OpMax()(m, a[it]);
     }
     m = t.reduce(m, OpMax());
     bad = t.reduce(bad, OpOr());
     if (bad || m == -lg_inf(C())) return -1;
     if (rs.greedy) {
-        uint32_t at = 0xffffffffu;
-        for (int i = t.rank; i < V; i += t.size)
-            if (to_c(get(i)) == m && (uint32_t)i < at) at = (uint32_t)i;
-        return (int)t.reduce(at, OpMin());
+        int at = 0x7fffffff;
+#pragma unroll
+        for (int it = ITEMS - 1; it >= 0; --it)
+            if (mine.has(it) && a[it] == m) at = mine.first + it;
+        return t.reduce(at, OpMin());
     }
-    const double scale = __longlong_as_double((long long)(1023 + shift) << 52);
-    auto share = [&](int i) {  // infinite logits share the mass among themselves
-        const C a = to_c(get(i));
-        return a == m ? 1.0 : exp(((double)a - (double)m) * rs.inv_t);
-    };
-    auto mass = [&](int i) { return (u64)__double2ull_rn(share(i) * scale); };
-    auto key_at = [&](int i) { return key_of(to_c(get(i))); };
-    Ranked<Key> last{0, 0xffffffffu};  // the last class that stays
-    auto stays = [&](int i, Key k) { return k > last.key || (k == last.key && (uint32_t)i <= last.idx); };
-    if (rs.top_k < V)
-        last = team_select<Key>(t, V, (u64)rs.top_k, key_at, [&](int, Key) { return 1ull; });
-    if (rs.top_p < 1.0) {
-        u64 total = 0;
-        for (int i = t.rank; i < V; i += t.size)
-            if (stays(i, key_at(i))) total += mass(i);
-        total = t.reduce(total, OpSum());
-        const Ranked<Key> cut = team_select<Key>(t, V, mass_part(rs.top_p, total), key_at,
-                                                 [&](int i, Key k) { return stays(i, k) ? mass(i) : 0ull; });
-        last = cut;
+    u64 w[ITEMS];
+    uint32_t stay = 0, small = 0;  // small: below min-p
+#pragma unroll
+    for (int it = 0; it < ITEMS; ++it) {
+        w[it] = 0;
+        if (!mine.has(it)) continue;
+        const double e = a[it] == m ? 1.0 : exp(((double)a[it] - (double)m) * rs.inv_t);
+        w[it] = whole_mass(e, scale);
+        stay |= 1u << it;
+        if (e < rs.min_p) small |= 1u << it;
     }
-    auto kept = [&](int i) {
-        if (!stays(i, key_at(i))) return 0ull;
-        if (rs.min_p > 0.0 && share(i) < rs.min_p) return 0ull;
-        return mass(i);
-    };
-    const int per = (V + t.size - 1) / t.size;  // runs of classes by index
-    const int i0 = t.rank * per < V ? t.rank * per : V, i1 = i0 + per < V ? i0 + per : V;
-    u64 own = 0;
-    for (int i = i0; i < i1; ++i) own += kept(i);
-    u64 upto = t.exscan(own);
-    const u64 total = t.reduce(own, OpSum());
-    const u64 target = draw_target(rs.u, total);
-    uint32_t at = 0xffffffffu;
-    if (upto < target && upto + own >= target)
-        for (int i = i0; i < i1; ++i) {
-            upto += kept(i);
-            if (upto >= target) {
-                at = (uint32_t)i;
-                break;
+    // keeps the shortest prefix (in order) of what stays whose metric reaches `target`
+    auto cut = [&](u64 target, auto metric) {
+        if (G == 1) {
+            uint32_t keep = 0;
+#pragma unroll
+            for (int it = 0; it < ITEMS; ++it) {
+                u64 before = 0;
+#pragma unroll
+                for (int j = 0; j < ITEMS; ++j) {
+                    const bool first = j < it ? key[j] >= key[it] : (j > it && key[j] > key[it]);
+                    if (first && ((stay >> j) & 1)) before += metric(j);
+                }
+                if (((stay >> it) & 1) && before < target) keep |= 1u << it;
             }
+            stay = keep;
+            return;
         }
-    return (int)t.reduce(at, OpMin());
+        Key bound = 0;
+        for (int b = kBits - 1; b >= 0; --b) {
+            const Key cand = bound | ((Key)1 << b);
+            u64 f = 0;
+#pragma unroll
+            for (int it = 0; it < ITEMS; ++it)
+                if (key[it] >= cand && ((stay >> it) & 1)) f += metric(it);
+            f = t.reduce(f, OpSum());
+            if (f >= target) bound = cand;
+            if (f == target) break;
+        }
+        u64 above = 0, ties = 0;
+#pragma unroll
+        for (int it = 0; it < ITEMS; ++it)
+            if ((stay >> it) & 1) {
+                if (key[it] > bound) above += metric(it);
+                if (key[it] == bound) ties += metric(it);
+            }
+        // of equal keys the lower indices: the lanes' classes are in the order of the lanes
+        u64 before = t.reduce(above, OpSum()) + t.exscan(ties);
+        uint32_t keep = 0;
+#pragma unroll
+        for (int it = 0; it < ITEMS; ++it) {
+            if (!((stay >> it) & 1) || key[it] < bound) continue;
+            if (key[it] > bound || before < target) keep |= 1u << it;
+            if (key[it] == bound) before += metric(it);
+        }
+        stay = keep;
+    };
+    auto sum_of = [&](uint32_t bits) {
+        u64 f = 0;
+#pragma unroll
+        for (int it = 0; it < ITEMS; ++it)
+            if ((bits >> it) & 1) f += w[it];
+        return f;
+    };
+    if (rs.top_k < V) cut((u64)rs.top_k, [](int) { return 1ull; });
+    if (rs.top_p < 1.0) cut(mass_part(rs.top_p, t.reduce(sum_of(stay), OpSum())), [&](int it) { return w[it]; });
+    stay &= ~small;
+    const u64 own = sum_of(stay);
+    u64 upto = t.exscan(own);
+    const u64 target = draw_target(rs.u, t.reduce(own, OpSum()));
+    int at = 0x7fffffff;
+#pragma unroll
+    for (int it = 0; it < ITEMS; ++it) {
+        if (!((stay >> it) & 1)) continue;
+        if (upto < target && upto + w[it] >= target) at = mine.first + it;
+        upto += w[it];
+    }
+    return t.reduce(at, OpMin());
 }
 
-template <typename T, int G>
+template <typename T, int G, int ITEMS>
 __global__ void __launch_bounds__(kLgThreads)
-lg_sample_narrow_kernel(Rows<T> x, SampleArgs a, int shift, int tile, int pitch, int32_t* __restrict__ index) {
+lg_sample_narrow_kernel(Rows<T> x, SampleArgs a, int shift, int tile, int direct, int32_t* __restrict__ index) {
+    typedef typename Num<T>::C C;
     extern __shared__ __align__(16) unsigned char lg_smem[];
-    T* s = reinterpret_cast<T*>(lg_smem);
     const int64_t r0 = (int64_t)blockIdx.x * tile;
-    const int rows = (int)(x.n - r0 < tile ? x.n - r0 : tile);
-    tile_copy<T, false>(s, pitch, rows, x.V, const_cast<T*>(x.data) + r0 * x.row_stride, x.row_stride, x.class_stride);
-    __syncthreads();
+    const int rows = (int)(x.n - r0 < tile ? x.n - r0 : tile), V = x.V;
+    T* g = const_cast<T*>(x.data) + r0 * x.row_stride;
+    const TileIo<T> io(g, x.row_stride, x.class_stride, V, rows);
+    T* s = reinterpret_cast<T*>(lg_smem) + io.shift;
+    if (!direct) {
+        io.template copy<false>(s, g);
+        __syncthreads();
+    }
     const LaneTeam<G> t;
+    const Items<G, ITEMS> mine(t, V);
+    const double scale = __longlong_as_double((long long)(1023 + shift) << 52);
     for (int r = threadIdx.x / G; r < rows; r += kLgThreads / G) {
-        const T* row = s + (size_t)r * pitch;
-        const int got = sample_row<T>(t, [&](int i) { return row[i]; }, x.V, shift, row_sampling(a, r0 + r, x.V));
+        C v[ITEMS];
+        if (direct) {
+            const T* row = g + r * x.row_stride;
+#pragma unroll
+            for (int it = 0; it < ITEMS; ++it)
+                v[it] = mine.has(it) ? to_c(row[(int64_t)(mine.first + it) * x.class_stride]) : C(0);
+        } else {
+            const T* row = s + (size_t)r * io.pitch;
+#pragma unroll
+            for (int it = 0; it < ITEMS; ++it) v[it] = mine.has(it) ? to_c(row[mine.first + it]) : C(0);
+        }
+        const int got = sample_row<T, G, ITEMS>(t, mine, v, V, scale, row_sampling(a, r0 + r, V));
         if (t.rank == 0) index[r0 + r] = got;
     }
 }
@@ -189,10 +219,7 @@ struct Weigh {
     Ranked<Key> last;  // the last class that stays
     bool cut;
     __device__ double share(C a) const { return a == m ? 1.0 : exp(((double)a - (double)m) * inv_t); }
-    // rint(e 2^s) through the lowest bits of 2^52 + e 2^s
-    __device__ u64 whole(double e) const {
-        return (u64)__double_as_longlong(fma(e, scale, 4503599627370496.0)) - 0x4330000000000000ull;
-    }
+    __device__ u64 whole(double e) const { return whole_mass(e, scale); }
     __device__ u64 mass(C a) const { return whole(share(a)); }
     __device__ bool stays(int i, C a) const {
         const Key k = key_of(a);
@@ -569,12 +596,15 @@ int run_sample(const cbgpu_logits* x, const cbgpu_sampling* s, int32_t* index, c
         return lg_launch_wide(who, lg_sample_wide_kernel<T>, rows.n, w, w.smem, st, w.ahead, rows, a, shift, index);
     }
     auto narrow = [&](auto kernel, int lanes) {
-        const Tile t = narrow_tile(rows.V, sizeof(T), kLgThreads / lanes, rows.class_stride <= rows.row_stride);
-        return lg_launch(who, kernel, tiles_of(rows.n, t.rows), t.smem, st, rows, a, shift, t.rows, t.pitch, index);
+        const bool direct = lanes == 1 && rows.class_stride > rows.row_stride;
+        Tile t = narrow_tile(rows.V, sizeof(T), kLgThreads / lanes);
+        if (direct) t = Tile{kLgThreads, 0};
+        return lg_launch(who, kernel, tiles_of(rows.n, t.rows), t.smem, st, rows, a, shift, t.rows, (int)direct, index);
     };
-    return by_lanes(rows.V, [&] { return narrow(lg_sample_narrow_kernel<T, 1>, 1); },
-                    [&] { return narrow(lg_sample_narrow_kernel<T, 8>, 8); },
-                    [&] { return narrow(lg_sample_narrow_kernel<T, 32>, 32); });
+    if (rows.V <= 8) return narrow(lg_sample_narrow_kernel<T, 1, 8>, 1);
+    if (rows.V <= 16) return narrow(lg_sample_narrow_kernel<T, 1, 16>, 1);
+    if (rows.V <= 128) return narrow(lg_sample_narrow_kernel<T, 8, 16>, 8);
+    return narrow(lg_sample_narrow_kernel<T, 32, 32>, 32);
 }
 
 }  // namespace

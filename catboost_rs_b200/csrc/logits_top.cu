@@ -5,68 +5,146 @@
 
 namespace {
 
-// k rounds, each taking the first class after the one before it; then the
-// log-sum-exp of what is left, relative to its own largest.
-template <typename T, typename Team, typename Get>
-__device__ void top_row(const Team& t, Get get, int V, int k, Scale<typename Num<T>::C> sc, T* value, int32_t* index,
-                        typename Num<T>::C* tail) {
-    typedef typename Num<T>::C C;
-    typedef typename Num<T>::Key Key;
-    Ranked<Key> last{~(Key)0, 0u};  // before every class: no logit has the all-ones key
-    for (int j = 0; j < k + (tail ? 1 : 0); ++j) {
-        Ranked<Key> best{0, 0xffffffffu};
-        for (int i = t.rank; i < V; i += t.size) {
-            const Ranked<Key> r{key_of(to_c(get(i))), (uint32_t)i};
-            if (last.before(r) && r.before(best)) best = r;
-        }
-        best = team_first(t, best);
-        if (j == k) {  // the largest of the rest
-            C sum = 0;
-            const C top = best.idx < (uint32_t)V ? to_c(get((int)best.idx)) : -lg_inf(C());
-            const bool some = top > -lg_inf(C());
-            int bad = 0;
-            double acc = 0.0;
-            for (int i = t.rank; i < V; i += t.size) {
-                const C a = to_c(get(i));
-                bad |= a != a;
-                const Ranked<Key> r{key_of(a), (uint32_t)i};
-                if (last.before(r) && some) {
-                    sum = lg_exp(a - top, sc.c);
-                    acc += (double)sum;
-                }
+// Narrow rows.  A lane's classes are keys in registers (0: none, or taken; 1: NaN).
+// Up to kRounds of them are taken one by one, each lane offering its best;
+// above that (a warp a row) the k-th key is found bit by bit, and the keys
+// from it on are listed and sorted.
+constexpr int kRounds = 16;
+
+template <typename Key>
+struct TopList {
+    Key key[kLgMaxTop];
+    uint32_t idx[kLgMaxTop];
+};
+
+template <typename Key>
+__device__ void warp_sort(TopList<Key>& l, int n) {
+    const int lane = threadIdx.x & 31;
+    int size = 1;
+    while (size < n) size *= 2;
+    for (int i = n + lane; i < size; i += 32) l.key[i] = 0, l.idx[i] = 0xffffffffu;
+    __syncwarp();
+    for (int len = 2; len <= size; len *= 2)
+        for (int d = len / 2; d > 0; d /= 2) {
+            for (int p = lane; p < size / 2; p += 32) {
+                const int i = (p & (d - 1)) | ((p & ~(d - 1)) << 1), j = i | d;
+                const Ranked<Key> a{l.key[i], l.idx[i]}, b{l.key[j], l.idx[j]};
+                if ((i & len) == 0 ? b.before(a) : a.before(b))
+                    l.key[i] = b.key, l.idx[i] = b.idx, l.key[j] = a.key, l.idx[j] = a.idx;
             }
-            bad = t.reduce(bad, OpOr());
-            acc = t.reduce(acc, OpSum());
-            if (t.rank == 0) {
-                const double v = bad ? (double)lg_inf(C()) - (double)lg_inf(C())
-                                     : (some ? (double)top * sc.inv_t + log(acc) : -(double)lg_inf(C()));
-                *tail = (C)v;
-            }
-            return;
+            __syncwarp();
         }
-        if (t.rank == 0) {
-            value[j] = get((int)best.idx);
-            index[j] = (int32_t)best.idx;
-        }
-        last = best;
-    }
 }
 
-template <typename T, int G>
+template <typename T, int G, int ITEMS>
 __global__ void __launch_bounds__(kLgThreads)
-lg_top_narrow_kernel(Rows<T> x, int k, Scale<typename Num<T>::C> sc, int tile, int pitch, T* __restrict__ value,
+lg_top_narrow_kernel(Rows<T> x, int k, Scale<typename Num<T>::C> sc, int tile, T* __restrict__ value,
                      int32_t* __restrict__ index, typename Num<T>::C* __restrict__ tail) {
+    typedef typename Num<T>::C C;
+    typedef typename Num<T>::Key Key;
+    constexpr int kBits = (int)sizeof(Key) * 8 - Num<T>::kKeyDrop;
+    constexpr bool kLists = G == 32;
     extern __shared__ __align__(16) unsigned char lg_smem[];
-    T* s = reinterpret_cast<T*>(lg_smem);
+    __shared__ TopList<Key> lists[kLists ? kLgWarps : 1];
     const int64_t r0 = (int64_t)blockIdx.x * tile;
-    const int rows = (int)(x.n - r0 < tile ? x.n - r0 : tile);
-    tile_copy<T, false>(s, pitch, rows, x.V, const_cast<T*>(x.data) + r0 * x.row_stride, x.row_stride, x.class_stride);
+    const int rows = (int)(x.n - r0 < tile ? x.n - r0 : tile), V = x.V;
+    T* g = const_cast<T*>(x.data) + r0 * x.row_stride;
+    const TileIo<T> io(g, x.row_stride, x.class_stride, V, rows);
+    T* s = reinterpret_cast<T*>(lg_smem) + io.shift;
+    io.template copy<false>(s, g);
     __syncthreads();
     const LaneTeam<G> t;
+    const Items<G, ITEMS> mine(t, V);
     for (int r = threadIdx.x / G; r < rows; r += kLgThreads / G) {
-        const T* row = s + (size_t)r * pitch;
-        top_row<T>(t, [&](int i) { return row[i]; }, x.V, k, sc, value + (r0 + r) * k, index + (r0 + r) * k,
-                   tail ? tail + r0 + r : nullptr);
+        const T* row = s + (size_t)r * io.pitch;
+        T* val = value + (r0 + r) * k;
+        int32_t* idx = index + (r0 + r) * k;
+        Key key[ITEMS];
+#pragma unroll
+        for (int it = 0; it < ITEMS; ++it)
+            key[it] = mine.has(it) ? (key_of(to_c(row[mine.first + it])) >> Num<T>::kKeyDrop) + 1 : 0;
+        bool nan = false;  // among the first k
+        if (!kLists || k <= kRounds) {
+            Key best = 0;
+            int at = 0;
+            auto look = [&] {
+                best = 0;
+#pragma unroll
+                for (int it = 0; it < ITEMS; ++it) best = key[it] > best ? key[it] : best;
+                at = 0;
+#pragma unroll
+                for (int it = ITEMS - 1; it >= 0; --it) at = key[it] == best ? it : at;
+            };
+            look();
+            for (int j = 0; j < k; ++j) {
+                const Key top = t.reduce(best, OpMax());
+                const int i = t.reduce(best == top ? mine.first + at : 0x7fffffff, OpMin());
+                nan = top == 1;
+                if (best == top && i == mine.first + at) {
+                    val[j] = row[i];
+                    idx[j] = i;
+#pragma unroll
+                    for (int it = 0; it < ITEMS; ++it) key[it] = it == at ? 0 : key[it];
+                    look();
+                }
+            }
+        } else {
+            TopList<Key>& list = lists[kLists ? threadIdx.x >> 5 : 0];
+            Key bound = 0;
+            int above = 0;  // keys past the k-th key's bits, once it is found
+            bool exact = false;
+            for (int b = kBits - 1; b >= 0 && !exact; --b) {
+                const Key cand = bound | ((Key)1 << b);
+                int n = 0;
+#pragma unroll
+                for (int it = 0; it < ITEMS; ++it) n += key[it] >= cand;
+                n = team_count(t, n);
+                if (n >= k) bound = cand;
+                exact = n == k;
+            }
+            int own = 0, ties = 0;
+#pragma unroll
+            for (int it = 0; it < ITEMS; ++it) own += key[it] > bound, ties += key[it] == bound;
+            above = team_count(t, own);
+            // of equal keys the lower indices: the lanes' classes are in the order of the lanes
+            int spare = k - above - (int)t.exscan((u64)ties);
+            spare = spare < 0 ? 0 : (spare < ties ? spare : ties);
+            int to = (int)t.exscan((u64)(own + spare));
+#pragma unroll
+            for (int it = 0; it < ITEMS; ++it) {
+                const bool take = key[it] > bound || (key[it] == bound && spare > 0);
+                if (take && key[it] == bound) --spare;
+                if (take) {
+                    list.key[to] = key[it], list.idx[to] = (uint32_t)(mine.first + it);
+                    ++to;
+                    key[it] = 0;
+                }
+            }
+            __syncwarp();
+            warp_sort(list, k);
+            for (int j = t.rank; j < k; j += G) {
+                const int i = (int)list.idx[j];
+                val[j] = row[i];
+                idx[j] = i;
+            }
+            nan = list.key[k - 1] == 1;
+            __syncwarp();
+        }
+        if (!tail) continue;
+        C m = -lg_inf(C());
+#pragma unroll
+        for (int it = 0; it < ITEMS; ++it)
+            if (key[it] != 0) m = OpMax()(m, to_c(row[mine.first + it]));
+        m = floor_max(t.reduce(m, OpMax()));
+        C part = 0;
+#pragma unroll
+        for (int it = 0; it < ITEMS; ++it)
+            if (key[it] != 0) part += lg_exp(to_c(row[mine.first + it]) - m, sc.c);
+        const double sum = t.reduce((double)part, OpSum());
+        if (t.rank == 0) {
+            const double none = sum == 0.0 ? -lg_inf(0.0) : log(sum) + (double)m * sc.inv_t;
+            tail[r0 + r] = (C)(nan ? lg_inf(0.0) - lg_inf(0.0) : none);
+        }
     }
 }
 
@@ -157,13 +235,14 @@ int run_top(const cbgpu_logits* x, int k, double temp, void* value, int32_t* ind
                               (C*)tail);
     }
     auto narrow = [&](auto kernel, int lanes) {
-        const Tile t = narrow_tile(rows.V, sizeof(T), kLgThreads / lanes, rows.class_stride <= rows.row_stride);
-        return lg_launch(who, kernel, tiles_of(rows.n, t.rows), t.smem, st, rows, k, sc, t.rows, t.pitch, (T*)value,
-                         index, (C*)tail);
+        const Tile t = narrow_tile(rows.V, sizeof(T), kLgThreads / lanes);
+        return lg_launch(who, kernel, tiles_of(rows.n, t.rows), t.smem, st, rows, k, sc, t.rows, (T*)value, index,
+                         (C*)tail);
     };
-    return by_lanes(rows.V, [&] { return narrow(lg_top_narrow_kernel<T, 1>, 1); },
-                    [&] { return narrow(lg_top_narrow_kernel<T, 8>, 8); },
-                    [&] { return narrow(lg_top_narrow_kernel<T, 32>, 32); });
+    if (rows.V <= 8) return narrow(lg_top_narrow_kernel<T, 1, 8>, 1);
+    if (rows.V <= 16) return narrow(lg_top_narrow_kernel<T, 1, 16>, 1);
+    if (rows.V <= 128) return narrow(lg_top_narrow_kernel<T, 8, 16>, 8);
+    return narrow(lg_top_narrow_kernel<T, 32, 32>, 32);
 }
 
 }  // namespace
