@@ -23,16 +23,23 @@ from . import _lib
 MAX_CLASSES = 262144
 MAX_TOP = 256
 
-_torch = None
+_torch = None  # and what is asked of it in every call, set by the first
 _dtypes: dict = {}
+_get_device = _get_stream = _L = None
 
 
 def _t():
-    global _torch
+    global _torch, _get_device, _get_stream, _L
     if _torch is None:
         import torch
+        _L = _lib.load()
         _dtypes.update({torch.float64: _lib.F64, torch.float32: _lib.F32, torch.float16: _lib.F16,
                         torch.bfloat16: _lib.BF16})
+        if hasattr(torch._C, "_cuda_getCurrentRawStream"):
+            # what torch.cuda.current_device and current_stream end in, without their objects
+            _get_device, _get_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+        else:
+            _get_device, _get_stream = torch.cuda.current_device, lambda d: torch.cuda.current_stream(d).cuda_stream
         _torch = torch
     return _torch
 
@@ -60,14 +67,16 @@ def _bad(msg: str):
 
 
 def _logits(who, x):
-    torch = _t()
+    torch = _torch or _t()
     if not isinstance(x, torch.Tensor):
         raise _bad(f"{who}: logits must be a torch tensor")
-    if x.dim() != 2:
-        raise _bad(f"{who}: logits must be [n, classes], got {tuple(x.shape)}")
-    if x.dtype not in _dtypes:
+    shape = x.shape
+    if len(shape) != 2:
+        raise _bad(f"{who}: logits must be [n, classes], got {tuple(shape)}")
+    dtype = _dtypes.get(x.dtype)
+    if dtype is None:
         raise _bad(f"{who}: logits must be float64, float32, float16 or bfloat16, got {x.dtype}")
-    n, V = x.shape
+    n, V = shape
     if not 1 <= V <= MAX_CLASSES:
         raise _bad(f"{who}: {V} classes, outside 1..{MAX_CLASSES}")
     if n > 0x7fffffff:
@@ -75,7 +84,7 @@ def _logits(who, x):
     if not x.is_cuda:
         raise _bad(f"{who}: logits must be on a CUDA device")
     rs, cs = x.stride()
-    return _lib.Logits(x.data_ptr(), _dtypes[x.dtype], V, n, rs, cs)
+    return _lib.Logits(x.data_ptr(), dtype, V, n, rs, cs)
 
 
 def _side(who, name, v, x, shape, dtypes):
@@ -84,7 +93,7 @@ def _side(who, name, v, x, shape, dtypes):
         raise _bad(f"{who}: {name} must be a tensor on the logits' device")
     if v.dtype not in dtypes:
         raise _bad(f"{who}: {name} has dtype {v.dtype}, expected {' or '.join(str(d) for d in dtypes)}")
-    if tuple(v.shape) != shape:
+    if v.shape != shape:
         raise _bad(f"{who}: LengthMismatch: {name} is {tuple(v.shape)}, expected {shape}")
     return v if v.is_contiguous() else v.contiguous()
 
@@ -95,13 +104,14 @@ def _wide(x):
 
 def _run(x, fn, *args):
     """fn(*args, stream) on the device of x, on its current stream."""
-    dev = x.device.index
-    stream = C.c_void_p(_torch.cuda.current_stream(dev).cuda_stream)
-    if _torch.cuda.current_device() == dev:
-        _lib.check(fn(*args, stream))
+    dev = x.get_device()
+    if _get_device() == dev:
+        rc = fn(*args, _get_stream(dev))
     else:
         with _torch.cuda.device(dev):
-            _lib.check(fn(*args, stream))
+            rc = fn(*args, _get_stream(dev))
+    if rc:
+        _lib.check(rc)
 
 
 def _temperature(who, t, least=1e-6):
@@ -123,10 +133,10 @@ def top_logits(logits, k: int, *, temperature: float = 1.0, tail: bool = True) -
         raise _bad(f"{who}: k = {k} is outside 1..min({MAX_TOP}, {d.n_classes} classes)")
     temperature = _temperature(who, temperature)
     n = d.n
-    value = _torch.empty((n, k), dtype=logits.dtype, device=logits.device)
-    index = _torch.empty((n, k), dtype=_torch.int32, device=logits.device)
-    rest = _torch.empty((n,), dtype=_wide(logits), device=logits.device) if tail else None
-    _run(logits, _lib.load().cbgpu_top_logits, C.byref(d), k, temperature, value.data_ptr(), index.data_ptr(),
+    value = logits.new_empty((n, k))
+    index = logits.new_empty((n, k), dtype=_torch.int32)
+    rest = logits.new_empty((n,), dtype=_wide(logits)) if tail else None
+    _run(logits, _L.cbgpu_top_logits, C.byref(d), k, temperature, value.data_ptr(), index.data_ptr(),
          rest.data_ptr() if tail else None)
     return TopLogits(index, value, rest)
 
@@ -137,9 +147,9 @@ def _distill(who, logits, teacher, weight, temperature, der1):
     wide = _wide(logits)
     if not isinstance(teacher, TopLogits):
         raise _bad(f"{who}: teacher must be a TopLogits")
-    shape = tuple(getattr(teacher.index, "shape", ()))
+    shape = getattr(teacher.index, "shape", ())
     if len(shape) != 2 or shape[0] != n or not 1 <= shape[1] <= MAX_TOP:
-        raise _bad(f"{who}: LengthMismatch: the teacher's index is {shape}, expected ({n}, 1..{MAX_TOP})")
+        raise _bad(f"{who}: LengthMismatch: the teacher's index is {tuple(shape)}, expected ({n}, 1..{MAX_TOP})")
     index = _side(who, "the teacher's index", teacher.index, logits, shape, (_torch.int32, _torch.int64))
     value = _side(who, "the teacher's value", teacher.value, logits, shape, tuple(_dtypes))
     rest = None if teacher.tail is None else _side(who, "the teacher's tail", teacher.tail, logits, (n,), (wide,))
@@ -150,11 +160,11 @@ def _distill(who, logits, teacher, weight, temperature, der1):
             raise _bad(f"{who}: out must be a {logits.dtype} tensor on the logits' device")
         if der1.shape != logits.shape:
             raise _bad(f"{who}: LengthMismatch: out is {tuple(der1.shape)}, expected {tuple(logits.shape)}")
-    loss = _torch.empty((n,), dtype=wide, device=logits.device)
+    loss = logits.new_empty((n,), dtype=wide)
     t = _lib.Teacher(index.data_ptr(), value.data_ptr(), None if rest is None else rest.data_ptr(),
                      index.element_size(), _dtypes[value.dtype], shape[1])
     rs, cs = der1.stride() if der1 is not None else (0, 0)
-    _run(logits, _lib.load().cbgpu_distill, C.byref(d), C.byref(t), None if weight is None else weight.data_ptr(),
+    _run(logits, _L.cbgpu_distill, C.byref(d), C.byref(t), None if weight is None else weight.data_ptr(),
          temperature, loss.data_ptr(), None if der1 is None else der1.data_ptr(), rs, cs)
     return loss
 
@@ -174,10 +184,8 @@ def distill_derivatives(logits, teacher: TopLogits, *, weight=None, temperature:
     who = "distill_derivatives"
     if out is None:
         _logits(who, logits)
-        dense = logits.shape[0] * logits.shape[1] <= 1 or (sorted(logits.stride())[0] == 1 and (
-            logits.is_contiguous() or logits.t().is_contiguous()))
-        out = _torch.empty_like(logits) if dense else _torch.empty(
-            tuple(logits.shape), dtype=logits.dtype, device=logits.device)
+        dense = logits.is_contiguous() or logits.t().is_contiguous()
+        out = _torch.empty_like(logits) if dense else logits.new_empty(logits.shape)
     return Distilled(_distill(who, logits, teacher, weight, temperature, out), out)
 
 
@@ -222,6 +230,6 @@ def sample_classes(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_
         if int(top_k) < 0:
             raise _bad(f"{who}: top_k {top_k} < 0")
         s.top_k = min(int(top_k), MAX_CLASSES)
-    index = _torch.empty((n,), dtype=_torch.int32, device=logits.device)
-    _run(logits, _lib.load().cbgpu_sample_classes, C.byref(d), C.byref(s), index.data_ptr())
+    index = logits.new_empty((n,), dtype=_torch.int32)
+    _run(logits, _L.cbgpu_sample_classes, C.byref(d), C.byref(s), index.data_ptr())
     return index

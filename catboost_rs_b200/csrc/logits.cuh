@@ -35,7 +35,8 @@ namespace {
 
 constexpr int kLgMaxClasses = 262144;
 constexpr int kLgMaxTop = 256;
-constexpr int kLgNarrow = 1024;
+constexpr int kLgNarrow = 512;
+constexpr int kLgFew = 128;
 constexpr int kLgThreads = 256;
 
 int lfail(int code, const char* fmt, ...) {
@@ -172,6 +173,15 @@ struct LaneTeam {
         for (int o = G / 2; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(mask, v, o));
         return v;
     }
+    // a sum of masses, below 2^62
+    __device__ u64 sum(u64 v) const {
+        if (G < 32) return reduce(v, OpSum());
+        const uint32_t part = (1u << 26) - 1u;  // 32 of them fit 31 bits
+        const u64 lo = __reduce_add_sync(0xffffffffu, (uint32_t)v & part);
+        const u64 mid = __reduce_add_sync(0xffffffffu, (uint32_t)(v >> 26) & part);
+        const u64 hi = __reduce_add_sync(0xffffffffu, (uint32_t)(v >> 52));
+        return lo + (mid << 26) + (hi << 52);
+    }
     __device__ u64 exscan(u64 v) const {
         u64 inc = v;
 #pragma unroll
@@ -290,18 +300,22 @@ struct TileIo {
     }
 };
 
-// A lane's classes.
+// A lane's classes.  Loops over them are unrolled to ITEMS and stop, by fours, at `per`, which all
+// lanes share.
 template <int G, int ITEMS>
 struct Items {
-    int first, count;
+    int first, count, per;
     template <typename Team>
     __device__ Items(const Team& t, int V) {
-        const int per = (V + G - 1) / G;
+        per = (V + G - 1) / G;
         first = t.rank * per;
         count = V - first < per ? V - first : per;
     }
     __device__ bool has(int it) const { return it < count; }
 };
+#define LG_EACH(it)                                                      \
+    _Pragma("unroll") for (int four_ = 0; four_ < ITEMS; four_ += 4)     \
+        if (four_ < mine.per) _Pragma("unroll") for (int it = four_; it < four_ + 4; ++it)
 
 template <typename Key>
 struct Ranked {  // a class in the operators' order
@@ -1026,6 +1040,11 @@ int lg_launch_wide(const char* who, K kernel, int64_t n, const Wide& w, size_t s
     }
     return CBGPU_OK;
 }
+
+// Rows above kLgFew classes are wide when there are few of them: a block of 256 threads a row
+// instead of a warp (8 rows of 1000 f32, derivatives: 5 us against 22; at 20000 rows 193 against 391
+// before the warp's loops stopped at its classes).
+bool is_wide(int64_t n, int V) { return V > kLgNarrow || (V > kLgFew && n <= 148 * 8); }
 
 unsigned tiles_of(int64_t n, int rows) { return (unsigned)((n + rows - 1) / rows); }
 

@@ -84,20 +84,20 @@ lg_distill_narrow_kernel(Rows<T> x, TeacherArgs tc, const typename Num<T>::C* __
     for (int r = threadIdx.x / G; r < rows; r += kLgThreads / G) {
         T* row = s + (size_t)r * io.pitch;
         C* tgt = tgt_all + (size_t)r * tgt_pitch;
-        C a[ITEMS];
+        C a[ITEMS] = {};
         if (direct) {
             const T* from = g + r * x.row_stride;
-#pragma unroll
-            for (int it = 0; it < ITEMS; ++it)
+            LG_EACH(it)
                 a[it] = mine.has(it) ? to_c(from[(int64_t)(mine.first + it) * x.class_stride]) : -lg_inf(C());
         } else {
-#pragma unroll
-            for (int it = 0; it < ITEMS; ++it) a[it] = mine.has(it) ? to_c(row[mine.first + it]) : -lg_inf(C());
+            LG_EACH(it) a[it] = mine.has(it) ? to_c(row[mine.first + it]) : -lg_inf(C());
         }
         const double w = weight ? (double)weight[r0 + r] : 1.0;
         const double tl = tail ? (double)tail[r0 + r] : -lg_inf(0.0);
         for (int i = t.rank; i < V; i += G) set_absent(&tgt[i]);
         t.sync();
+        u64 claimed = 0;  // which of this lane's entries count
+        static_assert(G == 1 || kLgMaxTop / G <= 64, "a bit an entry");
         for (int j0 = 0; j0 < tc.k; j0 += G) {
             const int j = j0 + t.rank;
             const int64_t at = (r0 + r) * tc.k + j;
@@ -107,13 +107,15 @@ lg_distill_narrow_kernel(Rows<T> x, TeacherArgs tc, const typename Num<T>::C* __
                 const unsigned same = __match_any_sync(t.mask, take ? (int)idx : -1 - t.rank);
                 take = take && (__ffs(same) - 1) == (int)(threadIdx.x & 31);
             }
-            if (take && is_absent(tgt[idx])) tgt[idx] = plain_nan((C)load_any(tc.value, tc.value_dtype, at));
+            if (take && is_absent(tgt[idx])) {
+                tgt[idx] = plain_nan((C)load_any(tc.value, tc.value_dtype, at));
+                claimed |= 1ull << (G > 1 ? j0 / G : 0);
+            }
             t.sync();
         }
         C m = -lg_inf(C()), zm = -lg_inf(C());
         uint32_t top = 0;  // which of this lane's classes are entries
-#pragma unroll
-        for (int it = 0; it < ITEMS; ++it) {
+        LG_EACH(it) {
             m = OpMax()(m, a[it]);
             if (!mine.has(it)) continue;
             const C z = tgt[mine.first + it];
@@ -124,11 +126,27 @@ lg_distill_narrow_kernel(Rows<T> x, TeacherArgs tc, const typename Num<T>::C* __
         const double z_max = floor_max(fmax((double)zm * sc.inv_t, tl));
         C sum_top = 0, sum_rest = 0;
         double r_sum = 0.0, cross = 0.0;
-#pragma unroll
-        for (int it = 0; it < ITEMS; ++it) {
+        if (G > 1) {  // a lane an entry: fewer steps in 64 bits than by class
+            for (int j0 = 0; j0 < tc.k; j0 += G) {
+                if (!((claimed >> (j0 / G)) & 1)) continue;
+                const int i = (int)tc.idx((r0 + r) * tc.k + j0 + t.rank);
+                const C ai = to_c(row[i]);
+                const double d = (double)tgt[i] * sc.inv_t - z_max;
+                const C rj = part_exp((C)d);
+                r_sum += (double)rj;
+                if (rj != C(0)) cross += (double)rj * (d - ((double)ai - (double)m) * sc.inv_t);
+                tgt[i] = rj;
+            }
+            t.sync();
+        }
+        LG_EACH(it) {
             const C e = lg_exp(a[it] - m, sc.c);
             if ((top >> it) & 1) {
                 sum_top += e;
+                if (G > 1) {
+                    a[it] = e;
+                    continue;
+                }
                 const double d = (double)tgt[mine.first + it] * sc.inv_t - z_max;
                 const double rj = (double)part_exp((C)d);
                 r_sum += rj;
@@ -150,8 +168,7 @@ lg_distill_narrow_kernel(Rows<T> x, TeacherArgs tc, const typename Num<T>::C* __
         }
         if (t.rank == 0) loss[r0 + r] = (C)o.loss;
         if (!der1) continue;
-#pragma unroll
-        for (int it = 0; it < ITEMS; ++it) {
+        LG_EACH(it) {
             if (!mine.has(it)) continue;
             C d = C(0);
             if (!o.zero)
@@ -440,7 +457,7 @@ int run_distill(const cbgpu_logits* x, const cbgpu_teacher* tc, const void* weig
     const Rows<T> rows = rows_of<T>(x);
     const Scale<C> sc(temp);
     const TeacherArgs ta{tc->index, tc->value, tc->index_bytes, tc->value_dtype, tc->k};
-    if (rows.V > kLgNarrow) {
+    if (is_wide(rows.n, rows.V)) {
         const Wide w = wide_shape<T>(rows.n, rows.V);
         return lg_launch_wide(who, lg_distill_wide_kernel<T>, rows.n, w, w.smem, st, w.ahead, rows, ta, (const C*)tc->tail,
                               (const C*)weight, temp, sc, (C*)loss, (T*)der1, drs, dcs);
@@ -452,10 +469,12 @@ int run_distill(const cbgpu_logits* x, const cbgpu_teacher* tc, const void* weig
         return lg_launch(who, kernel, tiles_of(rows.n, t.rows), t.smem, st, rows, ta, (const C*)tc->tail,
                          (const C*)weight, temp, sc, t.rows, (int)direct, (C*)loss, (T*)der1, drs, dcs);
     };
-    if (rows.V <= 8) return narrow(lg_distill_narrow_kernel<T, 1, 8>, 1);
+    if (rows.V <= 4) return narrow(lg_distill_narrow_kernel<T, 1, 4>, 1);
+    if (rows.V <= 12) return narrow(lg_distill_narrow_kernel<T, 1, 12>, 1);
     if (rows.V <= 16) return narrow(lg_distill_narrow_kernel<T, 1, 16>, 1);
+    if (rows.V <= 32) return narrow(lg_distill_narrow_kernel<T, 8, 4>, 8);
     if (rows.V <= 128) return narrow(lg_distill_narrow_kernel<T, 8, 16>, 8);
-    return narrow(lg_distill_narrow_kernel<T, 32, 32>, 32);
+    return narrow(lg_distill_narrow_kernel<T, 32, 16>, 32);
 }
 
 }  // namespace

@@ -1,4 +1,6 @@
 // logits_sample.cu -- cbgpu_sample_classes: a class drawn from a row under temperature / top-k / top-p / min-p.
+#include <type_traits>
+
 #include "logits.cuh"
 
 namespace {
@@ -60,23 +62,21 @@ __device__ __forceinline__ u64 whole_mass(double e, double scale) {
     return (u64)__double_as_longlong(fma(e, scale, 4503599627370496.0)) - 0x4330000000000000ull;
 }
 
-// Narrow rows: keys (0: none; 1: NaN) and masses in registers, the classes
-// that stay as bits.  A thread that has a row to itself counts for each class
-// what comes before it; a team finds the cut's key bit by bit.
+// Narrow rows: logits and masses in registers, the classes that stay as bits.
+// A thread that has a row to itself counts for each class what comes before
+// it; a team finds the cut by halving an interval of logits.
 template <typename T, int G, int ITEMS>
 __device__ int sample_row(const LaneTeam<G>& t, const Items<G, ITEMS>& mine, const typename Num<T>::C (&a)[ITEMS], int V,
-                          double scale, const RowSampling& rs) {
+                          int shift, const RowSampling& rs) {
     typedef typename Num<T>::C C;
-    typedef typename Num<T>::Key Key;
-    constexpr int kBits = (int)sizeof(Key) * 8 - Num<T>::kKeyDrop;
-    Key key[ITEMS];
+    const double scale = __longlong_as_double((long long)(1023 + shift) << 52);
+    const double reach = (double)(shift + 2) * 0.6931471805599453 / rs.inv_t;  // behind it a weight is 0
     C m = -lg_inf(C());
     int bad = 0;
-#pragma unroll
-    for (int it = 0; it < ITEMS; ++it) {
-        key[it] = mine.has(it) ? (key_of(a[it]) >> Num<T>::kKeyDrop) + 1 : 0;
-        bad |= key[it] == 1;
-        if (mine.has(it)) m = OpMax()(m, a[it]);
+    LG_EACH(it) {
+        if (!mine.has(it)) continue;
+        bad |= a[it] != a[it];
+        m = OpMax()(m, a[it]);
     }
     m = t.reduce(m, OpMax());
     bad = t.reduce(bad, OpOr());
@@ -88,10 +88,9 @@ __device__ int sample_row(const LaneTeam<G>& t, const Items<G, ITEMS>& mine, con
             if (mine.has(it) && a[it] == m) at = mine.first + it;
         return t.reduce(at, OpMin());
     }
-    u64 w[ITEMS];
+    u64 w[ITEMS] = {};
     uint32_t stay = 0, small = 0;  // small: below min-p
-#pragma unroll
-    for (int it = 0; it < ITEMS; ++it) {
+    LG_EACH(it) {
         w[it] = 0;
         if (!mine.has(it)) continue;
         const double e = a[it] == m ? 1.0 : exp(((double)a[it] - (double)m) * rs.inv_t);
@@ -99,68 +98,85 @@ __device__ int sample_row(const LaneTeam<G>& t, const Items<G, ITEMS>& mine, con
         stay |= 1u << it;
         if (e < rs.min_p) small |= 1u << it;
     }
-    // keeps the shortest prefix (in order) of what stays whose metric reaches `target`
-    auto cut = [&](u64 target, auto metric) {
+    // Keeps the shortest prefix (in order) of what stays whose metric, the
+    // number or the mass of classes, reaches `target`.
+    auto cut = [&](u64 target, auto by_mass) {
+        constexpr bool kMass = decltype(by_mass)::value;
         if (G == 1) {
             uint32_t keep = 0;
-#pragma unroll
-            for (int it = 0; it < ITEMS; ++it) {
+            LG_EACH(it) {
                 u64 before = 0;
 #pragma unroll
-                for (int j = 0; j < ITEMS; ++j) {
-                    const bool first = j < it ? key[j] >= key[it] : (j > it && key[j] > key[it]);
-                    if (first && ((stay >> j) & 1)) before += metric(j);
+                for (int j = 0; j < ITEMS; ++j) {  // what does not stay weighs nothing
+                    const bool first = j < it ? a[j] >= a[it] : (j > it && a[j] > a[it]);
+                    if (first && ((stay >> j) & 1)) before += kMass ? w[j] : 1;
                 }
                 if (((stay >> it) & 1) && before < target) keep |= 1u << it;
             }
             stay = keep;
             return;
         }
-        Key bound = 0;
-        for (int b = kBits - 1; b >= 0; --b) {
-            const Key cand = bound | ((Key)1 << b);
-            u64 f = 0;
-#pragma unroll
-            for (int it = 0; it < ITEMS; ++it)
-                if (key[it] >= cand && ((stay >> it) & 1)) f += metric(it);
-            f = t.reduce(f, OpSum());
-            if (f >= target) bound = cand;
-            if (f == target) break;
+        // [lo, hi): where the last class that stays lies; it is halved until it holds one class or
+        // one value
+        u64 mass = 0;
+        int n = 0;
+        auto from = [&](C least) {
+            mass = 0, n = 0;
+            LG_EACH(it) if (((stay >> it) & 1) && a[it] >= least) {
+                ++n;
+                if (kMass) mass += w[it];
+            }
+            n = team_count(t, n);
+            if (kMass) mass = t.sum(mass);
+            return (kMass ? mass : (u64)n) >= target;
+        };
+        C lo = m, hi = lg_inf(C());
+        if (!from(m)) {
+            if (m == lg_inf(C())) return;  // beside infinite logits the others weigh nothing
+            hi = m;
+            int n_hi = n;
+            C low = m;
+            LG_EACH(it) if ((stay >> it) & 1) low = a[it] < low ? a[it] : low;
+            low = t.reduce(low, OpMin());
+            lo = (C)((double)m - reach);
+            lo = low > lo ? low : lo;
+            if (!from(lo)) return;  // what would be cut weighs nothing
+            int n_lo = n;
+            while (n_lo - n_hi > 1) {
+                const C mid = lo * C(0.5) + hi * C(0.5);
+                if (!(mid > lo && mid < hi)) break;
+                if (from(mid)) lo = mid, n_lo = n;
+                else hi = mid, n_hi = n;
+            }
         }
         u64 above = 0, ties = 0;
-#pragma unroll
-        for (int it = 0; it < ITEMS; ++it)
-            if ((stay >> it) & 1) {
-                if (key[it] > bound) above += metric(it);
-                if (key[it] == bound) ties += metric(it);
-            }
-        // of equal keys the lower indices: the lanes' classes are in the order of the lanes
-        u64 before = t.reduce(above, OpSum()) + t.exscan(ties);
+        LG_EACH(it) if (((stay >> it) & 1) && a[it] >= lo) {
+            (a[it] >= hi && hi > lo ? above : ties) += kMass ? w[it] : 1;
+        }
+        // of equal logits the lower indices: the lanes' classes are in the order of the lanes
+        u64 before = t.sum(above) + t.exscan(ties);
         uint32_t keep = 0;
-#pragma unroll
-        for (int it = 0; it < ITEMS; ++it) {
-            if (!((stay >> it) & 1) || key[it] < bound) continue;
-            if (key[it] > bound || before < target) keep |= 1u << it;
-            if (key[it] == bound) before += metric(it);
+        LG_EACH(it) if (((stay >> it) & 1) && a[it] >= lo) {
+            const bool sure = a[it] >= hi && hi > lo;
+            if (sure || before < target) keep |= 1u << it;
+            if (!sure) before += kMass ? w[it] : 1;
         }
         stay = keep;
     };
     auto sum_of = [&](uint32_t bits) {
         u64 f = 0;
-#pragma unroll
-        for (int it = 0; it < ITEMS; ++it)
+        LG_EACH(it)
             if ((bits >> it) & 1) f += w[it];
         return f;
     };
-    if (rs.top_k < V) cut((u64)rs.top_k, [](int) { return 1ull; });
-    if (rs.top_p < 1.0) cut(mass_part(rs.top_p, t.reduce(sum_of(stay), OpSum())), [&](int it) { return w[it]; });
+    if (rs.top_k < V) cut((u64)rs.top_k, std::false_type());
+    if (rs.top_p < 1.0) cut(mass_part(rs.top_p, t.sum(sum_of(stay))), std::true_type());
     stay &= ~small;
     const u64 own = sum_of(stay);
     u64 upto = t.exscan(own);
-    const u64 target = draw_target(rs.u, t.reduce(own, OpSum()));
+    const u64 target = draw_target(rs.u, t.sum(own));
     int at = 0x7fffffff;
-#pragma unroll
-    for (int it = 0; it < ITEMS; ++it) {
+    LG_EACH(it) {
         if (!((stay >> it) & 1)) continue;
         if (upto < target && upto + w[it] >= target) at = mine.first + it;
         upto += w[it];
@@ -184,20 +200,17 @@ lg_sample_narrow_kernel(Rows<T> x, SampleArgs a, int shift, int tile, int direct
     }
     const LaneTeam<G> t;
     const Items<G, ITEMS> mine(t, V);
-    const double scale = __longlong_as_double((long long)(1023 + shift) << 52);
     for (int r = threadIdx.x / G; r < rows; r += kLgThreads / G) {
-        C v[ITEMS];
+        C v[ITEMS] = {};
         if (direct) {
             const T* row = g + r * x.row_stride;
-#pragma unroll
-            for (int it = 0; it < ITEMS; ++it)
+            LG_EACH(it)
                 v[it] = mine.has(it) ? to_c(row[(int64_t)(mine.first + it) * x.class_stride]) : C(0);
         } else {
             const T* row = s + (size_t)r * io.pitch;
-#pragma unroll
-            for (int it = 0; it < ITEMS; ++it) v[it] = mine.has(it) ? to_c(row[mine.first + it]) : C(0);
+            LG_EACH(it) v[it] = mine.has(it) ? to_c(row[mine.first + it]) : C(0);
         }
-        const int got = sample_row<T, G, ITEMS>(t, mine, v, V, scale, row_sampling(a, r0 + r, V));
+        const int got = sample_row<T, G, ITEMS>(t, mine, v, V, shift, row_sampling(a, r0 + r, V));
         if (t.rank == 0) index[r0 + r] = got;
     }
 }
@@ -591,7 +604,7 @@ int run_sample(const cbgpu_logits* x, const cbgpu_sampling* s, int32_t* index, c
     int bits = 0;
     while ((1 << bits) < rows.V) ++bits;
     const int shift = bits < 10 ? 52 : 62 - bits;  // at most what a 64-bit exponential holds
-    if (rows.V > kLgNarrow) {
+    if (is_wide(rows.n, rows.V)) {
         const Wide w = wide_shape<T>(rows.n, rows.V);
         return lg_launch_wide(who, lg_sample_wide_kernel<T>, rows.n, w, w.smem, st, w.ahead, rows, a, shift, index);
     }
@@ -601,10 +614,12 @@ int run_sample(const cbgpu_logits* x, const cbgpu_sampling* s, int32_t* index, c
         if (direct) t = Tile{kLgThreads, 0};
         return lg_launch(who, kernel, tiles_of(rows.n, t.rows), t.smem, st, rows, a, shift, t.rows, (int)direct, index);
     };
-    if (rows.V <= 8) return narrow(lg_sample_narrow_kernel<T, 1, 8>, 1);
+    if (rows.V <= 4) return narrow(lg_sample_narrow_kernel<T, 1, 4>, 1);
+    if (rows.V <= 12) return narrow(lg_sample_narrow_kernel<T, 1, 12>, 1);
     if (rows.V <= 16) return narrow(lg_sample_narrow_kernel<T, 1, 16>, 1);
+    if (rows.V <= 32) return narrow(lg_sample_narrow_kernel<T, 8, 4>, 8);
     if (rows.V <= 128) return narrow(lg_sample_narrow_kernel<T, 8, 16>, 8);
-    return narrow(lg_sample_narrow_kernel<T, 32, 32>, 32);
+    return narrow(lg_sample_narrow_kernel<T, 32, 16>, 32);
 }
 
 }  // namespace

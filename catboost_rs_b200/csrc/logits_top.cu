@@ -59,9 +59,8 @@ lg_top_narrow_kernel(Rows<T> x, int k, Scale<typename Num<T>::C> sc, int tile, T
         const T* row = s + (size_t)r * io.pitch;
         T* val = value + (r0 + r) * k;
         int32_t* idx = index + (r0 + r) * k;
-        Key key[ITEMS];
-#pragma unroll
-        for (int it = 0; it < ITEMS; ++it)
+        Key key[ITEMS] = {};
+        LG_EACH(it)
             key[it] = mine.has(it) ? (key_of(to_c(row[mine.first + it])) >> Num<T>::kKeyDrop) + 1 : 0;
         bool nan = false;  // among the first k
         if (!kLists || k <= kRounds) {
@@ -69,11 +68,11 @@ lg_top_narrow_kernel(Rows<T> x, int k, Scale<typename Num<T>::C> sc, int tile, T
             int at = 0;
             auto look = [&] {
                 best = 0;
-#pragma unroll
-                for (int it = 0; it < ITEMS; ++it) best = key[it] > best ? key[it] : best;
+                LG_EACH(it) best = key[it] > best ? key[it] : best;
                 at = 0;
 #pragma unroll
-                for (int it = ITEMS - 1; it >= 0; --it) at = key[it] == best ? it : at;
+                for (int it = ITEMS - 1; it >= 0; --it)
+                    at = key[it] == best ? it : at;
             };
             look();
             for (int j = 0; j < k; ++j) {
@@ -83,35 +82,36 @@ lg_top_narrow_kernel(Rows<T> x, int k, Scale<typename Num<T>::C> sc, int tile, T
                 if (best == top && i == mine.first + at) {
                     val[j] = row[i];
                     idx[j] = i;
-#pragma unroll
-                    for (int it = 0; it < ITEMS; ++it) key[it] = it == at ? 0 : key[it];
+                    LG_EACH(it) key[it] = it == at ? 0 : key[it];
                     look();
                 }
             }
         } else {
             TopList<Key>& list = lists[kLists ? threadIdx.x >> 5 : 0];
-            Key bound = 0;
-            int above = 0;  // keys past the k-th key's bits, once it is found
+            // the bits that all keys share come first
+            Key most = 0, least = ~(Key)0;
+            LG_EACH(it) if (mine.has(it)) most = key[it] > most ? key[it] : most, least = key[it] < least ? key[it] : least;
+            most = t.reduce(most, OpMax()), least = t.reduce(least, OpMin());
+            const int bits = most == least ? 0 : 64 - __clzll((long long)(u64)(most ^ least));
+            Key bound = bits < kBits ? most >> bits << bits : 0;
+            int above = 0;
             bool exact = false;
-            for (int b = kBits - 1; b >= 0 && !exact; --b) {
+            for (int b = bits - 1; b >= 0 && !exact; --b) {
                 const Key cand = bound | ((Key)1 << b);
                 int n = 0;
-#pragma unroll
-                for (int it = 0; it < ITEMS; ++it) n += key[it] >= cand;
+                LG_EACH(it) n += key[it] >= cand;
                 n = team_count(t, n);
                 if (n >= k) bound = cand;
                 exact = n == k;
             }
             int own = 0, ties = 0;
-#pragma unroll
-            for (int it = 0; it < ITEMS; ++it) own += key[it] > bound, ties += key[it] == bound;
+            LG_EACH(it) own += key[it] > bound, ties += key[it] == bound;
             above = team_count(t, own);
             // of equal keys the lower indices: the lanes' classes are in the order of the lanes
             int spare = k - above - (int)t.exscan((u64)ties);
             spare = spare < 0 ? 0 : (spare < ties ? spare : ties);
             int to = (int)t.exscan((u64)(own + spare));
-#pragma unroll
-            for (int it = 0; it < ITEMS; ++it) {
+            LG_EACH(it) {
                 const bool take = key[it] > bound || (key[it] == bound && spare > 0);
                 if (take && key[it] == bound) --spare;
                 if (take) {
@@ -132,13 +132,11 @@ lg_top_narrow_kernel(Rows<T> x, int k, Scale<typename Num<T>::C> sc, int tile, T
         }
         if (!tail) continue;
         C m = -lg_inf(C());
-#pragma unroll
-        for (int it = 0; it < ITEMS; ++it)
+        LG_EACH(it)
             if (key[it] != 0) m = OpMax()(m, to_c(row[mine.first + it]));
         m = floor_max(t.reduce(m, OpMax()));
         C part = 0;
-#pragma unroll
-        for (int it = 0; it < ITEMS; ++it)
+        LG_EACH(it)
             if (key[it] != 0) part += lg_exp(to_c(row[mine.first + it]) - m, sc.c);
         const double sum = t.reduce((double)part, OpSum());
         if (t.rank == 0) {
@@ -229,7 +227,7 @@ int run_top(const cbgpu_logits* x, int k, double temp, void* value, int32_t* ind
     const char* who = "top_logits";
     const Rows<T> rows = rows_of<T>(x);
     const Scale<C> sc(temp);
-    if (rows.V > kLgNarrow) {
+    if (is_wide(rows.n, rows.V)) {
         const Wide w = wide_shape<T>(rows.n, rows.V);
         return lg_launch_wide(who, lg_top_wide_kernel<T>, rows.n, w, w.smem, st, w.ahead, rows, k, sc, (T*)value, index,
                               (C*)tail);
@@ -239,10 +237,13 @@ int run_top(const cbgpu_logits* x, int k, double temp, void* value, int32_t* ind
         return lg_launch(who, kernel, tiles_of(rows.n, t.rows), t.smem, st, rows, k, sc, t.rows, (T*)value, index,
                          (C*)tail);
     };
-    if (rows.V <= 8) return narrow(lg_top_narrow_kernel<T, 1, 8>, 1);
+    if (rows.V <= 4) return narrow(lg_top_narrow_kernel<T, 1, 4>, 1);
+    if (rows.V <= 12) return narrow(lg_top_narrow_kernel<T, 1, 12>, 1);
     if (rows.V <= 16) return narrow(lg_top_narrow_kernel<T, 1, 16>, 1);
-    if (rows.V <= 128) return narrow(lg_top_narrow_kernel<T, 8, 16>, 8);
-    return narrow(lg_top_narrow_kernel<T, 32, 32>, 32);
+    if (rows.V <= 32 && k <= kRounds) return narrow(lg_top_narrow_kernel<T, 8, 4>, 8);
+    if (rows.V <= 128 && k <= kRounds) return narrow(lg_top_narrow_kernel<T, 8, 16>, 8);
+    if (rows.V <= 128) return narrow(lg_top_narrow_kernel<T, 32, 4>, 32);
+    return narrow(lg_top_narrow_kernel<T, 32, 16>, 32);
 }
 
 }  // namespace

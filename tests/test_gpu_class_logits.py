@@ -359,6 +359,51 @@ def test_sampling_frequencies_follow_the_softmax():
     assert np.abs(got - p).max() <= 1.5 / n
 
 
+# ---- many rows -------------------------------------------------------------------------
+# Rows of some hundred classes are worked on by a warp each where there are many of them, and wide rows
+# by fewer blocks each: every operator on whole batches, compared on some of the rows.
+
+MANY = [(1300, 129, "f32", "rows"), (1201, 300, "bf16", "offset"), (1185, 512, "f16", "rows"),
+        (1190, 257, "f64", "dims"), (1250, 64, "f32", "strided"), (1250, 513, "bf16", "rows"),
+        (200, 40007, "bf16", "rows"), (180, 33000, "f32", "offset"), (160, 20000, "f64", "rows")]
+
+
+def some(n):
+    return sorted({0, 1, n // 3, n // 2, n - 2, n - 1})
+
+
+@pytest.mark.parametrize("n,V,dtype,layout", MANY)
+def test_many_rows(n, V, dtype, layout):
+    x = make(n, V, dtype, layout, V)
+    wide = torch.float64 if dtype == "f64" else torch.float32
+    at = torch.tensor(some(n), device="cuda")
+    host_x = x.index_select(0, at)
+    for k in (5, 40):
+        top = cb.top_logits(x, k)
+        for j, r in enumerate(some(n)):
+            wi, wv, wt = ref.top(host(host_x[j:j + 1])[0], k, 1.0)
+            assert (top.index[r].cpu().numpy() == wi).all() and (host(top.value[r]) == wv).all()
+            assert abs(float(top.tail[r]) - wt) <= 130 * unit(dtype) + 3 * unit(dtype) * abs(wt)
+    t = make_teacher(n, V, 24, dtype, V + 1, True)
+    w = torch.linspace(0.5, 2.0, n, device="cuda", dtype=wide)
+    d = cb.distill_derivatives(x, t, weight=w, temperature=1.5)
+    for j, r in enumerate(some(n)):
+        wl, wd, p, q = ref.distill(host(host_x[j:j + 1])[0], t.index[r].cpu().numpy(), host(t.value[r]), float(t.tail[r]),
+                                   float(w[r]), 1.5)
+        rel = 2 * unit(dtype) * (3 * 40 + 4)  # reach <= 40, as in check_distill
+        assert abs(float(d.loss[r]) - wl) <= 2.25 * float(w[r]) * (2 * rel + 6 * unit(dtype) * 40) + 4 * unit(dtype) * wl
+        small = float(torch.finfo(x.dtype).smallest_normal) * float(torch.finfo(x.dtype).eps)
+        bound = float(w[r]) * 1.5 * rel * 2 * (p + q) + rounding(dtype) * np.abs(wd) + small
+        assert (np.abs(host(d.der1[r]) - wd) <= bound).all()
+    u = torch.rand((n,), generator=torch.Generator("cuda").manual_seed(V), device="cuda")
+    for kw in (dict(), dict(top_k=7), dict(top_p=0.8), dict(top_k=100, top_p=0.9, min_p=0.01), dict(min_p=0.2),
+               dict(top_k=300, top_p=0.97, temperature=2.0), dict(temperature=0.0)):
+        got = cb.sample_classes(x, u, **kw)
+        full = dict(dict(temperature=1.0, top_k=0, top_p=1.0, min_p=0.0), **kw)
+        for j, r in enumerate(some(n)):
+            assert int(got[r]) == ref.sample(host(host_x[j:j + 1])[0], float(u[r]), **full), (kw, r)
+
+
 # ---- how they are called ---------------------------------------------------------------
 
 def batch(V, dtype="bf16", n=130):
