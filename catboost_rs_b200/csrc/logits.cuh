@@ -321,7 +321,10 @@ template <typename Key>
 struct Ranked {  // a class in the operators' order
     Key key;
     uint32_t idx;
-    __device__ bool before(const Ranked& o) const { return key > o.key || (key == o.key && idx < o.idx); }
+    __device__ bool before(const Ranked& o) const {
+        if (sizeof(Key) == 4) return ((u64)key << 32 | (uint32_t)~idx) > ((u64)o.key << 32 | (uint32_t)~o.idx);
+        return key > o.key || (key == o.key && idx < o.idx);
+    }
 };
 template <typename Team, typename Key>
 __device__ __forceinline__ Ranked<Key> team_first(const Team& t, Ranked<Key> v) {
@@ -708,6 +711,7 @@ __device__ __forceinline__ void block_reduce(V (&v)[N], V (*scratch)[kLgWarps], 
 
 constexpr int kTopCap = 1024;  // classes the first block can collect
 
+constexpr int kHits = 512;
 constexpr int kBins = 1024;    // of the sampler's histogram, which lies where the list comes to lie
 struct SampleHist {
     float mass[kBins];
@@ -724,6 +728,8 @@ struct TopShared {
         SampleHist hist;
     };
     uint32_t bound[16][2];  // of every block: its k-th and its ceil(k / blocks)-th largest thread maximum
+    int base, vectors;
+    uint16_t hit[kHits];    // vectors that hold a class to collect
     u64 part[2][16];        // sums that go round the cluster
     u64 warp_part[kLgWarps];
     int count;
@@ -834,13 +840,39 @@ __device__ Ranked<typename Num<T>::Key> cluster_select(const ClusterInfo& cl, Sh
 // The first block's list in order; `n` entries, at most kTopCap.
 template <typename Key>
 __device__ void sort_list(TopShared<Key>& sh, int n) {
+    static_assert(kTopCap >= 2 * kLgThreads, "room for the ranked entries behind the list");
+    const int tid = threadIdx.x;
+    if (n <= kLgThreads) {  // every entry counts those before it, some threads an entry
+        int per = 1;
+        while (n * per * 2 <= kLgThreads) per *= 2;
+        const int c = tid / per;
+        const Ranked<Key> own{sh.key[c < n ? c : 0], sh.idx[c < n ? c : 0]};
+        int rank = 0;
+#pragma unroll 8
+        for (int i = tid & (per - 1); i < n; i += per) rank += Ranked<Key>{sh.key[i], sh.idx[i]}.before(own) ? 1 : 0;
+        for (int o = 1; o < per; o <<= 1) {
+            const int t = __shfl_xor_sync(0xffffffffu, rank, o & 31);
+            rank += o < 32 ? t : 0;
+        }
+        if (per > 32) {  // an entry's threads are whole warps
+            if (tid < n) sh.idx[kLgThreads + tid] = 0u;
+            __syncthreads();
+            if ((tid & 31) == 0 && c < n) atomicAdd(&sh.idx[kLgThreads + c], (uint32_t)rank);
+            __syncthreads();
+            rank = c < n ? (int)sh.idx[kLgThreads + c] : 0;
+        }
+        __syncthreads();
+        if (c < n && (tid & (per - 1)) == 0) sh.key[rank] = own.key, sh.idx[rank] = own.idx;
+        __syncthreads();
+        return;
+    }
     int size = 1;
     while (size < n) size *= 2;
-    for (int i = n + threadIdx.x; i < size; i += kLgThreads) sh.key[i] = 0, sh.idx[i] = 0xffffffffu;
+    for (int i = n + tid; i < size; i += kLgThreads) sh.key[i] = 0, sh.idx[i] = 0xffffffffu;
     __syncthreads();
     for (int len = 2; len <= size; len *= 2)
         for (int d = len / 2; d > 0; d /= 2) {
-            for (int p = threadIdx.x; p < size / 2; p += kLgThreads) {
+            for (int p = tid; p < size / 2; p += kLgThreads) {
                 const int i = (p & (d - 1)) | ((p & ~(d - 1)) << 1), j = i | d;
                 const Ranked<Key> a{sh.key[i], sh.idx[i]}, b{sh.key[j], sh.idx[j]};
                 if ((i & len) == 0 ? b.before(a) : a.before(b))
@@ -850,85 +882,132 @@ __device__ void sort_list(TopShared<Key>& sh, int n) {
         }
 }
 
+// The largest bound that at least `target` of a block's kLgThreads values in shared memory reach, to
+// 12 bits behind those that the values share; one warp.
+__device__ __forceinline__ uint32_t warp_bound(const uint32_t* of, int target) {
+    uint32_t v[kLgThreads / 32], most = 0, least = 0xffffffffu;
+#pragma unroll
+    for (int j = 0; j < kLgThreads / 32; ++j) {
+        v[j] = of[((int)threadIdx.x & 31) + 32 * j];
+        most = v[j] > most ? v[j] : most, least = v[j] < least ? v[j] : least;
+    }
+    most = __reduce_max_sync(0xffffffffu, most), least = __reduce_min_sync(0xffffffffu, least);
+    const int bits = 32 - __clz((int)(most ^ least));
+    uint32_t bound = bits < 32 ? most >> bits << bits : 0u;
+    for (int b = bits - 1; b >= 0 && b >= bits - 12; --b) {
+        const uint32_t cand = bound | (1u << b);
+        int n = 0;
+#pragma unroll
+        for (int j = 0; j < kLgThreads / 32; ++j) n += v[j] >= cand;
+        n = (int)__reduce_add_sync(0xffffffffu, (unsigned)n);
+        if (n >= target) bound = cand;
+        if (n == target) break;
+    }
+    return bound;
+}
+
 // Collects the row's first k classes, and perhaps some after them, in the
 // first block's list (not sorted; returns how many, in every thread); they are
 // replaced by -inf in the row, and `rest` gets the largest of this thread's classes
 // that stay.  `mine`: the largest of this thread's classes.  Every block of the cluster runs.
-template <typename T>
+// see(vector, least): this thread's vectors on the way, the collected classes as
+// -inf and what stays below `least`; not for the exact bound (`exact`), which leaves that to the caller.
+template <typename T, typename See>
 __device__ int wide_top(const ClusterInfo& cl, TopShared<typename Num<T>::Key>& sh, const WideRow<T>& w, uint4* s,
-                        typename Num<T>::C mine, int k, int& turn, typename Num<T>::C& rest) {
+                        typename Num<T>::C mine, int k, int& turn, typename Num<T>::C& rest, bool& exact, See see) {
     typedef typename Num<T>::C C;
     typedef typename Num<T>::Key Key;
-    constexpr int kDrop = (int)sizeof(Key) * 8 - 20;  // the bounds keep 20 bits of a key
-    const uint32_t top = (uint32_t)(key_of(mine) >> kDrop);
+    constexpr int kDrop = (int)sizeof(Key) * 8 - 32;  // the bounds keep 32 bits of a key
+    const int tid = threadIdx.x;
     const int share = (k + cl.blocks - 1) / cl.blocks;
-    uint32_t bk = 0, bs = 0;
-    for (int b = 19; b >= 0; --b) {
-        const uint32_t ck = bk | (1u << b), cs = bs | (1u << b);
-        if (__syncthreads_count(top >= ck) >= k) bk = ck;
-        if (share != k && __syncthreads_count(top >= cs) >= share) bs = cs;
+    sh.idx[tid] = (uint32_t)(key_of(mine) >> kDrop);
+    if (tid == 0) sh.count = 0, sh.vectors = 0;
+    __syncthreads();
+    if (tid < 64) {
+        const uint32_t b = warp_bound(sh.idx, tid < 32 ? k : share);
+        if ((tid & 31) < cl.blocks) cl.of(&sh.bound[cl.rank][0], tid & 31)[tid >> 5] = b;
     }
-    if (share == k) bs = bk;
-    if (threadIdx.x == 0) sh.count = 0;
-    if (cl.blocks > 1) {
-        if ((int)threadIdx.x < cl.blocks) {
-            uint32_t* to = cl.of(&sh.bound[cl.rank][0], (int)threadIdx.x);
-            to[0] = bk, to[1] = bs;
-        }
-        cl.sync();
-        bs = 0xffffffffu;
-        for (int b = 0; b < cl.blocks; ++b) {
-            bk = bk > sh.bound[b][0] ? bk : sh.bound[b][0];
-            bs = bs < sh.bound[b][1] ? bs : sh.bound[b][1];
-        }
-    } else {
-        __syncthreads();
+    cl.sync();
+    uint32_t bk = 0, bs = 0xffffffffu;
+    for (int b = 0; b < cl.blocks; ++b) {
+        bk = bk > sh.bound[b][0] ? bk : sh.bound[b][0];
+        bs = bs < sh.bound[b][1] ? bs : sh.bound[b][1];
     }
     const Key bound = (Key)(bk > bs ? bk : bs) << kDrop;
     const C least = bound <= key_of(-lg_inf(C())) ? -lg_inf(C()) : of_key(bound);
-    TopShared<Key>* first = cl.of(&sh, 0);
+    T* se = reinterpret_cast<T*>(s);
+    // a block collects in its own arrays; the first block's are the list
     auto take = [&](int i, C a, T* at) {
-        const int p = atomicAdd(&first->count, 1);
-        if (p < kTopCap) first->key[p] = key_of(a), first->idx[p] = (uint32_t)i;
+        const int p = atomicAdd(&sh.count, 1);
+        if (p < kTopCap) sh.key[p] = key_of(a), sh.idx[p] = (uint32_t)i;
         *at = from_c<T>(-lg_inf(C()));
     };
-    T* se = reinterpret_cast<T*>(s);
+    auto hand_over = [&] {
+        __syncthreads();
+        if (cl.rank != 0) {
+            TopShared<Key>* first = cl.of(&sh, 0);
+            const int n = sh.count < kTopCap ? sh.count : kTopCap;
+            if (tid == 0 && n > 0) sh.base = atomicAdd(&first->count, sh.count);
+            __syncthreads();
+            for (int p = tid; p < n; p += kLgThreads)
+                if (sh.base + p < kTopCap) first->key[sh.base + p] = sh.key[p], first->idx[sh.base + p] = sh.idx[p];
+        }
+        cl.sync();
+    };
     constexpr int VE = WideRow<T>::VE;
     rest = -lg_inf(C());
-    for (int v = threadIdx.x; v < w.nv; v += kLgThreads) {
+    exact = false;
+    // vectors that hold one are noted, so that a warp does not go through their classes for each of them
+    auto open = [&](int v) {
+        C a[VE];
+        unpack(s[v], a, T());
+        const int i = w.first(v);
+#pragma unroll
+        for (int j = 0; j < VE; ++j) {
+            if (a[j] >= least && i + j >= 0 && i + j < w.V) {
+                take(i + j, a[j], se + v * VE + j);
+                a[j] = -lg_inf(C());
+            } else {
+                rest = OpMax()(rest, a[j]);
+            }
+        }
+        see(a, least);
+    };
+#pragma unroll 2
+    for (int v = tid; v < w.nv; v += kLgThreads) {
         const uint4 q = s[v];
         VecMax<T> m;
         m(q);
         if (m.get() < least) {
             rest = OpMax()(rest, m.get());
-            continue;
-        }
-        C a[VE];
-        unpack(q, a, T());
-        const int i = w.first(v);
-#pragma unroll
-        for (int j = 0; j < VE; ++j) {
-            if (a[j] >= least && i + j >= 0 && i + j < w.V) take(i + j, a[j], se + v * VE + j);
-            else rest = OpMax()(rest, a[j]);
+            C a[VE];
+            unpack(q, a, T());
+            see(a, least);
+        } else {
+            const int p = atomicAdd(&sh.vectors, 1);
+            if (p < kHits) sh.hit[p] = (uint16_t)v;
+            else open(v);
         }
     }
-    cl.sync();
-    int n = first->count;
+    __syncthreads();
+    for (int p = tid; p < sh.vectors && p < kHits; p += kLgThreads) open(sh.hit[p]);
+    hand_over();
+    const int n = cl.of(&sh, 0)->count;
     if (n >= k && n <= kTopCap) return n;
     // the exact bound, on the row as it was
+    exact = true;
     cl.sync();
-    if (cl.rank == 0 && threadIdx.x == 0) sh.count = 0;
+    if (tid == 0) sh.count = 0;
     w.load(s, [](const uint4&) {});
     __syncthreads();
-    const Ranked<Key> last =
-        cluster_select(cl, sh, w, s, (u64)k, turn, [](int, C, Key) { return 1ull; });
+    const Ranked<Key> last = cluster_select(cl, sh, w, s, (u64)k, turn, [](int, C, Key) { return 1ull; });
     rest = -lg_inf(C());
     __syncthreads();
     each_class(w, s, [&](int i, C a, int at) {
         if (last.before(Ranked<Key>{key_of(a), (uint32_t)i})) rest = OpMax()(rest, a);
         else take(i, a, se + at);
     });
-    cl.sync();
+    hand_over();
     return k;
 }
 

@@ -245,7 +245,7 @@ struct Weigh {
     }
 };
 
-constexpr int kSegments = 8192 / 32 + 1;  // of 32 vectors; the largest row's blocks hold 8192
+constexpr int kSegments = 8192 / 32 + 1 > kLgThreads ? 8192 / 32 + 1 : kLgThreads;  // of 32 vectors; a block holds up to 8193
 
 // Exclusive scan of a value a thread over the block.
 __device__ __forceinline__ u64 block_exscan(u64 v, u64 (&warp_part)[kLgWarps]) {
@@ -417,7 +417,8 @@ lg_sample_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, SampleArg
                    Ranked<Key>{0, 0xffffffffu}, false};
     if (rs.top_k <= kLgMaxTop) {
         C rest;
-        const int n = wide_top(cl, sh, w, s, mine, rs.top_k, turn, rest);
+        bool exact;
+        const int n = wide_top(cl, sh, w, s, mine, rs.top_k, turn, rest, exact, [](C(&)[WideRow<T>::VE], C) {});
         if (cl.blocks > 1) cl.sync();  // no block leaves while another reads its shared memory
         if (cl.rank != 0) return;
         __syncthreads();

@@ -155,15 +155,15 @@ lg_top_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, int k, Scale
     constexpr int VE = WideRow<T>::VE;
     extern __shared__ __align__(16) unsigned char lg_smem[];
     __shared__ TopShared<Key> sh;
-    __shared__ C red_max[1][kLgWarps];
-    __shared__ double red[1][kLgWarps];
+    __shared__ C red_max[kLgWarps];
+    __shared__ double red[kLgWarps];
     __shared__ struct {
         double sum;
         C max;
     } parts[16];
     uint4* s = reinterpret_cast<uint4*>(lg_smem);
     const ClusterInfo cl;
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, lane = tid & 31, warp_id = tid >> 5;
     const int64_t r = row0 + (int64_t)(blockIdx.x / (unsigned)cl.blocks);
     const WideRow<T> w(x, r, cl.rank, per);
     if (cl.blocks > 1) cluster_arrive<false>();
@@ -172,28 +172,47 @@ lg_top_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, int k, Scale
     w.load(s, [&](const uint4& q) { most(q); });
     if (cl.blocks > 1) cluster_wait();  // every block runs
     int turn = 0;
-    C rest;
-    const int n = wide_top(cl, sh, w, s, most.get(), k, turn, rest);
-    if (tail) {  // the log-sum-exp of what stayed in the row, and of the list behind its first k
-        C m[1] = {rest};
-        block_reduce(m, red_max, OpMax());
-        const Base<C> here(floor_max(m[0]), sc);
-        double sum[1] = {0.0};
-        auto add = [&](auto huge) {
-#pragma unroll 4
+    C rest, ref = C(0);
+    bool exact;
+    double sum = 0.0;
+    // the tail's sum is taken on the way, relative to the least class that is collected
+    const int n = wide_top(cl, sh, w, s, most.get(), k, turn, rest, exact, [&](C(&a)[VE], C least) {
+        if (!tail) return;
+        ref = floor_max(least);
+        const Base<C> at(ref, sc);
+        if (at.huge) at.template exps<true>(a);
+        else at.template exps<false>(a);
+        sum += Base<C>::total(a);
+    });
+    if (tail) {
+        sum = warp_sum(sum, 32);
+        rest = warp_max(rest);
+        if (lane == 0) red[warp_id] = sum, red_max[warp_id] = rest;
+        __syncthreads();
+        sum = red[0], rest = red_max[0];
+#pragma unroll
+        for (int i = 1; i < kLgWarps; ++i) sum += red[i], rest = OpMax()(rest, red_max[i]);
+        if (exact || (sum < 1e-20 && rest > -lg_inf(C()))) {  // the rest lies far below: relative to its own largest
+            __syncthreads();
+            ref = floor_max(rest);
+            const Base<C> at(ref, sc);
+            double part = 0.0;
             for (int v = tid; v < w.nv; v += kLgThreads) {
                 C a[VE];
                 unpack(s[v], a, T());
-                here.template exps<decltype(huge)::value>(a);
-                sum[0] += Base<C>::total(a);
+                if (at.huge) at.template exps<true>(a);
+                else at.template exps<false>(a);
+                part += Base<C>::total(a);
             }
-        };
-        if (here.huge) add(std::true_type());
-        else add(std::false_type());
-        block_reduce(sum, red, OpSum());
+            part = warp_sum(part, 32);
+            if (lane == 0) red[warp_id] = part;
+            __syncthreads();
+            sum = red[0];
+            for (int i = 1; i < kLgWarps; ++i) sum += red[i];
+        }
         if (tid == 0) {
             auto* to = cl.of(&parts[cl.rank], 0);
-            to->max = m[0], to->sum = sum[0];
+            to->max = ref, to->sum = sum;
         }
     }
     if (cl.blocks > 1) cl.sync();  // also: no block leaves while another reads its shared memory
@@ -205,13 +224,13 @@ lg_top_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, int k, Scale
         index[r * k + j] = (int32_t)sh.idx[j];
     }
     if (!tail || tid >= 32) return;
-    C m = tid < cl.blocks ? parts[tid].max : -lg_inf(C());
+    // only parts that hold something have a say in the base; the list behind its first k is below it
+    const bool has = tid < cl.blocks && parts[tid].sum != 0.0;
+    C m = has ? parts[tid].max : -lg_inf(C());
     if (tid == 0 && n > k) m = OpMax()(m, of_key(sh.key[k]));
     m = warp_max(m);
     const Base<C> base(floor_max(m), sc);
-    double sum = 0.0;
-    if (tid < cl.blocks && parts[tid].sum != 0.0)
-        sum = parts[tid].sum * exp(Base<C>(floor_max(parts[tid].max), sc).ln_shift(base));
+    sum = has ? parts[tid].sum * exp(Base<C>(parts[tid].max, sc).ln_shift(base)) : 0.0;
     for (int j = k + tid; j < n; j += 32) sum += (double)base.exp(of_key(sh.key[j]));
     sum = warp_sum(sum, 32);
     if (tid == 0) {
