@@ -356,7 +356,7 @@ struct WideRow {
         nv = all - v0 < per ? all - v0 : per;
     }
     __device__ int first(int v) const { return (v0 + v) * VE - head; }  // class of vector v's first element
-    __device__ bool whole(int i) const { return i >= 0 && i + VE <= V; }
+    __device__ bool valid(int i) const { return i >= 0 && i < V; }
     __device__ int slot(int i) const {  // where class i lies in this block's memory, or -1
         const int at = i + head - v0 * VE;
         return at >= 0 && at < nv * VE ? at : -1;
@@ -712,6 +712,8 @@ __device__ __forceinline__ void block_reduce(V (&v)[N], V (*scratch)[kLgWarps], 
 constexpr int kTopCap = 1024;  // classes the first block can collect
 
 constexpr int kHits = 512;
+constexpr int kSegments = 8192 / 32 + 1;  // a block holds up to 8193 vectors
+constexpr int kGather = 3;
 constexpr int kBins = 1024;    // of the sampler's histogram, which lies where the list comes to lie
 struct SampleHist {
     float mass[kBins];
@@ -726,12 +728,14 @@ struct TopShared {
             uint32_t idx[kTopCap];
         };
         SampleHist hist;
+        u64 segment[kSegments];  // the sampler's masses of 32 vectors each
     };
     uint32_t bound[16][2];  // of every block: its k-th and its ceil(k / blocks)-th largest thread maximum
+    uint32_t flag[16];
     int base, vectors;
     uint16_t hit[kHits];    // vectors that hold a class to collect
-    u64 part[2][16];        // sums that go round the cluster
-    u64 warp_part[kLgWarps];
+    u64 part[2][16][kGather];  // values that go round the cluster
+    u64 warp_part[kGather][kLgWarps];
     int count;
 };
 
@@ -756,35 +760,61 @@ struct ClusterInfo {
     }
 };
 
-// A value of each block's first thread, to sh.part[the turn before][block] of every block.  `turn`
-// alternates between calls.
-template <typename Sh>
-__device__ const u64* cluster_gather(const ClusterInfo& cl, Sh& sh, u64 v, int& turn) {
-    if ((int)threadIdx.x < 32) {
-        v = __shfl_sync(0xffffffffu, v, 0);
-        if ((int)threadIdx.x < cl.blocks) *cl.of(&sh.part[turn][cl.rank], (int)threadIdx.x) = v;
+// N values of each block's first warp (the same in its lanes), to sh.part[the turn before][block][0..N)
+// of every block.  `turn` alternates between calls.
+template <int N, typename Sh>
+__device__ const u64 (*cluster_gather(const ClusterInfo& cl, Sh& sh, const u64 (&v)[N], int& turn))[kGather] {
+    static_assert(N <= kGather, "words a block");
+    if ((int)threadIdx.x < cl.blocks) {
+        u64* to = cl.of(&sh.part[turn][cl.rank][0], (int)threadIdx.x);
+#pragma unroll
+        for (int i = 0; i < N; ++i) to[i] = v[i];
     }
     cl.sync();
     turn ^= 1;
     return sh.part[turn ^ 1];
 }
 
-// Sum over the cluster of a value a thread, in every thread.
+// Sums over the cluster of N values a thread (each below 2^62 in all), in every thread.
+template <int N, typename Sh>
+__device__ void cluster_total(const ClusterInfo& cl, Sh& sh, u64 (&v)[N], int& turn) {
+    const LaneTeam<32> warp;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        v[i] = warp.sum(v[i]);
+        if (warp.rank == 0) sh.warp_part[i][threadIdx.x >> 5] = v[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        v[i] = 0;
+        for (int j = 0; j < kLgWarps; ++j) v[i] += sh.warp_part[i][j];
+    }
+    const u64(*of)[kGather] = cluster_gather<N>(cl, sh, v, turn);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        v[i] = 0;
+        for (int b = 0; b < cl.blocks; ++b) v[i] += of[b][i];
+    }
+}
 template <typename Sh>
 __device__ u64 cluster_total(const ClusterInfo& cl, Sh& sh, u64 v, int& turn) {
-    v = warp_sum(v, 32);
-    if ((threadIdx.x & 31) == 0) sh.warp_part[threadIdx.x >> 5] = v;
-    __syncthreads();
-    if ((int)threadIdx.x < cl.blocks) {
-        u64 t = 0;
-        for (int i = 0; i < kLgWarps; ++i) t += sh.warp_part[i];
-        *cl.of(&sh.part[turn][cl.rank], (int)threadIdx.x) = t;
+    u64 one[1] = {v};
+    cluster_total<1>(cl, sh, one, turn);
+    return one[0];
+}
+
+// fn(class, logit, place) for every place of this thread's vectors, also those outside the row (-inf; valid() tells)
+template <typename T, typename Fn>
+__device__ __forceinline__ void each_place(const WideRow<T>& w, const uint4* s, Fn fn) {
+    constexpr int VE = WideRow<T>::VE;
+    for (int v = threadIdx.x; v < w.nv; v += kLgThreads) {
+        typename Num<T>::C a[VE];
+        unpack(s[v], a, T());
+        const int i = w.first(v);
+#pragma unroll
+        for (int j = 0; j < VE; ++j) fn(i + j, a[j], v * VE + j);
     }
-    cl.sync();
-    u64 t = 0;
-    for (int b = 0; b < cl.blocks; ++b) t += sh.part[turn][b];
-    turn ^= 1;
-    return t;
 }
 
 // fn(class, logit) for this thread's classes
@@ -912,9 +942,11 @@ __device__ __forceinline__ uint32_t warp_bound(const uint32_t* of, int target) {
 // that stay.  `mine`: the largest of this thread's classes.  Every block of the cluster runs.
 // see(vector, least): this thread's vectors on the way, the collected classes as
 // -inf and what stays below `least`; not for the exact bound (`exact`), which leaves that to the caller.
+// `flag`: whether any thread of the cluster came with it set.
 template <typename T, typename See>
 __device__ int wide_top(const ClusterInfo& cl, TopShared<typename Num<T>::Key>& sh, const WideRow<T>& w, uint4* s,
-                        typename Num<T>::C mine, int k, int& turn, typename Num<T>::C& rest, bool& exact, See see) {
+                        typename Num<T>::C mine, int k, int& turn, typename Num<T>::C& rest, bool& exact, bool& flag,
+                        See see) {
     typedef typename Num<T>::C C;
     typedef typename Num<T>::Key Key;
     constexpr int kDrop = (int)sizeof(Key) * 8 - 32;  // the bounds keep 32 bits of a key
@@ -922,16 +954,20 @@ __device__ int wide_top(const ClusterInfo& cl, TopShared<typename Num<T>::Key>& 
     const int share = (k + cl.blocks - 1) / cl.blocks;
     sh.idx[tid] = (uint32_t)(key_of(mine) >> kDrop);
     if (tid == 0) sh.count = 0, sh.vectors = 0;
-    __syncthreads();
+    flag = __syncthreads_or(flag) != 0;
     if (tid < 64) {
         const uint32_t b = warp_bound(sh.idx, tid < 32 ? k : share);
-        if ((tid & 31) < cl.blocks) cl.of(&sh.bound[cl.rank][0], tid & 31)[tid >> 5] = b;
+        if ((tid & 31) < cl.blocks) {
+            cl.of(&sh.bound[cl.rank][0], tid & 31)[tid >> 5] = b;
+            if (tid < 32) *cl.of(&sh.flag[cl.rank], tid) = flag;
+        }
     }
     cl.sync();
     uint32_t bk = 0, bs = 0xffffffffu;
     for (int b = 0; b < cl.blocks; ++b) {
         bk = bk > sh.bound[b][0] ? bk : sh.bound[b][0];
         bs = bs < sh.bound[b][1] ? bs : sh.bound[b][1];
+        flag |= sh.flag[b] != 0;
     }
     const Key bound = (Key)(bk > bs ? bk : bs) << kDrop;
     const C least = bound <= key_of(-lg_inf(C())) ? -lg_inf(C()) : of_key(bound);

@@ -57,6 +57,8 @@ __device__ __forceinline__ u64 draw_target(double u, u64 total) {
     return (down >= 64 ? hi >> (down - 64) : (hi << (64 - down)) | (lo >> down)) + 1ull;
 }
 
+__device__ __forceinline__ double power_of_2(int e) { return __longlong_as_double((long long)(1023 + e) << 52); }
+
 // rint(e 2^s) through the lowest bits of 2^52 + e 2^s
 __device__ __forceinline__ u64 whole_mass(double e, double scale) {
     return (u64)__double_as_longlong(fma(e, scale, 4503599627370496.0)) - 0x4330000000000000ull;
@@ -69,7 +71,7 @@ template <typename T, int G, int ITEMS>
 __device__ int sample_row(const LaneTeam<G>& t, const Items<G, ITEMS>& mine, const typename Num<T>::C (&a)[ITEMS], int V,
                           int shift, const RowSampling& rs) {
     typedef typename Num<T>::C C;
-    const double scale = __longlong_as_double((long long)(1023 + shift) << 52);
+    const double scale = power_of_2(shift);
     const double reach = (double)(shift + 2) * 0.6931471805599453 / rs.inv_t;  // behind it a weight is 0
     C m = -lg_inf(C());
     int bad = 0;
@@ -223,6 +225,32 @@ lg_sample_narrow_kernel(Rows<T> x, SampleArgs a, int shift, int tile, int direct
 // the bin's classes are collected and sorted, and the cut is then taken with
 // exact masses, which also show whether the bin was the right one.
 
+// exp of a non-positive number by the table-driven method of P. T. P. Tang (ACM TOMS 15, 1989): with
+// x log2(e) = n / 64 + r / 64, |r| <= 1/2, it is 2^(n / 64), from a table of 64 and an exponent, times a polynomial
+// in r ln2 / 64 (below 0.0055: degree 5 leaves 4e-17).  12 operations in 64 bits with what Weigh adds; exp()
+// takes two to three times as many, and the draw from whole rows is bound by them.
+constexpr int kExpTable = 64;
+struct ExpTable {
+    double of[kExpTable];
+    __device__ void fill() {  // by the block; a barrier follows
+        if (threadIdx.x < kExpTable) of[threadIdx.x] = exp2((double)threadIdx.x / kExpTable);
+    }
+    // 2^(y / 64), y in (-64 * 1000, 0]
+    __device__ double operator()(double y) const {
+        const double t = y + 6755399441055744.0;  // 1.5 2^52: the low word of t is n
+        const int n = __double2loint(t);
+        const double r = y - (t - 6755399441055744.0);
+        constexpr double c = 0.6931471805599453 / kExpTable;
+        double p = fma(r, c * c * c * c * c / 120.0, c * c * c * c / 24.0);
+        p = fma(r, p, c * c * c / 6.0);
+        p = fma(r, p, c * c / 2.0);
+        p = fma(r, p, c);
+        const double b = of[n & (kExpTable - 1)];
+        const double e = fma(b * r, p, b);
+        return __hiloint2double(__double2hiint(e) + ((n >> 6) << 20), __double2loint(e));
+    }
+};
+
 template <typename T>
 struct Weigh {
     typedef typename Num<T>::C C;
@@ -231,7 +259,16 @@ struct Weigh {
     double inv_t, scale, min_p;
     Ranked<Key> last;  // the last class that stays
     bool cut;
-    __device__ double share(C a) const { return a == m ? 1.0 : exp(((double)a - (double)m) * inv_t); }
+    const ExpTable* table;
+    double per64;  // 64 log2(e) / T
+    __device__ Weigh(C m_, double inv_t_, int shift, const ExpTable* t)
+        : m(m_), inv_t(inv_t_), scale(power_of_2(shift)), min_p(0.0),
+          last{0, 0xffffffffu}, cut(false), table(t), per64(inv_t_ * (kExpTable * 1.4426950408889634)) {}
+    __device__ double share(C a) const {
+        const double y = ((double)a - (double)m) * per64;
+        const double e = (*table)(fmax(y, -64.0 * 1000.0));
+        return a == m ? 1.0 : (y > -64.0 * 60.0 ? e : 0.0);  // 2^-60: less than half of any last bit
+    }
     __device__ u64 whole(double e) const { return whole_mass(e, scale); }
     __device__ u64 mass(C a) const { return whole(share(a)); }
     __device__ bool stays(int i, C a) const {
@@ -245,10 +282,8 @@ struct Weigh {
     }
 };
 
-constexpr int kSegments = 8192 / 32 + 1 > kLgThreads ? 8192 / 32 + 1 : kLgThreads;  // of 32 vectors; a block holds up to 8193
-
-// Exclusive scan of a value a thread over the block.
-__device__ __forceinline__ u64 block_exscan(u64 v, u64 (&warp_part)[kLgWarps]) {
+// Exclusive scan of a value a thread over the block, and the block's sum.
+__device__ __forceinline__ u64 block_exscan(u64 v, u64 (&warp_part)[kLgWarps], u64& total) {
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
     u64 inc = v;
     for (int o = 1; o < 32; o <<= 1) {
@@ -258,13 +293,16 @@ __device__ __forceinline__ u64 block_exscan(u64 v, u64 (&warp_part)[kLgWarps]) {
     if (lane == 31) warp_part[wid] = inc;
     __syncthreads();
     u64 base = 0;
-    for (int i = 0; i < wid; ++i) base += warp_part[i];
+    total = 0;
+    for (int i = 0; i < kLgWarps; ++i) {
+        if (i == wid) base = total;
+        total += warp_part[i];
+    }
     __syncthreads();
     return base + inc - v;
 }
-
 __device__ __forceinline__ u64 block_total(u64 v, u64 (&warp_part)[kLgWarps]) {
-    v = warp_sum(v, 32);
+    v = LaneTeam<32>().sum(v);
     if ((threadIdx.x & 31) == 0) warp_part[threadIdx.x >> 5] = v;
     __syncthreads();
     u64 t = 0;
@@ -275,10 +313,12 @@ __device__ __forceinline__ u64 block_total(u64 v, u64 (&warp_part)[kLgWarps]) {
 
 // Draws from the classes that stay; every block of the cluster, one of them writes.
 template <typename T, typename Sh>
-__device__ void wide_draw(const ClusterInfo& cl, Sh& sh, u64* seg, const WideRow<T>& w, const uint4* s,
+__device__ void wide_draw(const ClusterInfo& cl, Sh& sh, const WideRow<T>& w, const uint4* s,
                           const Weigh<T>& weigh, double u, int& turn, int32_t* index) {
     constexpr int VE = WideRow<T>::VE;
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+    const LaneTeam<32> warp;
+    u64* seg = sh.segment;  // in place of the list: no block is at it any more
     auto lane_mass = [&](int v) {
         u64 own = 0;
         if (v < w.nv) {
@@ -291,26 +331,25 @@ __device__ void wide_draw(const ClusterInfo& cl, Sh& sh, u64* seg, const WideRow
     };
     const int segs = w.nv > 0 ? (w.nv + 31) / 32 : 0;
     for (int g = wid; g < segs; g += kLgWarps) {
-        const u64 sum = warp_sum(lane_mass(g * 32 + lane), 32);
+        const u64 sum = warp.sum(lane_mass(g * 32 + lane));
         if (lane == 0) seg[g] = sum;
     }
     __syncthreads();
     // a run of segments a thread
     const int per = (segs + kLgThreads - 1) / kLgThreads, g0 = (int)threadIdx.x * per;
-    u64 own = 0;
+    u64 own = 0, block[1];
     for (int g = g0; g < g0 + per && g < segs; ++g) own += seg[g];
-    u64 upto = block_exscan(own, sh.warp_part);
-    const u64* of = cluster_gather(cl, sh, block_total(own, sh.warp_part), turn);
+    u64 upto = block_exscan(own, sh.warp_part[0], block[0]);
+    const u64(*of)[kGather] = cluster_gather<1>(cl, sh, block, turn);
     u64 total = 0, before = 0;
     for (int b = 0; b < cl.blocks; ++b) {
         if (b == cl.rank) before = total;
-        total += of[b];
+        total += of[b][0];
     }
     const u64 target = draw_target(u, total);
+    if (!(before < target && before + block[0] >= target)) return;  // another block's
     __shared__ int s_seg;
     __shared__ u64 s_upto;
-    if (threadIdx.x == 0) s_seg = -1;
-    __syncthreads();
     upto += before;
     if (upto < target && upto + own >= target)
         for (int g = g0;; ++g) {
@@ -321,15 +360,10 @@ __device__ void wide_draw(const ClusterInfo& cl, Sh& sh, u64* seg, const WideRow
             upto += seg[g];
         }
     __syncthreads();
-    if (s_seg < 0 || wid != 0) return;
+    if (wid != 0) return;
     const int v = s_seg * 32 + lane;
     const u64 mine = lane_mass(v);
-    u64 inc = mine;
-    for (int o = 1; o < 32; o <<= 1) {
-        const u64 t = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += t;
-    }
-    u64 sum = s_upto + inc - mine;
+    u64 sum = s_upto + warp.exscan(mine);
     if (sum < target && sum + mine >= target) {
         typename Num<T>::C a[VE];
         unpack(s[v], a, T());
@@ -344,21 +378,25 @@ __device__ void wide_draw(const ClusterInfo& cl, Sh& sh, u64* seg, const WideRow
 
 // The draw from the first block's sorted list of k <= kLgThreads classes: a thread a class.
 template <typename T, typename Sh>
-__device__ void list_draw(Sh& sh, int k, const Weigh<T>& weigh, const RowSampling& rs, u64* w_of, int32_t* index) {
+__device__ void list_draw(Sh& sh, int k, const Weigh<T>& weigh, const RowSampling& rs, int32_t* index) {
     typedef typename Num<T>::C C;
     const int j = threadIdx.x;
+    static_assert(kTopCap - 512 >= 2 * kLgThreads, "masses behind the list");
+    u64* w_of = reinterpret_cast<u64*>(&sh.idx[512]);
     const double e = j < k ? weigh.share((C)of_key(sh.key[j])) : 0.0;
     u64 own = j < k ? weigh.whole(e) : 0;
     if (rs.top_p < 1.0) {
-        const u64 before = block_exscan(own, sh.warp_part);
-        if (before >= mass_part(rs.top_p, block_total(own, sh.warp_part))) own = 0;
+        u64 total;
+        const u64 before = block_exscan(own, sh.warp_part[0], total);
+        if (before >= mass_part(rs.top_p, total)) own = 0;
     }
     if (e < rs.min_p) own = 0;
-    const u64 target = draw_target(rs.u, block_total(own, sh.warp_part));
+    const u64 target = draw_target(rs.u, block_total(own, sh.warp_part[0]));
     w_of[j] = own;
     __syncthreads();
     if (own == 0) return;
     u64 upto = 0;  // of the kept classes before this one by index
+#pragma unroll 8
     for (int i = 0; i < k; ++i) upto += sh.idx[i] < sh.idx[j] ? w_of[i] : 0;
     if (upto < target && upto + own >= target) *index = (int32_t)sh.idx[j];
 }
@@ -371,10 +409,9 @@ lg_sample_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, SampleArg
     typedef typename Num<T>::Key Key;
     extern __shared__ __align__(16) unsigned char lg_smem[];
     __shared__ TopShared<Key> sh;
-    __shared__ u64 seg[kSegments];
-    static_assert(kSegments >= kLgThreads, "list_draw's masses");
-    __shared__ C red_max[1][kLgWarps];
+    __shared__ C red_max[2][kLgWarps];
     __shared__ Ranked<Key> s_cut;
+    __shared__ ExpTable table;
     uint4* s = reinterpret_cast<uint4*>(lg_smem);
     const ClusterInfo cl;
     const int tid = threadIdx.x;
@@ -384,64 +421,72 @@ lg_sample_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, SampleArg
     if (tid == 0 && r + ahead < x.n) WideRow<T>(x, r + ahead, cl.rank, per).prefetch();
     VecMaxNan<T> most;
     w.load(s, [&](const uint4& q) { most(q); });
+    table.fill();
     const RowSampling rs = row_sampling(a, r, x.V);
     const C mine = most.get();
-    C m[1] = {mine};
-    block_reduce(m, red_max, [](C p, C q) { return VecMaxNan<C>::both(p, q); });
-    if (cl.blocks > 1) cluster_wait();  // every block runs: its shared memory can be written
-    int turn = 0;
-    {
-        const u64* of = cluster_gather(cl, sh, (u64)__double_as_longlong((double)m[0]), turn);
-        for (int b = 0; b < cl.blocks; ++b) m[0] = VecMaxNan<C>::both(m[0], (C)__longlong_as_double((long long)of[b]));
-    }
     int32_t* out = index + r;
-    if (m[0] != m[0] || m[0] == -lg_inf(C())) {  // a NaN, or every class masked
+    int turn = 0;
+    if (cl.blocks > 1) cluster_wait();  // every block runs: its shared memory can be written
+    if (rs.top_k <= kLgMaxTop && !rs.greedy) {
+        C rest;
+        bool exact, bad = mine != mine;
+        const int n = wide_top(cl, sh, w, s, bad ? -lg_inf(C()) : mine, rs.top_k, turn, rest, exact, bad,
+                               [](C(&)[WideRow<T>::VE], C) {});
+        if (cl.blocks > 1) cl.sync();  // no block leaves while another reads its shared memory
+        if (cl.rank != 0) return;
+        __syncthreads();
+        sort_list(sh, n);
+        const C m = (C)of_key(sh.key[0]);
+        if (bad || m == -lg_inf(C())) {
+            if (tid == 0) *out = -1;
+            return;
+        }
+        list_draw<T>(sh, rs.top_k, Weigh<T>(m, rs.inv_t, shift, &table), rs, out);
+        return;
+    }
+    // the largest logit, and the least that is not masked (negated)
+    C low = -lg_inf(C());
+    if (rs.top_k < x.V || rs.top_p < 1.0)
+        each_place(w, s, [&](int, C v, int) { low = v != -lg_inf(C()) ? OpMax()(low, -v) : low; });
+    C ends[2] = {mine, low};
+    block_reduce(ends, red_max, [](C p, C q) { return VecMaxNan<C>::both(p, q); });
+    {
+        const u64 v[2] = {(u64)__double_as_longlong((double)ends[0]), (u64)__double_as_longlong((double)ends[1])};
+        const u64(*of)[kGather] = cluster_gather<2>(cl, sh, v, turn);
+        for (int b = 0; b < cl.blocks; ++b) {
+            ends[0] = VecMaxNan<C>::both(ends[0], (C)__longlong_as_double((long long)of[b][0]));
+            ends[1] = OpMax()(ends[1], (C)__longlong_as_double((long long)of[b][1]));
+        }
+    }
+    const C m = ends[0];
+    if (m != m || m == -lg_inf(C())) {  // a NaN, or every class masked
         if (cl.rank == 0 && tid == 0) *out = -1;
         return;
     }
     if (rs.greedy) {
         uint32_t at = 0xffffffffu;
-        each_class(w, s, [&](int i, C v, int) { at = v == m[0] && (uint32_t)i < at ? (uint32_t)i : at; });
+        each_class(w, s, [&](int i, C v, int) { at = v == m && (uint32_t)i < at ? (uint32_t)i : at; });
         at = __reduce_min_sync(0xffffffffu, at);
         if (tid == 0) sh.count = 0x7fffffff;
         __syncthreads();
         if ((tid & 31) == 0) atomicMin(&sh.count, (int)(at & 0x7fffffffu));
         __syncthreads();
-        const u64* of = cluster_gather(cl, sh, (u64)sh.count, turn);
-        u64 first = of[0];
-        for (int b = 1; b < cl.blocks; ++b) first = first < of[b] ? first : of[b];
+        const u64 v[1] = {(u64)sh.count};
+        const u64(*of)[kGather] = cluster_gather<1>(cl, sh, v, turn);
+        u64 first = of[0][0];
+        for (int b = 1; b < cl.blocks; ++b) first = first < of[b][0] ? first : of[b][0];
         if (cl.rank == 0 && tid == 0) *out = (int32_t)first;
         return;
     }
-    Weigh<T> weigh{m[0], rs.inv_t, __longlong_as_double((long long)(1023 + shift) << 52), 0.0,
-                   Ranked<Key>{0, 0xffffffffu}, false};
-    if (rs.top_k <= kLgMaxTop) {
-        C rest;
-        bool exact;
-        const int n = wide_top(cl, sh, w, s, mine, rs.top_k, turn, rest, exact, [](C(&)[WideRow<T>::VE], C) {});
-        if (cl.blocks > 1) cl.sync();  // no block leaves while another reads its shared memory
-        if (cl.rank != 0) return;
-        __syncthreads();
-        sort_list(sh, n);
-        list_draw<T>(sh, rs.top_k, weigh, rs, seg, out);
-        return;
-    }
+    Weigh<T> weigh(m, rs.inv_t, shift, &table);
     if (rs.top_k < x.V || rs.top_p < 1.0) {
         const bool by_count = rs.top_k < x.V, by_mass = rs.top_p < 1.0;
         // behind it a weight is below a quarter of the last bit: 0
         const float reach = (float)((double)(shift + 2) * 0.6931471805599453 / rs.inv_t);
-        C low = lg_inf(C());
-        each_class(w, s, [&](int, C v, int) { low = v < low && v != -lg_inf(C()) ? v : low; });
-        C neg[1] = {-low};
-        block_reduce(neg, red_max, OpMax());
-        {
-            const u64* of = cluster_gather(cl, sh, (u64)__double_as_longlong((double)neg[0]), turn);
-            for (int b = 0; b < cl.blocks; ++b) neg[0] = OpMax()(neg[0], (C)__longlong_as_double((long long)of[b]));
-        }
-        const float range = fminf((float)(m[0] + neg[0]), reach);
+        const float range = fminf((float)(m + ends[1]), reach);
         const float per_bin = range > 0.0f && range < lg_inf(0.0f) ? (float)(kBins - 1) / range : 0.0f;
         auto bin_of = [&](C v) {  // larger logits have lower bins
-            const float d = v == m[0] ? 0.0f : (float)(m[0] - v) * per_bin;
+            const float d = v == m ? 0.0f : (float)(m - v) * per_bin;
             return d < (float)(kBins - 1) ? (int)d : kBins - 1;
         };
         for (int i = tid; i < kBins; i += kLgThreads) sh.hist.mass[i] = 0.0f, sh.hist.count[i] = 0u;
@@ -449,37 +494,73 @@ lg_sample_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, SampleArg
         const float c = (float)(rs.inv_t * 1.4426950408889634);
         each_class(w, s, [&](int, C v, int) {
             const int b = bin_of(v);
-            if (by_mass) atomicAdd(&sh.hist.mass[b], v == m[0] ? 1.0f : ex2((float)(v - m[0]) * c));
+            if (by_mass) atomicAdd(&sh.hist.mass[b], v == m ? 1.0f : ex2((float)(v - m) * c));
             if (by_count) atomicAdd(&sh.hist.count[b], 1u);
         });
-        cl.sync();
-        // every thread sums kBins / kLgThreads bins over the blocks, in the blocks' order
-        constexpr int kPer = kBins / kLgThreads;
-        double mass_own = 0.0, mass_bin[kPer];
-        u64 count_own = 0, count_bin[kPer];
-        for (int j = 0; j < kPer; ++j) {
-            float f = 0.0f;
-            u64 n = 0;
-            for (int b = 0; b < cl.blocks; ++b) {
-                const SampleHist* h = cl.of(&sh.hist, b);
-                f += h->mass[tid * kPer + j];
-                n += h->count[tid * kPer + j];
+        __shared__ struct {
+            int bin, count_bin;
+            u64 above, mass;
+        } found;
+        // the first block adds the histograms up and gives the bins to all.  The order in which the f32
+        // masses are added is open: they only say where to look
+        if (cl.blocks > 1) {
+            cl.sync();
+            if (cl.rank != 0) {
+                SampleHist* to = cl.of(&sh.hist, 0);
+                for (int i = tid; i < kBins; i += kLgThreads) {
+                    if (by_mass && sh.hist.mass[i] != 0.0f) atomicAdd(&to->mass[i], sh.hist.mass[i]);
+                    if (by_count && sh.hist.count[i] != 0u) atomicAdd(&to->count[i], sh.hist.count[i]);
+                }
             }
-            mass_bin[j] = (double)f, mass_own += mass_bin[j];
-            count_bin[j] = n, count_own += n;
         }
-        // masses as integers: the scan below serves both (rounded alike in every block)
-        u64 mass_int = (u64)(mass_own * 1048576.0);
-        const u64 mass_upto = block_exscan(mass_int, sh.warp_part), count_upto = block_exscan(count_own, sh.warp_part);
-        cl.sync();  // the histograms are read: the list can take their place
-        __shared__ int s_bin;
-        __shared__ u64 s_above, s_mass;
+        cl.sync();
+        if (cl.rank == 0) {
+            constexpr int kPer = kBins / kLgThreads;
+            float mass_bin[kPer];
+            u64 mass_own = 0, count_own = 0, mass_all, count_all;
+            for (int j = 0; j < kPer; ++j) {
+                mass_bin[j] = sh.hist.mass[tid * kPer + j];
+                mass_own += (u64)((double)mass_bin[j] * 1048576.0);
+                count_own += sh.hist.count[tid * kPer + j];
+            }
+            const u64 mass_upto = block_exscan(mass_own, sh.warp_part[0], mass_all);
+            const u64 count_upto = block_exscan(count_own, sh.warp_part[1], count_all);
+            if (tid == 0) found.bin = 0, found.count_bin = 0, found.above = 0, found.mass = mass_all;
+            __syncthreads();
+            const u64 k = (u64)rs.top_k;
+            if (by_count && count_upto < k && count_upto + count_own >= k) {
+                u64 above = count_upto, mass = mass_upto;
+                int j = 0;
+                for (; above + sh.hist.count[tid * kPer + j] < k; ++j) {
+                    above += sh.hist.count[tid * kPer + j];
+                    mass += (u64)((double)mass_bin[j] * 1048576.0);
+                }
+                found.count_bin = tid * kPer + j, found.above = above;
+                found.mass = mass + (u64)((double)mass_bin[j] * 1048576.0);
+            }
+            __syncthreads();
+            const u64 goal = (u64)(rs.top_p * (double)found.mass);
+            if (by_mass && mass_upto < goal && mass_upto + mass_own >= goal) {
+                u64 upto = mass_upto;
+                int j = 0;
+                for (; j + 1 < kPer; ++j) {
+                    upto += (u64)((double)mass_bin[j] * 1048576.0);
+                    if (upto >= goal) break;
+                }
+                found.bin = tid * kPer + j;
+            }
+            if (tid == 0) sh.count = 0;
+            __syncthreads();
+            if (tid > 0 && tid < cl.blocks) *cl.of(&found, tid) = found;
+        }
+        cl.sync();  // the bins are known, and the list can take the histogram's place
         auto push = [&](int i, C v) {
             TopShared<Key>* first = cl.of(&sh, 0);
             const int p = atomicAdd(&first->count, 1);
             if (p < kTopCap) first->key[p] = key_of(v), first->idx[p] = (uint32_t)i;
         };
         auto restart = [&] {  // an empty list; also ends what read the last one
+            cl.sync();
             if (cl.rank == 0 && tid == 0) sh.count = 0;
             cl.sync();
         };
@@ -488,19 +569,9 @@ lg_sample_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, SampleArg
         };
         if (by_count) {
             const u64 k = (u64)rs.top_k;
-            if (count_upto < k && count_upto + count_own >= k) {
-                u64 above = count_upto;
-                int j = 0;
-                while (above + count_bin[j] < k) above += count_bin[j++];
-                double upto = (double)mass_upto;
-                for (int i = 0; i <= j; ++i) upto += mass_bin[i] * 1048576.0;
-                s_bin = tid * kPer + j, s_above = above, s_mass = (u64)upto;
-            }
-            __syncthreads();
-            const int bin = s_bin;
-            const u64 above = s_above;
+            const int bin = found.count_bin;
+            const u64 above = found.above;
             weigh.cut = bin < kBins - 1 || range < reach;  // else what is cut weighs nothing
-            restart();
             if (weigh.cut)
                 each_class(w, s, [&](int i, C v, int) {
                     if (bin_of(v) == bin) push(i, v);
@@ -521,39 +592,23 @@ lg_sample_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, SampleArg
             }
         }
         if (by_mass) {
-            __syncthreads();
-            if (!by_count && tid == kLgThreads - 1) s_mass = mass_upto + mass_int;
-            if (tid == 0) s_bin = 0;
-            __syncthreads();
-            {
-                const u64 goal = (u64)(rs.top_p * (double)s_mass);
-                if (mass_upto < goal && mass_upto + mass_int >= goal) {
-                    double upto = (double)mass_upto;
-                    int j = 0;
-                    while (j + 1 < kPer && upto + mass_bin[j] * 1048576.0 < (double)goal) upto += mass_bin[j++] * 1048576.0;
-                    s_bin = tid * kPer + j;
-                }
-            }
-            __syncthreads();
-            int bin = s_bin, lo = -1, hi = kBins, step = 1;  // the cut's bin is in (lo, hi)
-            for (;;) {
-                restart();
-                u64 above = 0, within = 0, total = 0;
-                each_class(w, s, [&](int i, C v, int) {
+            int bin = found.bin, lo = -1, hi = kBins, step = 1;  // the cut's bin is in (lo, hi)
+            for (bool first = !by_count;; first = false) {
+                if (!first) restart();
+                u64 sums[3] = {0, 0, 0};  // of all that stays; above the bin; in it
+                each_place(w, s, [&](int i, C v, int) {
                     if (!weigh.stays(i, v)) return;
                     const u64 f = weigh.mass(v);
                     const int b = bin_of(v);
-                    total += f;
-                    above += b < bin ? f : 0;
-                    if (b == bin) {
-                        within += f;
+                    sums[0] += f;
+                    sums[1] += b < bin ? f : 0;
+                    if (b == bin && w.valid(i)) {
+                        sums[2] += f;
                         push(i, v);
                     }
                 });
-                total = cluster_total(cl, sh, total, turn);
-                above = cluster_total(cl, sh, above, turn);
-                within = cluster_total(cl, sh, within, turn);
-                const u64 goal = mass_part(rs.top_p, total);
+                cluster_total<3>(cl, sh, sums, turn);
+                const u64 above = sums[1], within = sums[2], goal = mass_part(rs.top_p, sums[0]);
                 if (above >= goal || above + within < goal) {  // the f32 masses were a little off: a bin near
                     if (above >= goal) hi = bin, bin = bin - step > lo ? bin - step : lo + 1;
                     else lo = bin, bin = bin + step < hi ? bin + step : hi - 1;
@@ -569,7 +624,8 @@ lg_sample_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, SampleArg
                         const int run = (n + kLgThreads - 1) / kLgThreads, j0 = tid * run;
                         u64 own = 0;
                         for (int j = j0; j < j0 + run && j < n; ++j) own += weigh.mass((C)of_key(sh.key[j]));
-                        u64 upto = above + block_exscan(own, sh.warp_part);
+                        u64 all;
+                        u64 upto = above + block_exscan(own, sh.warp_part[0], all);
                         if (upto < goal && upto + own >= goal)
                             for (int j = j0;; ++j) {
                                 upto += weigh.mass((C)of_key(sh.key[j]));
@@ -593,7 +649,8 @@ lg_sample_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, SampleArg
         }
     }
     weigh.min_p = rs.min_p;
-    wide_draw(cl, sh, seg, w, s, weigh, rs.u, turn, out);
+    __syncthreads();
+    wide_draw(cl, sh, w, s, weigh, rs.u, turn, out);
 }
 
 template <typename T>

@@ -173,10 +173,10 @@ lg_top_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, int k, Scale
     if (cl.blocks > 1) cluster_wait();  // every block runs
     int turn = 0;
     C rest, ref = C(0);
-    bool exact;
+    bool exact, flag = false;
     double sum = 0.0;
     // the tail's sum is taken on the way, relative to the least class that is collected
-    const int n = wide_top(cl, sh, w, s, most.get(), k, turn, rest, exact, [&](C(&a)[VE], C least) {
+    const int n = wide_top(cl, sh, w, s, most.get(), k, turn, rest, exact, flag, [&](C(&a)[VE], C least) {
         if (!tail) return;
         ref = floor_max(least);
         const Base<C> at(ref, sc);
