@@ -89,7 +89,7 @@ def _logits(who, x):
 
 def _side(who, name, v, x, shape, dtypes):
     """A contiguous operand beside the logits, of one of `dtypes`."""
-    if not isinstance(v, _torch.Tensor) or v.device != x.device:
+    if not isinstance(v, _torch.Tensor) or v.get_device() != x.get_device():
         raise _bad(f"{who}: {name} must be a tensor on the logits' device")
     if v.dtype not in dtypes:
         raise _bad(f"{who}: {name} has dtype {v.dtype}, expected {' or '.join(str(d) for d in dtypes)}")
@@ -133,16 +133,19 @@ def top_logits(logits, k: int, *, temperature: float = 1.0, tail: bool = True) -
         raise _bad(f"{who}: k = {k} is outside 1..min({MAX_TOP}, {d.n_classes} classes)")
     temperature = _temperature(who, temperature)
     n = d.n
-    value = logits.new_empty((n, k))
-    index = logits.new_empty((n, k), dtype=_torch.int32)
-    rest = logits.new_empty((n,), dtype=_wide(logits)) if tail else None
+    value = logits.new_empty(n, k)
+    index = logits.new_empty(n, k, dtype=_torch.int32)
+    rest = logits.new_empty(n, dtype=_wide(logits)) if tail else None
     _run(logits, _L.cbgpu_top_logits, C.byref(d), k, temperature, value.data_ptr(), index.data_ptr(),
          rest.data_ptr() if tail else None)
     return TopLogits(index, value, rest)
 
 
-def _distill(who, logits, teacher, weight, temperature, der1):
-    d = _logits(who, logits)
+def _distill(who, logits, teacher, weight, temperature, der1, d=None):
+    """The loss; der1, when not None, is checked unless `d`, the logits' description, comes with it."""
+    own = d is not None
+    if not own:
+        d = _logits(who, logits)
     n = d.n
     wide = _wide(logits)
     if not isinstance(teacher, TopLogits):
@@ -155,12 +158,12 @@ def _distill(who, logits, teacher, weight, temperature, der1):
     rest = None if teacher.tail is None else _side(who, "the teacher's tail", teacher.tail, logits, (n,), (wide,))
     weight = None if weight is None else _side(who, "weight", weight, logits, (n,), (wide,))
     temperature = _temperature(who, temperature)
-    if der1 is not None:
-        if not isinstance(der1, _torch.Tensor) or der1.device != logits.device or der1.dtype != logits.dtype:
+    if der1 is not None and not own:
+        if not isinstance(der1, _torch.Tensor) or der1.get_device() != logits.get_device() or der1.dtype != logits.dtype:
             raise _bad(f"{who}: out must be a {logits.dtype} tensor on the logits' device")
         if der1.shape != logits.shape:
             raise _bad(f"{who}: LengthMismatch: out is {tuple(der1.shape)}, expected {tuple(logits.shape)}")
-    loss = logits.new_empty((n,), dtype=wide)
+    loss = logits.new_empty(n, dtype=wide)
     t = _lib.Teacher(index.data_ptr(), value.data_ptr(), None if rest is None else rest.data_ptr(),
                      index.element_size(), _dtypes[value.dtype], shape[1])
     rs, cs = der1.stride() if der1 is not None else (0, 0)
@@ -183,9 +186,10 @@ def distill_derivatives(logits, teacher: TopLogits, *, weight=None, temperature:
     own loss puts on each row.  `out` takes der1; it may be the logits."""
     who = "distill_derivatives"
     if out is None:
-        _logits(who, logits)
-        dense = logits.is_contiguous() or logits.t().is_contiguous()
+        d = _logits(who, logits)
+        dense = logits.is_contiguous() or (d.row_stride == 1 and d.class_stride == d.n)
         out = _torch.empty_like(logits) if dense else logits.new_empty(logits.shape)
+        return Distilled(_distill(who, logits, teacher, weight, temperature, out, d), out)
     return Distilled(_distill(who, logits, teacher, weight, temperature, out), out)
 
 
@@ -230,6 +234,6 @@ def sample_classes(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_
         if int(top_k) < 0:
             raise _bad(f"{who}: top_k {top_k} < 0")
         s.top_k = min(int(top_k), MAX_CLASSES)
-    index = logits.new_empty((n,), dtype=_torch.int32)
+    index = logits.new_empty(n, dtype=_torch.int32)
     _run(logits, _L.cbgpu_sample_classes, C.byref(d), C.byref(s), index.data_ptr())
     return index

@@ -722,7 +722,7 @@ struct SampleHist {
 
 template <typename Key>
 struct TopShared {
-    union {
+    union __align__(16) {
         struct {
             Key key[kTopCap];
             uint32_t idx[kTopCap];
@@ -874,25 +874,27 @@ __device__ void sort_list(TopShared<Key>& sh, int n) {
     const int tid = threadIdx.x;
     if (n <= kLgThreads) {  // every entry counts those before it, some threads an entry
         int per = 1;
-        while (n * per * 2 <= kLgThreads) per *= 2;
-        const int c = tid / per;
+        while (n * per * 2 <= kLgThreads && per < 32) per *= 2;
+        const int c = tid / per, part = tid & (per - 1);
         const Ranked<Key> own{sh.key[c < n ? c : 0], sh.idx[c < n ? c : 0]};
         int rank = 0;
-#pragma unroll 8
-        for (int i = tid & (per - 1); i < n; i += per) rank += Ranked<Key>{sh.key[i], sh.idx[i]}.before(own) ? 1 : 0;
-        for (int o = 1; o < per; o <<= 1) {
-            const int t = __shfl_xor_sync(0xffffffffu, rank, o & 31);
-            rank += o < 32 ? t : 0;
-        }
-        if (per > 32) {  // an entry's threads are whole warps
-            if (tid < n) sh.idx[kLgThreads + tid] = 0u;
+        if (sizeof(Key) == 4) {  // key and index as one number, read by pairs
+            u64* both = reinterpret_cast<u64*>(&sh.idx[kTopCap - 2 * kLgThreads]);
+            if (tid < kLgThreads) both[tid] = tid < n ? (u64)sh.key[tid] << 32 | (uint32_t)~sh.idx[tid] : 0ull;
             __syncthreads();
-            if ((tid & 31) == 0 && c < n) atomicAdd(&sh.idx[kLgThreads + c], (uint32_t)rank);
-            __syncthreads();
-            rank = c < n ? (int)sh.idx[kLgThreads + c] : 0;
+            const u64 mine = (u64)own.key << 32 | (uint32_t)~own.idx;
+#pragma unroll 4
+            for (int i = 2 * part; i < n; i += 2 * per) {
+                const ulonglong2 t = *reinterpret_cast<const ulonglong2*>(both + i);
+                rank += (t.x > mine ? 1 : 0) + (t.y > mine ? 1 : 0);
+            }
+        } else {
+#pragma unroll 4
+            for (int i = part; i < n; i += per) rank += Ranked<Key>{sh.key[i], sh.idx[i]}.before(own) ? 1 : 0;
         }
+        for (int o = 1; o < per; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
         __syncthreads();
-        if (c < n && (tid & (per - 1)) == 0) sh.key[rank] = own.key, sh.idx[rank] = own.idx;
+        if (c < n && part == 0) sh.key[rank] = own.key, sh.idx[rank] = own.idx;
         __syncthreads();
         return;
     }
@@ -1090,10 +1092,14 @@ Tile narrow_tile(int V, size_t bytes_a_class, int teams) {
     return Tile{(int)rows, rows * row + 32};
 }
 
+// What a kernel that needs asking is allowed: always the same, so that calls on several threads do not take
+// it from each other.  The static arrays (up to 25 KB) fit beside it.
+constexpr int kLgSmemMost = 200 * 1024;
+
 template <typename K, typename... A>
 int lg_launch(const char* who, K kernel, unsigned grid, size_t smem, cudaStream_t st, A... args) {
     if (smem > 20 * 1024) {  // with the kernels' static arrays (up to 25 KB) above the 48 KB that need no asking
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kLgSmemMost);
         if (e != cudaSuccess) return lfail(CBGPU_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
     }
     kernel<<<grid, kLgThreads, smem, st>>>(args...);
@@ -1102,10 +1108,12 @@ int lg_launch(const char* who, K kernel, unsigned grid, size_t smem, cudaStream_
     return CBGPU_OK;
 }
 
-// Blocks of a wide row's cluster, vectors a block, shared memory.  About 64 KB a block (at 3
-// 7 blocks an SM one block's copies run under another's arithmetic); when
-// there are few rows, more blocks, down to 2 KB each, so that a row's bytes come through
-// more SMs.
+// Blocks of a wide row's cluster, vectors a block, shared memory.  About 64 KB a block (3 blocks an SM,
+// so that one's copies run under another's arithmetic; 16 to 48 KB a block were slower, since each
+// block pays for its barriers and sums: derivatives of 4096 x 64000 bf16 270 us at 64 KB, 320 at
+// 43 KB); when there are few rows, up to 8 blocks of 6 KB or more, so that a row's bytes come
+// through more SMs.  Clusters of 16 are for rows above 512 KB only: one of them is 10 us slower to
+// start and to meet than one of 8.
 struct Wide {
     int blocks, per;
     size_t smem;
@@ -1116,7 +1124,7 @@ Wide wide_shape(int64_t n, int V) {
     const int ve = 16 / (int)sizeof(T), vectors = (V + 2 * (ve - 1)) / ve;
     Wide w{1, 0, 0, 0};
     while (w.blocks < 16 && (size_t)V * sizeof(T) > (size_t)65536 * w.blocks) w.blocks *= 2;
-    while (w.blocks < 16 && n * w.blocks * 2 <= 148 * 2 && (size_t)vectors * 16 >= (size_t)4096 * w.blocks)
+    while (w.blocks < 8 && n * w.blocks <= 148 && (size_t)vectors * 16 >= (size_t)12288 * w.blocks)
         w.blocks *= 2;
     w.per = (vectors + w.blocks - 1) / w.blocks;
     w.smem = (size_t)w.per * 16;
@@ -1131,7 +1139,7 @@ template <typename K, typename... A>
 int lg_launch_wide(const char* who, K kernel, int64_t n, const Wide& w, size_t smem, cudaStream_t st, A... args) {
     cudaError_t e = cudaSuccess;
     if (smem > 32 * 1024)  // with the kernels' static arrays (less than 16 KB) above the 48 KB that need no asking
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kLgSmemMost);
     if (e == cudaSuccess && w.blocks > 8)
         e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     cudaLaunchConfig_t cfg = {};

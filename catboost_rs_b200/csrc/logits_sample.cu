@@ -226,23 +226,25 @@ lg_sample_narrow_kernel(Rows<T> x, SampleArgs a, int shift, int tile, int direct
 // exact masses, which also show whether the bin was the right one.
 
 // exp of a non-positive number by the table-driven method of P. T. P. Tang (ACM TOMS 15, 1989): with
-// x log2(e) = n / 64 + r / 64, |r| <= 1/2, it is 2^(n / 64), from a table of 64 and an exponent, times a polynomial
-// in r ln2 / 64 (below 0.0055: degree 5 leaves 4e-17).  12 operations in 64 bits with what Weigh adds; exp()
-// takes two to three times as many, and the draw from whole rows is bound by them.
+// x log2(e) = (n + r) / 64, |r| <= 1/2, it is 2^(n / 64), from a table of 64 and an exponent, times a polynomial
+// in r ln2 / 64 (below 0.0055: degree 4 leaves 4e-14, as much as a mass is rounded by).  The draw from whole
+// rows is bound by these operations: 12 in 64 bits a class, where exp() and its range checks take
+// some 30 (64 x 131071 f32: 55 us with 15 and the checks class by class).
 constexpr int kExpTable = 64;
 struct ExpTable {
     double of[kExpTable];
     __device__ void fill() {  // by the block; a barrier follows
         if (threadIdx.x < kExpTable) of[threadIdx.x] = exp2((double)threadIdx.x / kExpTable);
     }
-    // 2^(y / 64), y in (-64 * 1000, 0]
+    // 2^(y / 64) for y <= 0; y below -64000 counts as that
     __device__ double operator()(double y) const {
+        const uint32_t hi = (uint32_t)__double2hiint(y);  // of negative numbers the larger is further down
+        y = __hiloint2double((int)(hi < 0xc0ef4000u ? hi : 0xc0ef4000u), __double2loint(y));
         const double t = y + 6755399441055744.0;  // 1.5 2^52: the low word of t is n
         const int n = __double2loint(t);
         const double r = y - (t - 6755399441055744.0);
         constexpr double c = 0.6931471805599453 / kExpTable;
-        double p = fma(r, c * c * c * c * c / 120.0, c * c * c * c / 24.0);
-        p = fma(r, p, c * c * c / 6.0);
+        double p = fma(r, c * c * c * c / 24.0, c * c * c / 6.0);
         p = fma(r, p, c * c / 2.0);
         p = fma(r, p, c);
         const double b = of[n & (kExpTable - 1)];
@@ -258,17 +260,15 @@ struct Weigh {
     C m;
     double inv_t, scale, min_p;
     Ranked<Key> last;  // the last class that stays
-    bool cut;
+    bool cut, infinite;
     const ExpTable* table;
     double per64;  // 64 log2(e) / T
     __device__ Weigh(C m_, double inv_t_, int shift, const ExpTable* t)
-        : m(m_), inv_t(inv_t_), scale(power_of_2(shift)), min_p(0.0),
-          last{0, 0xffffffffu}, cut(false), table(t), per64(inv_t_ * (kExpTable * 1.4426950408889634)) {}
-    __device__ double share(C a) const {
-        const double y = ((double)a - (double)m) * per64;
-        const double e = (*table)(fmax(y, -64.0 * 1000.0));
-        return a == m ? 1.0 : (y > -64.0 * 60.0 ? e : 0.0);  // 2^-60: less than half of any last bit
-    }
+        : m(m_), inv_t(inv_t_), scale(power_of_2(shift)), min_p(0.0), last{0, 0xffffffffu}, cut(false),
+          infinite(m_ == lg_inf(C())), table(t), per64(inv_t_ * (kExpTable * 1.4426950408889634)) {}
+    __device__ double finite_share(C a) const { return (*table)(((double)a - (double)m) * per64); }
+    // infinite logits share the mass among themselves
+    __device__ double share(C a) const { return infinite ? (a == m ? 1.0 : 0.0) : finite_share(a); }
     __device__ u64 whole(double e) const { return whole_mass(e, scale); }
     __device__ u64 mass(C a) const { return whole(share(a)); }
     __device__ bool stays(int i, C a) const {
@@ -279,6 +279,19 @@ struct Weigh {
         if (!stays(i, a)) return 0;
         const double e = share(a);
         return e < min_p ? 0 : whole(e);
+    }
+    // the mass of a vector whose first class is i
+    template <int N>
+    __device__ u64 vector(int i, const C (&a)[N]) const {
+        u64 sum = 0;
+        if (cut || infinite || min_p > 0.0) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) sum += (*this)(i + j, a[j]);
+            return sum;
+        }
+#pragma unroll
+        for (int j = 0; j < N; ++j) sum += whole(finite_share(a[j]));
+        return sum;
     }
 };
 
@@ -324,8 +337,7 @@ __device__ void wide_draw(const ClusterInfo& cl, Sh& sh, const WideRow<T>& w, co
         if (v < w.nv) {
             typename Num<T>::C a[VE];
             unpack(s[v], a, T());
-#pragma unroll
-            for (int j = 0; j < VE; ++j) own += weigh(w.first(v) + j, a[j]);
+            own = weigh.vector(w.first(v), a);
         }
         return own;
     };
