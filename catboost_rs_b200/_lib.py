@@ -71,7 +71,7 @@ EXPORTS = [
     "cbgpu_select_borders", "cbgpu_apply_oblivious",
     "cbgpu_multi_begin_raw", "cbgpu_multi_begin_cat_raw", "cbgpu_multi_grow_tree", "cbgpu_multi_approx", "cbgpu_multi_end",
     "cbgpu_rank_begin_raw",
-    "cbgpu_top_logits", "cbgpu_distill", "cbgpu_sample_classes",
+    "cbgpu_multi_set_teacher", "cbgpu_top_logits", "cbgpu_distill", "cbgpu_sample_classes",
 ]
 
 _lib = None
@@ -147,6 +147,7 @@ def load(path: str = LIB_PATH):
         "cbgpu_rank_begin_raw": ([C.POINTER(BeginArgs), vp, i32, vp, vp, i64, C.POINTER(RankParams), vp, vp, vp,
                                   C.POINTER(vp)], C.c_int),
         "cbgpu_multi_end": ([vp], C.c_int),
+        "cbgpu_multi_set_teacher": ([vp, vp, vp, vp, i32, f64], C.c_int),
         "cbgpu_top_logits": ([C.POINTER(Logits), i32, f64, vp, vp, vp, vp], C.c_int),
         "cbgpu_distill": ([C.POINTER(Logits), C.POINTER(Teacher), vp, f64, vp, vp, i64, i64, vp], C.c_int),
         "cbgpu_sample_classes": ([C.POINTER(Logits), C.POINTER(Sampling), vp, vp], C.c_int),

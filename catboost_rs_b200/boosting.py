@@ -190,7 +190,8 @@ def perfect_hash_bins(column):
 
 def fit_multiclass(float_columns: Sequence[np.ndarray], borders: Sequence[Sequence[float]], target_class,
                    n_classes: int, params: FitParams, weights=None, *, staged: bool = False,
-                   device: int = 0, cat_columns=None, loss: str = "MultiClass") -> MultiClassModel:
+                   device: int = 0, cat_columns=None, loss: str = "MultiClass", teacher=None,
+                   temperature: float = 1.0) -> MultiClassModel:
     """Multi-output fit (Newton leaves) on raw f32 columns with fixed borders:
     cb-train's multi-output loop (boosting.rs:7400-8930 at approx_dimension K)
     over the device's multi-output arm.
@@ -202,12 +203,18 @@ def fit_multiclass(float_columns: Sequence[np.ndarray], borders: Sequence[Sequen
     The three diagonal losses solve each dimension's leaf on its own
     (boosting.rs:8323-8420).  cat_columns are one-hot categorical features
     (any hashable values; bins in first-seen order); they need bootstrap No,
-    as upstream."""
+    as upstream.
+
+    `teacher`, with target_class None, trains MultiClass on another model's
+    class logits instead of labels: a class_logits.TopLogits (arrays or
+    tensors) of every row's top logits, with the tail at `temperature`."""
     p = params
+    if (teacher is None) == (target_class is None):
+        raise ValueError("fit_multiclass takes either target_class or a teacher")
     cols = [np.ascontiguousarray(c, dtype=np.float32) for c in float_columns]
     F = len(cols)
     n = cols[0].size if F else (len(cat_columns[0]) if cat_columns else 0)
-    y = np.ascontiguousarray(target_class, dtype=np.float64)
+    y = None if target_class is None else np.ascontiguousarray(target_class, dtype=np.float64)
     w = None if weights is None else np.ascontiguousarray(weights, dtype=np.float64)
     sw = seq_sum(w) if w is not None else float(n)
     scaled_l2 = p.l2_leaf_reg * (sw / n) if n else p.l2_leaf_reg
@@ -227,6 +234,12 @@ def fit_multiclass(float_columns: Sequence[np.ndarray], borders: Sequence[Sequen
                                       n_bins, lr, scaled_l2, cfg, approx_dim=K, cat_columns=cat_bins)
     if not ok:
         raise RuntimeError(f"device declined: {rt.decline_reason}")
+    if teacher is not None:
+        host = [None if v is None else np.asarray(v.detach().cpu().double() if hasattr(v, "detach") else v)
+                for v in (teacher.index, teacher.value, teacher.tail)]
+        if not rt.set_teacher(*host, temperature):
+            rt.end_device_training()
+            raise RuntimeError(f"device declined: {rt.decline_reason}")
     T, D = p.iterations, p.depth
     sf = np.zeros((T, D), dtype=np.int32)
     sb = np.zeros((T, D), dtype=np.int32)

@@ -8,7 +8,8 @@
 // (crates/cb-train/src/boosting.rs:7400-8930 at approx_dimension K) is what
 // this arm reproduces, one CUDA stream per session:
 //
-//   per tree   mc_der_kernel       pending leaf update, softmax, weighted der1
+//   per tree   mc_der_kernel       pending leaf update, softmax, weighted der1 (on a teacher's top
+//                                  logits: cbgpu_distill's derivative)
 //              bootstrap           (the scalar path's kernels)
 //              mc_max / mc_pack    K + 1 score channels as int64 fixed point
 //   per level  mc_hist_kernel      (feature, channel, row chunk) blocks, the
@@ -143,11 +144,12 @@ __device__ __forceinline__ uint32_t block_excl_scan_u32(uint32_t v, uint32_t* sm
 
 // Softmax probabilities of one object (loss.rs:424-455): max-subtracted exp,
 // sequential sum, division.
+// inv_t: 1 / temperature of a fit on a teacher, else 1.
 __device__ __forceinline__ void mc_softmax(const double* __restrict__ approx, int64_t n, int64_t i, int K,
-                                           double* p) {
+                                           double* p, double inv_t = 1.0) {
     double mx = -INFINITY;
     for (int d = 0; d < K; ++d) {
-        const double a = approx[(size_t)d * n + i];
+        const double a = __dmul_rn(approx[(size_t)d * n + i], inv_t);
         p[d] = a;
         if (a > mx) mx = a;
     }
@@ -548,7 +550,7 @@ __global__ void mc_route_kernel(int64_t n, int level, const uint8_t* __restrict_
 __global__ void __launch_bounds__(kMcThreads)
 mc_leafsum_kernel(int64_t n, int K, int L, const double* __restrict__ approx, const double* __restrict__ wd1,
                   const double* __restrict__ weight, const uint16_t* __restrict__ leaf, int leaf_shift_in, int diag,
-                  const double* __restrict__ tmat, unsigned long long* __restrict__ sums, int use_smem,
+                  const double* __restrict__ tmat, unsigned long long* __restrict__ sums, int use_smem, double inv_t,
                   McState* __restrict__ ms) {
     // RMSEWithUncertainty's ders are unbounded: its sums take the tree's score
     // shift less 2 (|w der2| <= 2 |w der1_1| + 2 w <= 4 max channel)
@@ -593,7 +595,7 @@ mc_leafsum_kernel(int64_t n, int K, int L, const double* __restrict__ approx, co
             }
             continue;
         }
-        mc_softmax(approx, n, i, K, p);
+        mc_softmax(approx, n, i, K, p, inv_t);
         int j = 0;
         for (int dy = 0; dy < K; ++dy) {
             add(cell + K + j++, __dmul_rn(__dmul_rn(p[dy], __dsub_rn(p[dy], 1.0)), w));
@@ -687,6 +689,14 @@ __global__ void mc_newton_kernel(int K, int L, const unsigned long long* __restr
         leaf_raw[(size_t)q * K + d] = delta;                 // leaf-major, raw (the seam's layout)
         leaf_lrv[(size_t)d * L + q] = __dmul_rn(delta, lr);  // dim-major, x lr (normalize_leaf_values)
     }
+}
+
+// A fit on a teacher: the derivatives come from cbgpu_distill.
+__global__ void mc_finite_kernel(int64_t count, const double* __restrict__ v, McState* __restrict__ ms) {
+    bool bad = false;
+    for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < count; i += (int64_t)gridDim.x * blockDim.x)
+        bad |= !isfinite(v[i]);
+    if (__any_sync(0xffffffffu, bad) && (threadIdx.x & 31) == 0) atomicOr(&ms->err, kMcErrNonFinite);
 }
 
 __global__ void mc_fill2_kernel(int64_t n, double* __restrict__ approx, double b0, double b1) {
@@ -2118,6 +2128,11 @@ struct cbgpu_multi_session {
     int F0 = 0;                    // float features; F0..F-1 are one-hot categorical
     int loss = 0;                  // cbgpu_loss of a multi-output session
     int diag = 0;                  // 1: the diagonal losses (OneVsAll, MultiLogloss, MultiCrossEntropy)
+    // a teacher's top logits (cbgpu_multi_set_teacher): [n][t_k] classes and logits, [n] tails, and the loss
+    int t_k = 0, t_shift = 0;  // t_shift: what the leaf sums' shift has given way
+    double t_temp = 1.0;
+    int32_t* d_tindex = nullptr;
+    double *d_tvalue = nullptr, *d_ttail = nullptr, *d_tloss = nullptr;
     double* d_tmat = nullptr;      // [K][n] label matrix of MultiLogloss / MultiCrossEntropy
     uint8_t* d_present = nullptr;  // [F - F0][NB] learn-set bins of each categorical feature
     float sample_rate = 1.0f, temp = 1.0f;
@@ -2223,6 +2238,10 @@ struct cbgpu_multi_session {
         if (st) cudaStreamSynchronize(st);
         cudaFree(d_srank_ws);
         cudaFree(d_tmat);
+        cudaFree(d_tindex);
+        cudaFree(d_tvalue);
+        cudaFree(d_ttail);
+        cudaFree(d_tloss);
         cudaFree(d_present);
         cudaFree(d_gw);
         cudaFree(d_yseeds);
@@ -3027,6 +3046,10 @@ int cbgpu_multi_grow_tree(cbgpu_multi_session* s, const double* approx_k, const 
         MCU(cudaStreamSynchronize(st));
         s->target_ready = true;
     }
+    if (!s->target_ready && s->t_k > 0) {
+        if (target) return mfail(CBGPU_ERR_INVALID, "multi_grow: a session with a teacher takes no target");
+        s->target_ready = true;
+    }
     if (!s->target_ready) {
         if (!target) return mfail(CBGPU_ERR_INVALID, "multi_grow: the first call needs the target");
         std::vector<int32_t> cls((size_t)n);
@@ -3135,6 +3158,14 @@ int cbgpu_multi_grow_tree(cbgpu_multi_session* s, const double* approx_k, const 
             RkLossParams{s->sm_lambda, s->sm_beta, s->lm_sigma, s->lm_top, s->lm_norm, s->d_lmden, s->d_lmideal,
                          s->d_lmorder, s->lm_no_op},
             s->wd1, s->d_der2, s->d_ms);
+    } else if (s->t_k > 0) {
+        if (s->pending)
+            mc_apply_pending_kernel<<<g, kMcThreads, 0, st>>>(n, K, L, s->approx, s->leaf, s->leaf_lrv);
+        const cbgpu_logits rows = {s->approx, CBGPU_F64, K, n, 1, n};
+        const cbgpu_teacher teacher = {s->d_tindex, s->d_tvalue, s->d_ttail, 4, CBGPU_F64, s->t_k};
+        const int rc = cbgpu_distill(&rows, &teacher, s->weight, s->t_temp, s->d_tloss, s->wd1, 1, n, st);
+        if (rc) return rc;
+        mc_finite_kernel<<<grid_for((int64_t)K * n), kMcThreads, 0, st>>>((int64_t)K * n, s->wd1, s->d_ms);
     } else {
         mc_der_kernel<<<g, kMcThreads, 0, st>>>(n, K, s->approx, s->target, s->weight, s->leaf, s->leaf_lrv, L,
                                                 s->pending ? 1 : 0, s->diag, s->d_tmat, s->wd1, s->d_ms);
@@ -3333,7 +3364,7 @@ int cbgpu_multi_grow_tree(cbgpu_multi_session* s, const double* approx_k, const 
             MCU(cudaFuncSetAttribute(mc_leafsum_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ltab));
         mc_leafsum_kernel<<<g, kMcThreads, luse ? ltab : 0, st>>>(n, K, L, s->approx, s->wd1, s->weight, s->leaf,
                                                                  s->leaf_shift, s->diag, s->d_tmat, s->sums, luse,
-                                                                 s->d_ms);
+                                                                 1.0 / s->t_temp, s->d_ms);
         mc_newton_kernel<<<(L + 63) / 64, 64, 0, st>>>(K, L, s->sums, s->leaf_shift, s->l2, s->lr, s->diag, s->d_ms,
                                                        s->leaf_raw, s->leaf_lrv);
         MCU(cudaGetLastError());
@@ -3366,6 +3397,57 @@ int cbgpu_multi_grow_tree(cbgpu_multi_session* s, const double* approx_k, const 
     if (n_splits) *n_splits = D;
     if (leaf_values) memcpy(leaf_values, s->h_raw, sizeof(double) * (size_t)L * K);
     s->pending = true;
+    return CBGPU_OK;
+}
+
+int cbgpu_multi_set_teacher(cbgpu_multi_session* s, const int32_t* index, const double* value, const double* tail,
+                            int32_t k, double temperature) {
+    if (!s) return mfail(CBGPU_ERR_INVALID, "multi_set_teacher: no session");
+    if (s->rank_mode >= 0 || s->loss != CBGPU_LOSS_MULTICLASS)
+        return mfail(CBGPU_DECLINED, "multi_set_teacher: only MultiClass sessions take a teacher");
+    if (s->target_ready) return mfail(CBGPU_ERR_INVALID, "multi_set_teacher: the session has its target already");
+    if (!index || !value) return mfail(CBGPU_ERR_INVALID, "multi_set_teacher: index or value is NULL");
+    if (k < 1 || k > 256) return mfail(CBGPU_ERR_INVALID, "multi_set_teacher: k = %d is outside 1..256", k);
+    if (!(temperature >= 1e-3 && temperature <= 1e3))
+        return mfail(CBGPU_ERR_INVALID, "multi_set_teacher: temperature %g is outside 1e-3..1e3", temperature);
+    const int64_t n = s->n;
+    for (int64_t i = 0; i < n; ++i) {
+        for (int32_t j = 0; j < k; ++j) {
+            const int32_t c = index[i * k + j];
+            const double z = value[i * k + j];
+            if (c < -1 || c >= s->K)
+                return mfail(CBGPU_ERR_INVALID, "multi_set_teacher: class %d at row %lld is outside -1..%d", c,
+                             (long long)i, s->K - 1);
+            if (c >= 0 && !(z < INFINITY))  // -inf is a class the teacher rules out
+                return mfail(CBGPU_ERR_INVALID, "multi_set_teacher: logit %g at row %lld", z, (long long)i);
+        }
+        if (tail && !(tail[i] < INFINITY))
+            return mfail(CBGPU_ERR_INVALID, "multi_set_teacher: tail %g at row %lld", tail[i], (long long)i);
+    }
+    MCU(cudaSetDevice(s->device));
+    // (an earlier teacher, or one that found no memory, gives way)
+    cudaFree(s->d_tindex);
+    cudaFree(s->d_tvalue);
+    cudaFree(s->d_ttail);
+    cudaFree(s->d_tloss);
+    s->d_tindex = nullptr;
+    s->d_tvalue = s->d_ttail = s->d_tloss = nullptr;
+    s->t_k = 0;
+    MDA(s->d_tindex, (size_t)n * k);
+    MDA(s->d_tvalue, (size_t)n * k);
+    MDA(s->d_tloss, n);
+    if (tail) MDA(s->d_ttail, n);
+    MCU(cudaMemcpyAsync(s->d_tindex, index, sizeof(int32_t) * (size_t)n * k, cudaMemcpyHostToDevice, s->st));
+    MCU(cudaMemcpyAsync(s->d_tvalue, value, sizeof(double) * (size_t)n * k, cudaMemcpyHostToDevice, s->st));
+    if (tail) MCU(cudaMemcpyAsync(s->d_ttail, tail, sizeof(double) * (size_t)n, cudaMemcpyHostToDevice, s->st));
+    MCU(cudaStreamSynchronize(s->st));
+    // |w der1| <= max|w| T: the leaf sums' fixed point gives way by T's exponent
+    int e = 0;
+    std::frexp(std::max(temperature, 1.0), &e);
+    s->leaf_shift += s->t_shift - e;
+    s->t_shift = e;
+    s->t_k = k;
+    s->t_temp = temperature;
     return CBGPU_OK;
 }
 

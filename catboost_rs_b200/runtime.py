@@ -444,6 +444,26 @@ class B200MultiRuntime(B200Runtime):
         return DeviceGrownTree(splits=[(int(sf[i]), int(sb[i]), False) for i in range(k)], leaf_values=lv,
                                approx_dim=K, leaf_of=lo if lo is not None else np.zeros(0, dtype=np.uint32))
 
+    def set_teacher(self, index, value, tail=None, temperature: float = 1.0) -> bool:
+        """Train this MultiClass session on a teacher's top logits
+        (cbgpu_multi_set_teacher) instead of class indices: index [n, k]
+        classes (-1: no entry), value [n, k] logits, tail [n] the log-sum-exp
+        of its other classes at the temperature.  Before the first tree; the
+        grow calls then take no target.  False when the session declines."""
+        if not self._s:
+            raise _lib.CbGpuError(_lib.ERR_INVALID, "no session")
+        i = np.ascontiguousarray(index, dtype=np.int32)
+        v = np.ascontiguousarray(value, dtype=np.float64)
+        t = None if tail is None else np.ascontiguousarray(tail, dtype=np.float64)
+        if i.ndim != 2 or i.shape[0] != self.n or v.shape != i.shape or (t is not None and t.shape != (self.n,)):
+            raise _lib.CbGpuError(_lib.ERR_INVALID, f"LengthMismatch: a teacher of {self.n} rows, got index {i.shape}, "
+                                  f"value {v.shape}, tail {None if t is None else t.shape}")
+        rc = _lib.check(self._L.cbgpu_multi_set_teacher(self._s, _ptr(i), _ptr(v), _ptr(t), i.shape[1],
+                                                        float(temperature)))
+        if rc == _lib.DECLINED:
+            self.decline_reason = _lib.last_error()
+        return rc == _lib.OK
+
     def end_device_training(self) -> None:
         if self._s:
             self._L.cbgpu_multi_end(self._s)

@@ -378,6 +378,21 @@ CBGPU_API int cbgpu_multi_grow_tree(cbgpu_multi_session* s, const double* approx
                                     int32_t* split_bin, int32_t* n_splits, double* leaf_values, void* leaf_of,
                                     int32_t leaf_of_bytes);
 
+/* Train a MultiClass session on a teacher's top logits instead of class
+ * indices (knowledge distillation; no counterpart in the reference).  Called
+ * between begin and the first grow; the grow calls' target is then NULL.
+ * Every tree follows der1 of cbgpu_distill (see there for the loss) over the
+ * approximants at `temperature`, and its leaves the softmax Hessian at it:
+ * at temperature T a fit's leaves are T times those of the same teacher
+ * probabilities at 1.
+ *  index [n][k]  classes, -1 = no entry (of equal classes in a row the first
+ *                counts);  value [n][k] the teacher's logits (-inf: ruled
+ *                out);  tail [n] ln sum exp(z / temperature) of its other
+ *                classes, or NULL;  k 1..256;  temperature 1e-3..1e3.
+ * Host arrays.  Declines other losses and ranking sessions. */
+CBGPU_API int cbgpu_multi_set_teacher(cbgpu_multi_session* s, const int32_t* index, const double* value,
+                                      const double* tail, int32_t k, double temperature);
+
 /* Loss parameters of the grouped families; NULL takes the defaults. */
 typedef struct {
     double l2_leaf_reg;     /* the unscaled l2 of PairLogitPairwise's scorer and leaves

@@ -178,3 +178,7 @@ def test_torch_can_be_imported_after_the_library():
     pytest.importorskip("torch")
     code = "import catboost_rs_b200 as cb; cb.load_library(); import torch"
     subprocess.run([sys.executable, "-c", code], check=True, timeout=300)
+
+
+def test_set_teacher_rejects_a_null_session_on_the_host():
+    refused(_lib.load().cbgpu_multi_set_teacher(None, None, None, None, 1, 1.0), "no session")

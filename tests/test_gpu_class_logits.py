@@ -513,3 +513,117 @@ def test_from_a_teachers_rows_to_drawn_labels():
     labels = cb.sample_classes(student, u, top_k=8)
     best = cb.top_logits(student, 8).index
     assert bool((best == labels[:, None]).any(dim=1).all())
+
+
+# ---- a booster trained on a teacher ------------------------------------------------------
+
+def columns(n, F, seed):
+    from oracle import oracle
+    rs = np.random.RandomState(seed)
+    X = rs.standard_normal((n, F)).astype(np.float32)
+    return X, [oracle.select_borders(X[:, f], 32) for f in range(F)], rs
+
+
+def fit(X, borders, K, **kw):
+    fp = cb.FitParams(loss="MultiClass", depth=4, iterations=4, learning_rate=0.2, l2_leaf_reg=3.0,
+                      boost_from_average=False, bootstrap_type=kw.pop("boot", "No"), random_seed=3)
+    return cb.fit_multiclass([X[:, f].copy() for f in range(X.shape[1])], borders, kw.pop("y", None), K, fp,
+                             staged=True, **kw)
+
+
+def same_trees(a, b, scale=1.0):
+    np.testing.assert_array_equal(a.split_feature, b.split_feature)
+    np.testing.assert_array_equal(a.split_bin, b.split_bin)
+    # sums of n values rounded to 2^-40 of their largest, and a Newton solve: the bar of the suite
+    assert np.abs(a.leaf_values - scale * b.leaf_values).max() <= 1e-9 * scale
+    assert np.abs(a.staged - scale * b.staged).max() <= 1e-9 * scale
+
+
+@pytest.mark.parametrize("boot", ["No", "Bernoulli"])
+def test_fit_on_a_teacher_that_is_sure_is_a_fit_on_labels(boot):
+    n, F, K = 6000, 6, 5
+    X, borders, rs = columns(n, F, 1)
+    y = rs.randint(0, K, n)
+    y[X[:, 0] > 0.3] = 2
+    w = rs.uniform(0.5, 2.0, n)
+    want = fit(X, borders, K, y=y, weights=w, boot=boot)
+    top = cb.TopLogits(y[:, None].astype(np.int32), np.zeros((n, 1)))
+    same_trees(fit(X, borders, K, teacher=top, weights=w, boot=boot), want)
+
+
+def test_fit_on_a_teacher_is_a_weighted_fit_on_every_class():
+    # soft targets q_c: the oracle's fit on every row once a class, weighted by q_c
+    from oracle import oracle
+    n, F, K = 3000, 5, 4
+    X, borders, rs = columns(n, F, 2)
+    z = 2.0 * np.nan_to_num(X[:, :K]) + 0.3 * rs.standard_normal((n, K))
+    q = np.exp(z - z.max(1, keepdims=True))
+    q /= q.sum(1, keepdims=True)
+    top = cb.top_logits(torch.from_numpy(z).cuda(), K)
+    got = fit(X, borders, K, teacher=top)
+    bins = oracle.quantize(X.T.copy(), borders)
+    # l2 is scaled by the mean weight: 1 / K over the expanded rows
+    o = oracle.train_multiclass(np.repeat(bins, K, axis=1), [len(b) for b in borders],
+                                np.tile(np.arange(K, dtype=np.int32), n), K, depth=4, iterations=4, learning_rate=0.2,
+                                l2_leaf_reg=3.0 * K, bootstrap_type="No", random_seed=3, weights=q.reshape(-1))
+    np.testing.assert_array_equal(got.split_feature, o.split_feature)
+    np.testing.assert_array_equal(got.split_bin, o.split_bin)
+    assert np.abs(got.leaf_values - o.leaf_values).max() <= 1e-9
+    # the tail's bucket of one class is that class
+    part = cb.top_logits(torch.from_numpy(z).cuda(), K - 1)
+    same_trees(fit(X, borders, K, teacher=part), got)
+    # temperature: probabilities of z / 2, leaves twice as large
+    half = cb.TopLogits(top.index, top.value / 2.0)
+    same_trees(fit(X, borders, K, teacher=cb.TopLogits(top.index, top.value), temperature=2.0),
+               fit(X, borders, K, teacher=half), 2.0)
+    # the loss of the staged approximants, as the device's own dim-major rows, against the definition
+    rows = torch.from_numpy(np.ascontiguousarray(got.staged[-1].T)).cuda().t()
+    check_distill(rows, cb.TopLogits(top.index, top.value), None, 1.0, "f64")
+    labels = cb.sample_classes(rows, torch.rand((n,), device="cuda"), top_k=2)
+    assert bool((cb.top_logits(rows, 2).index == labels[:, None]).any(dim=1).all())
+
+
+def test_teacher_refusals():
+    n, K = 50, 3
+    X, borders, rs = columns(n, 3, 3)
+    y = rs.randint(0, K, n)
+    top = cb.TopLogits(y[:, None], np.zeros((n, 1)))
+    with pytest.raises(ValueError):
+        fit(X, borders, K, y=y, teacher=top)
+    with pytest.raises(ValueError):
+        fit(X, borders, K)
+    with pytest.raises(RuntimeError, match="MultiClass"):
+        fit(X, borders, K, teacher=top, loss="MultiClassOneVsAll")
+    for bad in (cb.TopLogits(np.full((n, 1), K), np.zeros((n, 1))), cb.TopLogits(np.full((n, 1), -2), np.zeros((n, 1))),
+                cb.TopLogits(y[:, None], np.full((n, 1), np.nan)), cb.TopLogits(y[:, None], np.full((n, 1), np.inf)),
+                cb.TopLogits(y[:, None], np.zeros((n, 1)), np.full(n, np.nan)),
+                cb.TopLogits(y[:, None], np.zeros((n, 2))), cb.TopLogits(y[:9, None], np.zeros((9, 1))),
+                cb.TopLogits(y[:, None], np.zeros((n, 1)), np.zeros(n - 1)),
+                cb.TopLogits(np.zeros((n, 257), dtype=np.int32), np.zeros((n, 257)))):
+        with pytest.raises(cb.CbGpuError):
+            fit(X, borders, K, teacher=bad)
+    for t in (0.0, float("nan"), 1e4):
+        with pytest.raises(cb.CbGpuError):
+            fit(X, borders, K, teacher=top, temperature=t)
+    # a session's turn of calls: no teacher after the first tree, no target with a teacher
+    cfg = cb.DeviceTrainConfig()
+    for first in ("teacher", "target"):
+        rt = cb.B200MultiRuntime()
+        assert rt.begin_device_training_raw("MultiClass", 2, True, 1, "Cosine", [X[:, f].copy() for f in range(3)],
+                                            borders, None, n, 3, 33, 0.1, 3.0, cfg, approx_dim=K)
+        grow = lambda t: rt.grow_tree_on_device(None, t, [], family=("MultiOutput", None, K),  # noqa: E731
+                                                leaf_of_bytes=0, resident_approx=True)
+        if first == "teacher":
+            assert rt.set_teacher(top.index, top.value)
+            with pytest.raises(cb.CbGpuError, match="no target"):
+                grow(y)
+            assert len(grow(None).splits) == 2
+        else:
+            with pytest.raises(cb.CbGpuError, match="first call needs the target"):
+                grow(None)
+            grow(y)
+            with pytest.raises(cb.CbGpuError, match="target already"):
+                rt.set_teacher(top.index, top.value)
+        rt.end_device_training()
+    with pytest.raises(cb.CbGpuError, match="no session"):
+        cb.B200MultiRuntime().set_teacher(top.index, top.value)
