@@ -45,7 +45,7 @@ def build(verbose: bool = False, force: bool = False) -> str:
         if os.path.getmtime(OUT) >= newest:
             return OUT
     inc, libs = nccl_flags()
-    cmd = [nvcc_path(), "-std=c++17", "-O3", "-lineinfo", "-fmad=false", *ARCH,
+    cmd = [nvcc_path(), "-std=c++17", "-O3", "--threads", "0", "-lineinfo", "-fmad=false", *ARCH,
            "-shared", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
            "-ccbin", shutil.which("g++") or "g++",
            f"-I{os.path.join(os.path.dirname(HERE), 'include')}", *inc,
