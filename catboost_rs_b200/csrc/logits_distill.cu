@@ -46,6 +46,13 @@ __device__ __forceinline__ RowOut<C> distill_finish(double w, double t, double s
 
 __device__ __forceinline__ float part_exp(float x) { return __expf(x); }
 __device__ __forceinline__ double part_exp(double x) { return exp(x); }
+// exp(x) for x <= 0 of a narrow row
+__device__ __forceinline__ float row_exp(float x, const ExpTable&) { return __expf(x); }
+__device__ __forceinline__ double row_exp(double x, const ExpTable& t) { return t.exp<5, true>(x * ExpTable::kPerUnit); }
+__device__ __forceinline__ float row_exp(float d, const Scale<float>& sc, const ExpTable&) { return ex2(d * sc.c); }
+__device__ __forceinline__ double row_exp(double d, const Scale<double>& sc, const ExpTable& t) {
+    return t.exp<5, true>(d * sc.c * ExpTable::kPerUnit);
+}
 
 constexpr uint32_t kAbsent32 = 0xffffffffu;  // a NaN no arithmetic gives
 constexpr u64 kAbsent64 = ~0ull;
@@ -75,10 +82,10 @@ lg_distill_narrow_kernel(Rows<T> x, TeacherArgs tc, const typename Num<T>::C* __
     T* g = const_cast<T*>(x.data) + r0 * x.row_stride;
     const TileIo<T> io(g, x.row_stride, x.class_stride, V, rows);
     T* s = reinterpret_cast<T*>(lg_smem + ((size_t)tile * tgt_pitch * sizeof(C) + 15) / 16 * 16) + io.shift;
-    if (!direct) {
-        io.template copy<false>(s, g);
-        __syncthreads();
-    }
+    if (!direct) io.template copy<false>(s, g);
+    __shared__ ExpTable table;  // of f64 rows
+    if (sizeof(C) == 8) table.fill();
+    __syncthreads();
     const LaneTeam<G> t;
     const Items<G, ITEMS> mine(t, V);
     for (int r = threadIdx.x / G; r < rows; r += kLgThreads / G) {
@@ -132,7 +139,7 @@ lg_distill_narrow_kernel(Rows<T> x, TeacherArgs tc, const typename Num<T>::C* __
                 const int i = (int)tc.idx((r0 + r) * tc.k + j0 + t.rank);
                 const C ai = to_c(row[i]);
                 const double d = (double)tgt[i] * sc.inv_t - z_max;
-                const C rj = part_exp((C)d);
+                const C rj = row_exp((C)d, table);
                 r_sum += (double)rj;
                 if (rj != C(0)) cross += (double)rj * (d - ((double)ai - (double)m) * sc.inv_t);
                 tgt[i] = rj;
@@ -140,7 +147,7 @@ lg_distill_narrow_kernel(Rows<T> x, TeacherArgs tc, const typename Num<T>::C* __
             t.sync();
         }
         LG_EACH(it) {
-            const C e = lg_exp(a[it] - m, sc.c);
+            const C e = row_exp(a[it] - m, sc, table);
             if ((top >> it) & 1) {
                 sum_top += e;
                 if (G > 1) {
@@ -148,7 +155,7 @@ lg_distill_narrow_kernel(Rows<T> x, TeacherArgs tc, const typename Num<T>::C* __
                     continue;
                 }
                 const double d = (double)tgt[mine.first + it] * sc.inv_t - z_max;
-                const double rj = (double)part_exp((C)d);
+                const double rj = (double)row_exp((C)d, table);
                 r_sum += rj;
                 if (rj != 0.0) cross += rj * (d - ((double)a[it] - (double)m) * sc.inv_t);
                 tgt[mine.first + it] = (C)rj;
@@ -160,7 +167,7 @@ lg_distill_narrow_kernel(Rows<T> x, TeacherArgs tc, const typename Num<T>::C* __
         const double s_top = t.reduce((double)sum_top, OpSum()), s_rest = t.reduce((double)sum_rest, OpSum());
         r_sum = t.reduce(r_sum, OpSum());
         cross = t.reduce(cross, OpSum());
-        const double r_tail = exp(tl - z_max);
+        const double r_tail = (double)row_exp((C)(tl - z_max), table);
         RowOut<C> o = distill_finish<C>(w, temp, s_top, s_rest, r_sum + r_tail, r_tail, tl - z_max, cross);
         if (w == 0.0) {
             o = RowOut<C>{};

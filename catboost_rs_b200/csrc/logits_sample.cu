@@ -69,10 +69,11 @@ __device__ __forceinline__ u64 whole_mass(double e, double scale) {
 // it; a team finds the cut by halving an interval of logits.
 template <typename T, int G, int ITEMS>
 __device__ int sample_row(const LaneTeam<G>& t, const Items<G, ITEMS>& mine, const typename Num<T>::C (&a)[ITEMS], int V,
-                          int shift, const RowSampling& rs) {
+                          int shift, const RowSampling& rs, const ExpTable& table) {
     typedef typename Num<T>::C C;
     const double scale = power_of_2(shift);
     const double reach = (double)(shift + 2) * 0.6931471805599453 / rs.inv_t;  // behind it a weight is 0
+    const double per64 = rs.inv_t * ExpTable::kPerUnit;
     C m = -lg_inf(C());
     int bad = 0;
     LG_EACH(it) {
@@ -95,7 +96,7 @@ __device__ int sample_row(const LaneTeam<G>& t, const Items<G, ITEMS>& mine, con
     LG_EACH(it) {
         w[it] = 0;
         if (!mine.has(it)) continue;
-        const double e = a[it] == m ? 1.0 : exp(((double)a[it] - (double)m) * rs.inv_t);
+        const double e = a[it] == m ? 1.0 : table.exp<4, false>(((double)a[it] - (double)m) * per64);
         w[it] = whole_mass(e, scale);
         stay |= 1u << it;
         if (e < rs.min_p) small |= 1u << it;
@@ -104,20 +105,6 @@ __device__ int sample_row(const LaneTeam<G>& t, const Items<G, ITEMS>& mine, con
     // number or the mass of classes, reaches `target`.
     auto cut = [&](u64 target, auto by_mass) {
         constexpr bool kMass = decltype(by_mass)::value;
-        if (G == 1) {
-            uint32_t keep = 0;
-            LG_EACH(it) {
-                u64 before = 0;
-#pragma unroll
-                for (int j = 0; j < ITEMS; ++j) {  // what does not stay weighs nothing
-                    const bool first = j < it ? a[j] >= a[it] : (j > it && a[j] > a[it]);
-                    if (first && ((stay >> j) & 1)) before += kMass ? w[j] : 1;
-                }
-                if (((stay >> it) & 1) && before < target) keep |= 1u << it;
-            }
-            stay = keep;
-            return;
-        }
         // [lo, hi): where the last class that stays lies; it is halved until it holds one class or
         // one value
         u64 mass = 0;
@@ -145,7 +132,7 @@ __device__ int sample_row(const LaneTeam<G>& t, const Items<G, ITEMS>& mine, con
             if (!from(lo)) return;  // what would be cut weighs nothing
             int n_lo = n;
             while (n_lo - n_hi > 1) {
-                const C mid = lo * C(0.5) + hi * C(0.5);
+                const C mid = to_c(from_c<T>(lo * C(0.5) + hi * C(0.5)));  // a logit there can be
                 if (!(mid > lo && mid < hi)) break;
                 if (from(mid)) lo = mid, n_lo = n;
                 else hi = mid, n_hi = n;
@@ -171,8 +158,36 @@ __device__ int sample_row(const LaneTeam<G>& t, const Items<G, ITEMS>& mine, con
             if ((bits >> it) & 1) f += w[it];
         return f;
     };
-    if (rs.top_k < V) cut((u64)rs.top_k, std::false_type());
-    if (rs.top_p < 1.0) cut(mass_part(rs.top_p, t.sum(sum_of(stay))), std::true_type());
+    if (G == 1) {
+        if (rs.top_k < V || rs.top_p < 1.0) {
+            // what comes before each class, from one comparison a pair; before a class that top-k
+            // keeps all stays, so the masses serve top-p too
+            int rank[ITEMS] = {};
+            u64 before[ITEMS] = {};
+#pragma unroll
+            for (int j = 1; j < ITEMS; ++j)
+#pragma unroll
+                for (int i = 0; i < j; ++i) {
+                    const bool first = !(a[j] > a[i]);  // places without a class hold -inf
+                    rank[j] += first, rank[i] += !first;
+                    if (first) before[j] += w[i];
+                    else before[i] += w[j];
+                }
+            u64 total = 0;
+#pragma unroll
+            for (int it = 0; it < ITEMS; ++it) {
+                if (rank[it] >= rs.top_k) stay &= ~(1u << it);
+                total += (stay >> it) & 1 ? w[it] : 0;
+            }
+            const u64 goal = rs.top_p < 1.0 ? mass_part(rs.top_p, total) : total + 1;
+#pragma unroll
+            for (int it = 0; it < ITEMS; ++it)
+                if (before[it] >= goal) stay &= ~(1u << it);
+        }
+    } else {
+        if (rs.top_k < V) cut((u64)rs.top_k, std::false_type());
+        if (rs.top_p < 1.0) cut(mass_part(rs.top_p, t.sum(sum_of(stay))), std::true_type());
+    }
     stay &= ~small;
     const u64 own = sum_of(stay);
     u64 upto = t.exscan(own);
@@ -196,23 +211,25 @@ lg_sample_narrow_kernel(Rows<T> x, SampleArgs a, int shift, int tile, int direct
     T* g = const_cast<T*>(x.data) + r0 * x.row_stride;
     const TileIo<T> io(g, x.row_stride, x.class_stride, V, rows);
     T* s = reinterpret_cast<T*>(lg_smem) + io.shift;
-    if (!direct) {
-        io.template copy<false>(s, g);
-        __syncthreads();
-    }
+    if (!direct) io.template copy<false>(s, g);
+    __shared__ ExpTable table;
+    table.fill();
+    __syncthreads();
     const LaneTeam<G> t;
     const Items<G, ITEMS> mine(t, V);
     for (int r = threadIdx.x / G; r < rows; r += kLgThreads / G) {
-        C v[ITEMS] = {};
+        C v[ITEMS];
+#pragma unroll
+        for (int it = 0; it < ITEMS; ++it) v[it] = -lg_inf(C());
         if (direct) {
             const T* row = g + r * x.row_stride;
             LG_EACH(it)
-                v[it] = mine.has(it) ? to_c(row[(int64_t)(mine.first + it) * x.class_stride]) : C(0);
+                v[it] = mine.has(it) ? to_c(row[(int64_t)(mine.first + it) * x.class_stride]) : -lg_inf(C());
         } else {
             const T* row = s + (size_t)r * io.pitch;
-            LG_EACH(it) v[it] = mine.has(it) ? to_c(row[mine.first + it]) : C(0);
+            LG_EACH(it) v[it] = mine.has(it) ? to_c(row[mine.first + it]) : -lg_inf(C());
         }
-        const int got = sample_row<T, G, ITEMS>(t, mine, v, V, shift, row_sampling(a, r0 + r, V));
+        const int got = sample_row<T, G, ITEMS>(t, mine, v, V, shift, row_sampling(a, r0 + r, V), table);
         if (t.rank == 0) index[r0 + r] = got;
     }
 }
@@ -224,34 +241,6 @@ lg_sample_narrow_kernel(Rows<T> x, SampleArgs a, int shift, int tile, int direct
 // top-k cuts, a histogram over the logits (counts, and masses in f32) shows in which bin the cut lies;
 // the bin's classes are collected and sorted, and the cut is then taken with
 // exact masses, which also show whether the bin was the right one.
-
-// exp of a non-positive number by the table-driven method of P. T. P. Tang (ACM TOMS 15, 1989): with
-// x log2(e) = (n + r) / 64, |r| <= 1/2, it is 2^(n / 64), from a table of 64 and an exponent, times a polynomial
-// in r ln2 / 64 (below 0.0055: degree 4 leaves 4e-14, as much as a mass is rounded by).  The draw from whole
-// rows is bound by these operations: 12 in 64 bits a class, where exp() and its range checks take
-// some 30 (64 x 131071 f32: 55 us with 15 and the checks class by class).
-constexpr int kExpTable = 64;
-struct ExpTable {
-    double of[kExpTable];
-    __device__ void fill() {  // by the block; a barrier follows
-        if (threadIdx.x < kExpTable) of[threadIdx.x] = exp2((double)threadIdx.x / kExpTable);
-    }
-    // 2^(y / 64) for y <= 0; y below -64000 counts as that
-    __device__ double operator()(double y) const {
-        const uint32_t hi = (uint32_t)__double2hiint(y);  // of negative numbers the larger is further down
-        y = __hiloint2double((int)(hi < 0xc0ef4000u ? hi : 0xc0ef4000u), __double2loint(y));
-        const double t = y + 6755399441055744.0;  // 1.5 2^52: the low word of t is n
-        const int n = __double2loint(t);
-        const double r = y - (t - 6755399441055744.0);
-        constexpr double c = 0.6931471805599453 / kExpTable;
-        double p = fma(r, c * c * c * c / 24.0, c * c * c / 6.0);
-        p = fma(r, p, c * c / 2.0);
-        p = fma(r, p, c);
-        const double b = of[n & (kExpTable - 1)];
-        const double e = fma(b * r, p, b);
-        return __hiloint2double(__double2hiint(e) + ((n >> 6) << 20), __double2loint(e));
-    }
-};
 
 template <typename T>
 struct Weigh {
@@ -265,8 +254,8 @@ struct Weigh {
     double per64;  // 64 log2(e) / T
     __device__ Weigh(C m_, double inv_t_, int shift, const ExpTable* t)
         : m(m_), inv_t(inv_t_), scale(power_of_2(shift)), min_p(0.0), last{0, 0xffffffffu}, cut(false),
-          infinite(m_ == lg_inf(C())), table(t), per64(inv_t_ * (kExpTable * 1.4426950408889634)) {}
-    __device__ double finite_share(C a) const { return (*table)(((double)a - (double)m) * per64); }
+          infinite(m_ == lg_inf(C())), table(t), per64(inv_t_ * ExpTable::kPerUnit) {}
+    __device__ double finite_share(C a) const { return table->template exp<4, false>(((double)a - (double)m) * per64); }
     // infinite logits share the mass among themselves
     __device__ double share(C a) const { return infinite ? (a == m ? 1.0 : 0.0) : finite_share(a); }
     __device__ u64 whole(double e) const { return whole_mass(e, scale); }

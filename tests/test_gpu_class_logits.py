@@ -404,6 +404,42 @@ def test_many_rows(n, V, dtype, layout):
             assert int(got[r]) == ref.sample(host(host_x[j:j + 1])[0], float(u[r]), **full), (kw, r)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("V,layout", [(17, "rows"), (40, "rows"), (100, "offset"), (128, "rows"), (64, "dims")])
+def test_top_logits_of_very_many_rows(V, layout, dtype):
+    # enough rows for a thread a row; the rows that can go wrong are among them
+    n = 148 * 256 + 5
+    a = np.random.RandomState(V).standard_normal((n, V)) * 3
+    a[0] = 0.0
+    a[1] = -np.inf
+    a[2, 3:] = -np.inf
+    a[3, V // 2] = np.nan
+    a[4] = np.where(np.arange(V) % 2, -0.0, 0.0)
+    a[5] = np.arange(V) * 0.25
+    a[6] = -np.arange(V) * 0.25
+    a[7] = np.arange(V) // 4 % 3
+    a[8, V - 1] = np.inf
+    a[9] = np.nan
+    a[10, :9] = 300.0  # the rest lies far below
+    x = put(a, dtype, layout)
+    some_rows = torch.arange(0, 40, device="cuda")
+    h = host(x.index_select(0, some_rows))
+    for k in (1, 3, 4, 8):
+        got = cb.top_logits(x, k, temperature=0.8)
+        for r in range(40):
+            wi, wv, wt = ref.top(h[r], k, 0.8)
+            assert (got.index[r].cpu().numpy() == wi).all(), (r, got.index[r], wi)
+            assert np.array_equal(host(got.value[r]), wv, equal_nan=True)
+            t = float(got.tail[r])
+            if np.isfinite(wt):
+                assert abs(t - wt) <= 130 * unit(dtype) + 3 * unit(dtype) * abs(wt), (r, t, wt)
+            else:
+                # +inf among the rest: the difference of infinities is a NaN
+                assert np.array_equal(t, wt, equal_nan=True) or wt == np.inf, (r, t, wt)
+        assert torch.equal(got.index, cb.top_logits(x, k).index)
+        assert cb.top_logits(x, k, tail=False).tail is None
+
+
 # ---- how they are called ---------------------------------------------------------------
 
 def batch(V, dtype="bf16", n=130):
