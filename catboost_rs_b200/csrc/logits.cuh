@@ -110,6 +110,8 @@ __device__ __forceinline__ double of_key(u64 k) {
 
 __device__ __forceinline__ float lg_inf(float) { return __int_as_float(0x7f800000); }
 __device__ __forceinline__ double lg_inf(double) { return __longlong_as_double(0x7ff0000000000000ll); }
+__device__ __forceinline__ float lowest(float) { return __int_as_float((int)0xff7fffffu); }  // of the finite numbers
+__device__ __forceinline__ double lowest(double) { return __longlong_as_double((long long)0xffefffffffffffffull); }
 
 // exp((a - m) / T).  f32: 2^((a - m) c) with c = log2(e) / T rounded to f32 (a relative change of the
 // temperature by at most 2^-24, taken for teacher and student alike).
@@ -750,7 +752,6 @@ constexpr int kSegments = 8192 / 32 + 1;  // a block holds up to 8193 vectors
 constexpr int kGather = 3;
 constexpr int kBins = 1024;    // of the sampler's histogram, which lies where the list comes to lie
 struct SampleHist {
-    float mass[kBins];
     uint32_t count[kBins];
 };
 
@@ -1118,11 +1119,14 @@ struct Tile {
     int rows;
     size_t smem;
 };
-// Rows a narrow block stages: about 24 KB (8 blocks an SM), at least one for each lane team.
-Tile narrow_tile(int V, size_t bytes_a_class, int teams) {
+// Rows a narrow block stages: about 24 KB (8 blocks an SM), but not so many that the SMs have less than
+// four blocks each, and at least one for each lane team.
+Tile narrow_tile(int64_t n, int V, size_t bytes_a_class, int teams) {
     const size_t row = (size_t)(V | 1) * bytes_a_class;
     size_t rows = 24576 / row;
-    rows = rows < (size_t)teams ? (size_t)teams : rows / teams * teams;
+    const size_t share = (size_t)((n + 148 * 4 - 1) / (148 * 4));
+    rows = rows < share ? rows : share;
+    rows = rows <= (size_t)teams ? (size_t)teams : (rows + teams - 1) / teams * teams;
     return Tile{(int)rows, rows * row + 32};
 }
 

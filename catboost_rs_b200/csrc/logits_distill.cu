@@ -471,7 +471,7 @@ int run_distill(const cbgpu_logits* x, const cbgpu_teacher* tc, const void* weig
     }
     auto narrow = [&](auto kernel, int lanes) {
         const bool direct = lanes == 1 && rows.class_stride > rows.row_stride && (!der1 || dcs > drs);
-        Tile t = narrow_tile(rows.V, sizeof(T) + sizeof(C), kLgThreads / lanes);
+        Tile t = narrow_tile(rows.n, rows.V, sizeof(T) + sizeof(C), kLgThreads / lanes);
         if (direct) t = Tile{kLgThreads, (size_t)kLgThreads * (rows.V | 1) * sizeof(C) + 16};
         return lg_launch(who, kernel, tiles_of(rows.n, t.rows), t.smem, st, rows, ta, (const C*)tc->tail,
                          (const C*)weight, temp, sc, t.rows, (int)direct, (C*)loss, (T*)der1, drs, dcs);

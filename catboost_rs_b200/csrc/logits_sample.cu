@@ -237,10 +237,11 @@ lg_sample_narrow_kernel(Rows<T> x, SampleArgs a, int shift, int tile, int direct
 // ---- wide rows -------------------------------------------------------------------------------
 //
 // top-k up to kLgMaxTop: the first block collects the first k classes and does the rest alone.
-// Else each class that can be drawn is weighed once or twice.  Where top-p or a larger
-// top-k cuts, a histogram over the logits (counts, and masses in f32) shows in which bin the cut lies;
-// the bin's classes are collected and sorted, and the cut is then taken with
-// exact masses, which also show whether the bin was the right one.
+// Else each class is weighed once.  Where top-p or a larger top-k cuts, a
+// histogram of the logits shows in which bin the cut lies (a bin's classes weigh nearly the same, so
+// counts are enough: f32 masses added in shared memory took three times as long); the
+// bin's classes and its neighbours' are collected and sorted, and the cut is then taken
+// with exact masses, which also show whether the bin was the right one.
 
 template <typename T>
 struct Weigh {
@@ -269,11 +270,13 @@ struct Weigh {
         const double e = share(a);
         return e < min_p ? 0 : whole(e);
     }
+    // no cut, no min-p, no infinite logits
+    __device__ bool plain() const { return !(cut || infinite || min_p > 0.0); }
     // the mass of a vector whose first class is i
     template <int N>
     __device__ u64 vector(int i, const C (&a)[N]) const {
         u64 sum = 0;
-        if (cut || infinite || min_p > 0.0) {
+        if (!plain()) {
 #pragma unroll
             for (int j = 0; j < N; ++j) sum += (*this)(i + j, a[j]);
             return sum;
@@ -313,29 +316,15 @@ __device__ __forceinline__ u64 block_total(u64 v, u64 (&warp_part)[kLgWarps]) {
     return t;
 }
 
-// Draws from the classes that stay; every block of the cluster, one of them writes.
+// Draws from the classes that stay, given the mass that stays in each of the
+// block's segments of 32 vectors (sh.segment, behind a barrier); every block of the cluster, one of
+// them writes.
 template <typename T, typename Sh>
-__device__ void wide_draw(const ClusterInfo& cl, Sh& sh, const WideRow<T>& w, const uint4* s,
-                          const Weigh<T>& weigh, double u, int& turn, int32_t* index) {
+__device__ void segment_draw(const ClusterInfo& cl, Sh& sh, const WideRow<T>& w, const uint4* s, const Weigh<T>& weigh,
+                             int segs, double u, int& turn, int32_t* index) {
     constexpr int VE = WideRow<T>::VE;
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-    const LaneTeam<32> warp;
-    u64* seg = sh.segment;  // in place of the list: no block is at it any more
-    auto lane_mass = [&](int v) {
-        u64 own = 0;
-        if (v < w.nv) {
-            typename Num<T>::C a[VE];
-            unpack(s[v], a, T());
-            own = weigh.vector(w.first(v), a);
-        }
-        return own;
-    };
-    const int segs = w.nv > 0 ? (w.nv + 31) / 32 : 0;
-    for (int g = wid; g < segs; g += kLgWarps) {
-        const u64 sum = warp.sum(lane_mass(g * 32 + lane));
-        if (lane == 0) seg[g] = sum;
-    }
-    __syncthreads();
+    const u64* seg = sh.segment;
     // a run of segments a thread
     const int per = (segs + kLgThreads - 1) / kLgThreads, g0 = (int)threadIdx.x * per;
     u64 own = 0, block[1];
@@ -363,11 +352,14 @@ __device__ void wide_draw(const ClusterInfo& cl, Sh& sh, const WideRow<T>& w, co
     __syncthreads();
     if (wid != 0) return;
     const int v = s_seg * 32 + lane;
-    const u64 mine = lane_mass(v);
-    u64 sum = s_upto + warp.exscan(mine);
-    if (sum < target && sum + mine >= target) {
-        typename Num<T>::C a[VE];
+    typename Num<T>::C a[VE];
+    u64 mine = 0;
+    if (v < w.nv) {
         unpack(s[v], a, T());
+        mine = weigh.vector(w.first(v), a);
+    }
+    u64 sum = s_upto + LaneTeam<32>().exscan(mine);
+    if (sum < target && sum + mine >= target) {
 #pragma unroll
         for (int j = 0; j < VE; ++j) {
             const u64 next = sum + weigh(w.first(v) + j, a[j]);
@@ -375,6 +367,28 @@ __device__ void wide_draw(const ClusterInfo& cl, Sh& sh, const WideRow<T>& w, co
             sum = next;
         }
     }
+}
+
+// The segments' masses class by class, and the draw.
+template <typename T, typename Sh>
+__device__ void wide_draw(const ClusterInfo& cl, Sh& sh, const WideRow<T>& w, const uint4* s, const Weigh<T>& weigh,
+                          double u, int& turn, int32_t* index) {
+    const int lane = threadIdx.x & 31;
+    const int segs = w.nv > 0 ? (w.nv + 31) / 32 : 0;
+    const LaneTeam<32> warp;
+    for (int g = threadIdx.x >> 5; g < segs; g += kLgWarps) {
+        const int v = g * 32 + lane;
+        u64 own = 0;
+        if (v < w.nv) {
+            typename Num<T>::C a[WideRow<T>::VE];
+            unpack(s[v], a, T());
+            own = weigh.vector(w.first(v), a);
+        }
+        own = warp.sum(own);
+        if (lane == 0) sh.segment[g] = own;
+    }
+    __syncthreads();
+    segment_draw(cl, sh, w, s, weigh, segs, u, turn, index);
 }
 
 // The draw from the first block's sorted list of k <= kLgThreads classes: a thread a class.
@@ -402,8 +416,12 @@ __device__ void list_draw(Sh& sh, int k, const Weigh<T>& weigh, const RowSamplin
     if (upto < target && upto + own >= target) *index = (int32_t)sh.idx[j];
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kLgThreads)
+// What a launch's rows can ask for, so that its kernel holds no registers for the rest: no cut at all,
+// a top-k from the list alone, or anything (settings by rows).
+enum WidePath { kPathPlain, kPathList, kPathAny };
+
+template <typename T, WidePath kPath>
+__global__ void __launch_bounds__(kLgThreads, 3)
 lg_sample_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, SampleArgs a, int shift,
                       int32_t* __restrict__ index) {
     typedef typename Num<T>::C C;
@@ -428,7 +446,7 @@ lg_sample_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, SampleArg
     int32_t* out = index + r;
     int turn = 0;
     if (cl.blocks > 1) cluster_wait();  // every block runs: its shared memory can be written
-    if (rs.top_k <= kLgMaxTop && !rs.greedy) {
+    if (kPath != kPathPlain && rs.top_k <= kLgMaxTop && !rs.greedy) {
         C rest;
         bool exact, bad = mine != mine;
         const int n = wide_top(cl, sh, w, s, bad ? -lg_inf(C()) : mine, rs.top_k, turn, rest, exact, bad,
@@ -447,7 +465,7 @@ lg_sample_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, SampleArg
     }
     // the largest logit, and the least that is not masked (negated)
     C low = -lg_inf(C());
-    if (rs.top_k < x.V || rs.top_p < 1.0)
+    if (kPath == kPathAny && (rs.top_k < x.V || rs.top_p < 1.0))
         each_place(w, s, [&](int, C v, int) { low = v != -lg_inf(C()) ? OpMax()(low, -v) : low; });
     C ends[2] = {mine, low};
     block_reduce(ends, red_max, [](C p, C q) { return VecMaxNan<C>::both(p, q); });
@@ -480,72 +498,66 @@ lg_sample_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, SampleArg
         return;
     }
     Weigh<T> weigh(m, rs.inv_t, shift, &table);
-    if (rs.top_k < x.V || rs.top_p < 1.0) {
+    if (kPath == kPathAny && (rs.top_k < x.V || rs.top_p < 1.0)) {
         const bool by_count = rs.top_k < x.V, by_mass = rs.top_p < 1.0;
         // behind it a weight is below a quarter of the last bit: 0
         const float reach = (float)((double)(shift + 2) * 0.6931471805599453 / rs.inv_t);
         const float range = fminf((float)(m + ends[1]), reach);
         const float per_bin = range > 0.0f && range < lg_inf(0.0f) ? (float)(kBins - 1) / range : 0.0f;
         auto bin_of = [&](C v) {  // larger logits have lower bins
-            const float d = v == m ? 0.0f : (float)(m - v) * per_bin;
-            return d < (float)(kBins - 1) ? (int)d : kBins - 1;
+            if (weigh.infinite) return v == m ? 0 : kBins - 1;
+            const float d = fminf((float)(m - v) * per_bin, (float)(kBins - 1));
+            return __float_as_int(d + 8388608.0f) & (kBins - 1);
         };
-        for (int i = tid; i < kBins; i += kLgThreads) sh.hist.mass[i] = 0.0f, sh.hist.count[i] = 0u;
+        for (int i = tid; i < kBins; i += kLgThreads) sh.hist.count[i] = 0u;
         __syncthreads();
-        const float c = (float)(rs.inv_t * 1.4426950408889634);
-        each_class(w, s, [&](int, C v, int) {
-            const int b = bin_of(v);
-            if (by_mass) atomicAdd(&sh.hist.mass[b], v == m ? 1.0f : ex2((float)(v - m) * c));
-            if (by_count) atomicAdd(&sh.hist.count[b], 1u);
-        });
+        // (places outside the row, -inf, weigh nothing and are counted in the last bin, behind any cut)
+        each_place(w, s, [&](int, C v, int) { atomicAdd(&sh.hist.count[bin_of(v)], 1u); });
         __shared__ struct {
-            int bin, count_bin;
-            u64 above, mass;
+            int bin, count_bin;  // top-p's and top-k's
+            u64 above;           // classes before top-k's bin
         } found;
-        // the first block adds the histograms up and gives the bins to all.  The order in which the f32
-        // masses are added is open: they only say where to look
+        // the first block adds the histograms up and gives the bins to all
         if (cl.blocks > 1) {
             cl.sync();
             if (cl.rank != 0) {
                 SampleHist* to = cl.of(&sh.hist, 0);
-                for (int i = tid; i < kBins; i += kLgThreads) {
-                    if (by_mass && sh.hist.mass[i] != 0.0f) atomicAdd(&to->mass[i], sh.hist.mass[i]);
-                    if (by_count && sh.hist.count[i] != 0u) atomicAdd(&to->count[i], sh.hist.count[i]);
-                }
+                for (int i = tid; i < kBins; i += kLgThreads)
+                    if (sh.hist.count[i] != 0u) atomicAdd(&to->count[i], sh.hist.count[i]);
             }
         }
         cl.sync();
         if (cl.rank == 0) {
             constexpr int kPer = kBins / kLgThreads;
-            float mass_bin[kPer];
-            u64 mass_own = 0, count_own = 0, mass_all, count_all;
+            // masses in 2^-20: a bin weighs its count times its middle's weight
+            const float c = per_bin > 0.0f ? (float)(rs.inv_t * 1.4426950408889634) / per_bin : 0.0f;
+            u64 mass_bin[kPer], mass_own = 0, count_own = 0, mass_all, count_all;
             for (int j = 0; j < kPer; ++j) {
-                mass_bin[j] = sh.hist.mass[tid * kPer + j];
-                mass_own += (u64)((double)mass_bin[j] * 1048576.0);
-                count_own += sh.hist.count[tid * kPer + j];
+                const int bin = tid * kPer + j;
+                mass_bin[j] = (u64)((double)sh.hist.count[bin] * (double)ex2(-(float)bin * c) * 1048576.0);
+                mass_own += mass_bin[j];
+                count_own += sh.hist.count[bin];
             }
             const u64 mass_upto = block_exscan(mass_own, sh.warp_part[0], mass_all);
             const u64 count_upto = block_exscan(count_own, sh.warp_part[1], count_all);
-            if (tid == 0) found.bin = 0, found.count_bin = 0, found.above = 0, found.mass = mass_all;
+            __shared__ u64 s_mass;  // of what top-k leaves, to a bin
+            if (tid == 0) found.bin = 0, found.count_bin = 0, found.above = 0, s_mass = mass_all;
             __syncthreads();
             const u64 k = (u64)rs.top_k;
             if (by_count && count_upto < k && count_upto + count_own >= k) {
                 u64 above = count_upto, mass = mass_upto;
                 int j = 0;
-                for (; above + sh.hist.count[tid * kPer + j] < k; ++j) {
-                    above += sh.hist.count[tid * kPer + j];
-                    mass += (u64)((double)mass_bin[j] * 1048576.0);
-                }
+                for (; above + sh.hist.count[tid * kPer + j] < k; ++j) above += sh.hist.count[tid * kPer + j], mass += mass_bin[j];
                 found.count_bin = tid * kPer + j, found.above = above;
-                found.mass = mass + (u64)((double)mass_bin[j] * 1048576.0);
+                s_mass = mass + mass_bin[j];
             }
             __syncthreads();
-            const u64 goal = (u64)(rs.top_p * (double)found.mass);
+            const u64 goal = (u64)(rs.top_p * (double)s_mass);
             if (by_mass && mass_upto < goal && mass_upto + mass_own >= goal) {
                 u64 upto = mass_upto;
                 int j = 0;
                 for (; j + 1 < kPer; ++j) {
-                    upto += (u64)((double)mass_bin[j] * 1048576.0);
+                    upto += mass_bin[j];
                     if (upto >= goal) break;
                 }
                 found.bin = tid * kPer + j;
@@ -574,8 +586,8 @@ lg_sample_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, SampleArg
             const u64 above = found.above;
             weigh.cut = bin < kBins - 1 || range < reach;  // else what is cut weighs nothing
             if (weigh.cut)
-                each_class(w, s, [&](int i, C v, int) {
-                    if (bin_of(v) == bin) push(i, v);
+                each_place(w, s, [&](int i, C v, int) {
+                    if (bin_of(v) == bin && w.valid(i)) push(i, v);
                 });
             cl.sync();
             const int n = cl.of(&sh, 0)->count;
@@ -593,32 +605,75 @@ lg_sample_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, SampleArg
             }
         }
         if (by_mass) {
+            // The masses above the bin are kept by segments on the way (lane r of a warp has the r-th of its
+            // segments), so that the draw has only the bin's own classes to add.
+            const int lane = tid & 31, wid = tid >> 5, segs = w.nv > 0 ? (w.nv + 31) / 32 : 0;
+            constexpr int VE = WideRow<T>::VE;
+            u64 kept = 0;
             int bin = found.bin, lo = -1, hi = kBins, step = 1;  // the cut's bin is in (lo, hi)
             for (bool first = !by_count;; first = false) {
                 if (!first) restart();
-                u64 sums[3] = {0, 0, 0};  // of all that stays; above the bin; in it
-                each_place(w, s, [&](int i, C v, int) {
-                    if (!weigh.stays(i, v)) return;
-                    const u64 f = weigh.mass(v);
-                    const int b = bin_of(v);
-                    sums[0] += f;
-                    sums[1] += b < bin ? f : 0;
-                    if (b == bin && w.valid(i)) {
-                        sums[2] += f;
-                        push(i, v);
+                // logits above `high` are before the bin's neighbours, those from `low` on are in one of the three
+                const C high = per_bin > 0.0f && bin >= 2 ? m - (C)(((float)bin - 1.5f) / per_bin) : lg_inf(C());
+                C low = per_bin > 0.0f && bin + 2 < kBins ? m - (C)(((float)bin + 1.5f) / per_bin) : -lg_inf(C());
+                low = OpMax()(low, lowest(C()));  // not the masked classes
+                u64 sums[3] = {0, 0, 0};          // of all that stays; above; collected
+                if (tid == 0) sh.vectors = 0;
+                __syncthreads();
+                auto weigh_all = [&](auto plain) {
+                    int round = 0;
+                    for (int g = wid; g < segs; g += kLgWarps, ++round) {
+                        const int v = g * 32 + lane;
+                        u64 own = 0;  // above, and not too small for min-p
+                        if (v < w.nv) {
+                            C a[VE];
+                            unpack(s[v], a, T());
+                            const int i = w.first(v);
+#pragma unroll
+                            for (int j = 0; j < VE; ++j) {
+                                u64 f;
+                                if (decltype(plain)::value) {
+                                    f = weigh.whole(weigh.finite_share(a[j]));
+                                    if (a[j] > high) own += f;
+                                } else {
+                                    if (!weigh.stays(i + j, a[j])) continue;
+                                    const double e = weigh.share(a[j]);
+                                    f = weigh.whole(e);
+                                    if (a[j] > high) {
+                                        sums[1] += f;
+                                        own += e < rs.min_p ? 0 : f;
+                                    }
+                                }
+                                sums[0] += f;
+                                if (a[j] <= high && a[j] >= low && w.valid(i + j)) {
+                                    sums[2] += f;
+                                    push(i + j, a[j]);
+                                    const int p = atomicAdd(&sh.vectors, 1);
+                                    if (p < kHits) sh.hit[p] = (uint16_t)(v * VE + j);
+                                }
+                            }
+                        }
+                        if (decltype(plain)::value) sums[1] += own;
+                        own = LaneTeam<32>().sum(own);
+                        if (lane == round) kept = own;
                     }
-                });
+                };
+                if (weigh.plain() && !(rs.min_p > 0.0)) weigh_all(std::true_type());
+                else weigh_all(std::false_type());
                 cluster_total<3>(cl, sh, sums, turn);
                 const u64 above = sums[1], within = sums[2], goal = mass_part(rs.top_p, sums[0]);
-                if (above >= goal || above + within < goal) {  // the f32 masses were a little off: a bin near
-                    if (above >= goal) hi = bin, bin = bin - step > lo ? bin - step : lo + 1;
-                    else lo = bin, bin = bin + step < hi ? bin + step : hi - 1;
+                const bool before = above >= goal, behind = above + within < goal;
+                if ((before || behind) && hi - lo > 2) {  // the bins' weights were a little off: bins near
+                    if (before) hi = bin - 1 > lo ? bin - 1 : lo + 1, bin = bin - 1 - step;
+                    else lo = bin + 1 < hi ? bin + 1 : hi - 1, bin = bin + 1 + step;
+                    bin = bin > lo ? (bin < hi ? bin : hi - 1) : lo + 1;
+                    bin = bin < 0 ? 0 : (bin < kBins ? bin : kBins - 1);
                     step *= 2;
                     continue;
                 }
                 const int n = cl.of(&sh, 0)->count;
                 Ranked<Key> last;
-                if (n <= kTopCap) {
+                if (n <= kTopCap && !before && !behind) {
                     if (cl.rank == 0) {
                         sort_list(sh, n);
                         // a run of the list a thread
@@ -645,7 +700,21 @@ lg_sample_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, SampleArg
                 }
                 weigh.last = last;
                 weigh.cut = true;
-                break;
+                weigh.min_p = rs.min_p;
+                // (the list is read: cl.sync or cluster_select came after)
+                // (of the block alone: what follows goes round the cluster once either way)
+                if (before || behind || segs > 32 * kLgWarps || sh.vectors > kHits) break;  // weighed anew below
+                const int g = wid + kLgWarps * lane;
+                if (g < segs) sh.segment[g] = kept;
+                __syncthreads();
+                for (int p = tid; p < sh.vectors; p += kLgThreads) {
+                    const int at = sh.hit[p];
+                    const C a = to_c(reinterpret_cast<const T*>(s)[at]);
+                    atomicAdd(&sh.segment[at / (VE * 32)], weigh(w.first(0) + at, a));
+                }
+                __syncthreads();
+                segment_draw(cl, sh, w, s, weigh, segs, rs.u, turn, out);
+                return;
             }
         }
     }
@@ -665,11 +734,18 @@ int run_sample(const cbgpu_logits* x, const cbgpu_sampling* s, int32_t* index, c
     const int shift = bits < 10 ? 52 : 62 - bits;  // at most what a 64-bit exponential holds
     if (is_wide(rows.n, rows.V)) {
         const Wide w = wide_shape<T>(rows.n, rows.V);
-        return lg_launch_wide(who, lg_sample_wide_kernel<T>, rows.n, w, w.smem, st, w.ahead, rows, a, shift, index);
+        auto wide = [&](auto kernel) {
+            return lg_launch_wide(who, kernel, rows.n, w, w.smem, st, w.ahead, rows, a, shift, index);
+        };
+        const bool by_rows = a.top_k_rows || a.top_p_rows;
+        const int k = a.top_k > 0 && a.top_k < rows.V ? a.top_k : rows.V;
+        if (!by_rows && k <= kLgMaxTop) return wide(lg_sample_wide_kernel<T, kPathList>);
+        if (!by_rows && k == rows.V && a.top_p >= 1.0) return wide(lg_sample_wide_kernel<T, kPathPlain>);
+        return wide(lg_sample_wide_kernel<T, kPathAny>);
     }
     auto narrow = [&](auto kernel, int lanes) {
         const bool direct = lanes == 1 && rows.class_stride > rows.row_stride;
-        Tile t = narrow_tile(rows.V, sizeof(T), kLgThreads / lanes);
+        Tile t = narrow_tile(rows.n, rows.V, sizeof(T), kLgThreads / lanes);
         if (direct) t = Tile{kLgThreads, 0};
         return lg_launch(who, kernel, tiles_of(rows.n, t.rows), t.smem, st, rows, a, shift, t.rows, (int)direct, index);
     };

@@ -326,7 +326,7 @@ int run_top(const cbgpu_logits* x, int k, double temp, void* value, int32_t* ind
                               (C*)tail);
     }
     auto narrow = [&](auto kernel, int lanes) {
-        const Tile t = narrow_tile(rows.V, sizeof(T), kLgThreads / lanes);
+        const Tile t = narrow_tile(rows.n, rows.V, sizeof(T), kLgThreads / lanes);
         return lg_launch(who, kernel, tiles_of(rows.n, t.rows), t.smem, st, rows, k, sc, t.rows, (T*)value, index,
                          (C*)tail);
     };
