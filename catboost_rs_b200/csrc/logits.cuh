@@ -204,11 +204,27 @@ struct LaneTeam {
         if (G > 1) __syncwarp(mask);
     }
     template <typename V, typename Op>
-    __device__ V reduce(V v, Op op) const {
+    __device__ V steps(V v, Op op) const {
 #pragma unroll
         for (int o = G / 2; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(mask, v, o));
         return v;
     }
+    template <typename V, typename Op>
+    __device__ V reduce(V v, Op op) const {
+        return steps(v, op);
+    }
+    // a warp has these in one instruction
+    __device__ uint32_t reduce(uint32_t v, OpMax) const { return G == 32 ? __reduce_max_sync(0xffffffffu, v) : steps(v, OpMax()); }
+    __device__ uint32_t reduce(uint32_t v, OpMin) const { return G == 32 ? __reduce_min_sync(0xffffffffu, v) : steps(v, OpMin()); }
+    __device__ int reduce(int v, OpMin) const { return G == 32 ? __reduce_min_sync(0xffffffffu, v) : steps(v, OpMin()); }
+    __device__ int reduce(int v, OpOr) const { return G == 32 ? (int)__reduce_or_sync(0xffffffffu, (unsigned)v) : steps(v, OpOr()); }
+    __device__ float reduce(float v, OpMax) const {  // a NaN is dropped
+        if (G < 32) return steps(v, OpMax());
+        float r;
+        asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+        return r;
+    }
+    __device__ float reduce(float v, OpMin) const { return -reduce(-v, OpMax()); }
     // a sum of masses, below 2^62
     __device__ u64 sum(u64 v) const {
         if (G < 32) return reduce(v, OpSum());

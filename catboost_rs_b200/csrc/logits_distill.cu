@@ -17,7 +17,7 @@ namespace {
 // With e_i = exp((a_i - m) / T), s their sum, s_t the sum outside S, r_j the
 // teacher's exponentials and R their sum, the loss is
 //   w T^2 [ (sum r_j (z_j - z_max - a_j + m) / T + r_t (tail - z_max / T - ln s_t)) / R - ln R + ln s ]:
-// no difference of logarithms of rounded sums but ln s - ln R, both taken in 64 bits.
+// no difference of logarithms of rounded sums but ln (s / R), taken in 64 bits.
 
 template <typename C>
 struct RowOut {  // what turns a row's logits into its loss and derivative
@@ -35,12 +35,12 @@ __device__ __forceinline__ RowOut<C> distill_finish(double w, double t, double s
     if (o.zero) return o;
     double kl = cross;
     if (r_tail > 0.0 || r_tail != r_tail) kl += r_tail * (tail_rel - log(s_rest));
-    o.loss = w * t * t * (kl / r_sum - log(r_sum) + log(s));
-    const double wt = w * t;
-    o.q_scale = (C)(wt / r_sum);
-    o.c_top = (C)(wt / s);
-    const double q = r_tail / r_sum;
-    o.c_rest = (C)(wt * (1.0 / s - (q != 0.0 && s_rest != 0.0 ? q / s_rest : (q != q ? q : 0.0))));
+    const double per_r = 1.0 / r_sum, per_s = 1.0 / s, wt = w * t;
+    o.loss = wt * t * (kl * per_r + log(s * per_r));
+    o.q_scale = (C)(wt * per_r);
+    o.c_top = (C)(wt * per_s);
+    const double q = r_tail * per_r;
+    o.c_rest = (C)(wt * (per_s - (q != 0.0 && s_rest != 0.0 ? q / s_rest : (q != q ? q : 0.0))));
     return o;
 }
 
@@ -68,7 +68,7 @@ __device__ __forceinline__ double plain_nan(double v) {
 // Narrow rows: the student's exponentials stay in registers; tgt[i] = the
 // teacher's logit of class i, or absent, and then its exponential.
 template <typename T, int G, int ITEMS>
-__global__ void __launch_bounds__(kLgThreads)
+__global__ void __launch_bounds__(kLgThreads, 4)
 lg_distill_narrow_kernel(Rows<T> x, TeacherArgs tc, const typename Num<T>::C* __restrict__ tail,
                          const typename Num<T>::C* __restrict__ weight, double temp, Scale<typename Num<T>::C> sc,
                          int tile, int direct, typename Num<T>::C* __restrict__ loss, T* der1, int64_t drs,
@@ -103,8 +103,9 @@ lg_distill_narrow_kernel(Rows<T> x, TeacherArgs tc, const typename Num<T>::C* __
         const double tl = tail ? (double)tail[r0 + r] : -lg_inf(0.0);
         for (int i = t.rank; i < V; i += G) set_absent(&tgt[i]);
         t.sync();
-        u64 claimed = 0;  // which of this lane's entries count
+        u64 claimed = 0;  // which of this lane's entries count, a bit each
         static_assert(G == 1 || kLgMaxTop / G <= 64, "a bit an entry");
+        const bool by_entry = G > 1 || 2 * tc.k <= V;  // (V <= 16 of them for a thread)
         for (int j0 = 0; j0 < tc.k; j0 += G) {
             const int j = j0 + t.rank;
             const int64_t at = (r0 + r) * tc.k + j;
@@ -116,7 +117,7 @@ lg_distill_narrow_kernel(Rows<T> x, TeacherArgs tc, const typename Num<T>::C* __
             }
             if (take && is_absent(tgt[idx])) {
                 tgt[idx] = plain_nan((C)load_any(tc.value, tc.value_dtype, at));
-                claimed |= 1ull << (G > 1 ? j0 / G : 0);
+                claimed |= 1ull << (by_entry ? j0 / G : 0);
             }
             t.sync();
         }
@@ -133,11 +134,11 @@ lg_distill_narrow_kernel(Rows<T> x, TeacherArgs tc, const typename Num<T>::C* __
         const double z_max = floor_max(fmax((double)zm * sc.inv_t, tl));
         C sum_top = 0, sum_rest = 0;
         double r_sum = 0.0, cross = 0.0;
-        if (G > 1) {  // a lane an entry: fewer steps in 64 bits than by class
+        if (by_entry) {  // a lane an entry: fewer steps in 64 bits than by class (for which a warp's rows differ)
             for (int j0 = 0; j0 < tc.k; j0 += G) {
                 if (!((claimed >> (j0 / G)) & 1)) continue;
                 const int i = (int)tc.idx((r0 + r) * tc.k + j0 + t.rank);
-                const C ai = to_c(row[i]);
+                const C ai = to_c(direct ? g[r * x.row_stride + (int64_t)i * x.class_stride] : row[i]);
                 const double d = (double)tgt[i] * sc.inv_t - z_max;
                 const C rj = row_exp((C)d, table);
                 r_sum += (double)rj;
@@ -150,7 +151,7 @@ lg_distill_narrow_kernel(Rows<T> x, TeacherArgs tc, const typename Num<T>::C* __
             const C e = row_exp(a[it] - m, sc, table);
             if ((top >> it) & 1) {
                 sum_top += e;
-                if (G > 1) {
+                if (by_entry) {
                     a[it] = e;
                     continue;
                 }

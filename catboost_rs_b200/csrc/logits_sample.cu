@@ -184,6 +184,35 @@ __device__ int sample_row(const LaneTeam<G>& t, const Items<G, ITEMS>& mine, con
             for (int it = 0; it < ITEMS; ++it)
                 if (before[it] >= goal) stay &= ~(1u << it);
         }
+    } else if (rs.top_k <= 8 && rs.top_k < V) {
+        // a few: one by one in order, as many as top-k asks for, then until top-p's mass is there
+        uint32_t from = stay, got = 0;
+        auto next = [&](u64& its) {
+            C best = -lg_inf(C());
+            LG_EACH(it) if ((from >> it) & 1) best = OpMax()(best, a[it]);
+            const C top = t.reduce(best, OpMax());
+            int at = ITEMS;
+            its = 0;
+#pragma unroll
+            for (int it = ITEMS - 1; it >= 0; --it)
+                if (((from >> it) & 1) && a[it] == top) at = it, its = w[it];
+            const int i = at < ITEMS ? mine.first + at : 0x7fffffff, first = t.reduce(i, OpMin());
+            if (i == first && at < ITEMS) from &= ~(1u << at), got |= 1u << at;
+            its = i == first && at < ITEMS ? its : 0;
+        };
+        u64 its;
+        for (int j = 0; j < rs.top_k; ++j) next(its);
+        stay = got;
+        if (rs.top_p < 1.0) {
+            const u64 goal = mass_part(rs.top_p, t.sum(sum_of(stay)));
+            from = stay, got = 0;
+            u64 before = 0;
+            for (int j = 0; j < rs.top_k && before < goal; ++j) {
+                next(its);
+                before += t.sum(its);
+            }
+            stay = got;
+        }
     } else {
         if (rs.top_k < V) cut((u64)rs.top_k, std::false_type());
         if (rs.top_p < 1.0) cut(mass_part(rs.top_p, t.sum(sum_of(stay))), std::true_type());
@@ -202,7 +231,7 @@ __device__ int sample_row(const LaneTeam<G>& t, const Items<G, ITEMS>& mine, con
 }
 
 template <typename T, int G, int ITEMS>
-__global__ void __launch_bounds__(kLgThreads)
+__global__ void __launch_bounds__(kLgThreads, sizeof(T) == 8 ? 3 : 4)
 lg_sample_narrow_kernel(Rows<T> x, SampleArgs a, int shift, int tile, int direct, int32_t* __restrict__ index) {
     typedef typename Num<T>::C C;
     extern __shared__ __align__(16) unsigned char lg_smem[];
