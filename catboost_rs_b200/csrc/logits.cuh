@@ -429,35 +429,35 @@ struct WideRow {
     }
     // Copies this block's part to s; see(vector) is called for each vector on
     // the way.  kAhead loads a thread are under way at a time.
-    template <typename See>
+    template <int NT = kLgThreads, typename See>
     __device__ void load(uint4* s, See see) const {
         constexpr int kAhead = 8;
         const int lo = whole_lo(), hi = whole_hi();
         const uint4* g = reinterpret_cast<const uint4*>(row + ((int64_t)v0 * VE - head));
         int v = lo + threadIdx.x;
-        for (; v + (kAhead - 1) * kLgThreads < hi; v += kAhead * kLgThreads) {
+        for (; v + (kAhead - 1) * NT < hi; v += kAhead * NT) {
             uint4 q[kAhead];
 #pragma unroll
-            for (int u = 0; u < kAhead; ++u) q[u] = __ldcs(g + v + u * kLgThreads);
+            for (int u = 0; u < kAhead; ++u) q[u] = __ldcs(g + v + u * NT);
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
                 see(q[u]);
-                s[v + u * kLgThreads] = q[u];
+                s[v + u * NT] = q[u];
             }
         }
         {
             uint4 q[kAhead];
 #pragma unroll
             for (int u = 0; u < kAhead; ++u)
-                if (v + u * kLgThreads < hi) q[u] = __ldcs(g + v + u * kLgThreads);
+                if (v + u * NT < hi) q[u] = __ldcs(g + v + u * NT);
 #pragma unroll
             for (int u = 0; u < kAhead; ++u)
-                if (v + u * kLgThreads < hi) {
+                if (v + u * NT < hi) {
                     see(q[u]);
-                    s[v + u * kLgThreads] = q[u];
+                    s[v + u * NT] = q[u];
                 }
         }
-        ends([&](int e) {
+        ends<NT>([&](int e) {
             const uint4 q = edge(first(e));
             see(q);
             s[e] = q;
@@ -471,11 +471,11 @@ struct WideRow {
         asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(g), "r"((hi - lo) * 16) : "memory");
     }
     // fn(v) for the vectors outside [whole_lo, whole_hi)
-    template <typename Fn>
+    template <int NT = kLgThreads, typename Fn>
     __device__ void ends(Fn fn) const {
         const int lo = whole_lo(), hi = whole_hi();
         if (cs != 1) {
-            for (int v = threadIdx.x; v < nv; v += kLgThreads) fn(v);
+            for (int v = threadIdx.x; v < nv; v += NT) fn(v);
             return;
         }
         if (threadIdx.x == 0 && lo == 1 && nv > 0) fn(0);
@@ -1194,7 +1194,8 @@ Wide wide_shape(int64_t n, int V) {
 
 // Launches `kernel` with clusters of w.blocks, w.blocks blocks a row, as many rows at a time as a grid holds.
 template <typename K, typename... A>
-int lg_launch_wide(const char* who, K kernel, int64_t n, const Wide& w, size_t smem, cudaStream_t st, A... args) {
+int lg_launch_wide_n(const char* who, K kernel, int64_t n, const Wide& w, int threads, size_t smem, cudaStream_t st,
+                     A... args) {
     cudaError_t e = cudaSuccess;
     if (smem > 32 * 1024)  // with the kernels' static arrays (less than 16 KB) above the 48 KB that need no asking
         e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kLgSmemMost);
@@ -1205,7 +1206,7 @@ int lg_launch_wide(const char* who, K kernel, int64_t n, const Wide& w, size_t s
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = (unsigned)w.blocks;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cfg.blockDim = dim3(kLgThreads);
+    cfg.blockDim = dim3((unsigned)threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cfg.attrs = at;
@@ -1220,6 +1221,10 @@ int lg_launch_wide(const char* who, K kernel, int64_t n, const Wide& w, size_t s
         return lfail(CBGPU_ERR_CUDA, "%s: launch failed: %s", who, cudaGetErrorString(e));
     }
     return CBGPU_OK;
+}
+template <typename K, typename... A>
+int lg_launch_wide(const char* who, K kernel, int64_t n, const Wide& w, size_t smem, cudaStream_t st, A... args) {
+    return lg_launch_wide_n(who, kernel, n, w, kLgThreads, smem, st, args...);
 }
 
 // Rows above kLgFew classes are wide when there are few of them: a block of 256 threads a row

@@ -248,18 +248,18 @@ __device__ double distill_loss(const DistillPart<C>& p, int blocks, double w, do
     return distill_finish<double>(w, t, s_top, s_rest, r_sum + r_tail, r_tail, tl - z_max, cross).loss;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kLgThreads)
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT)
 lg_distill_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, TeacherArgs tc, const typename Num<T>::C* __restrict__ tail,
                        const typename Num<T>::C* __restrict__ weight, double temp, Scale<typename Num<T>::C> sc,
                        typename Num<T>::C* __restrict__ loss, T* der1, int64_t drs, int64_t dcs) {
     typedef typename Num<T>::C C;
-    constexpr int VE = WideRow<T>::VE;
+    constexpr int VE = WideRow<T>::VE, kWarps = NT / 32;
     extern __shared__ __align__(16) unsigned char lg_smem[];
-    __shared__ __align__(16) C red_max[2][kLgWarps];
+    __shared__ __align__(16) C red_max[2][kWarps];
     __shared__ union {
         int claim[kClaims];
-        double red[4][kLgThreads];  // s_rest, s_top, r_sum, cross of every thread
+        double red[4][NT];  // s_rest, s_top, r_sum, cross of every thread
     } u;
     __shared__ int s_idx[kLgMaxTop];
     __shared__ DistillPart<C> parts[16];
@@ -282,7 +282,6 @@ lg_distill_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, TeacherA
     };
     if (blocks > 1) cluster_arrive<false>();
 
-    static_assert(kLgThreads >= kLgMaxTop, "one thread an entry");
     // the row's own numbers are asked for before its logits and used after them
     const C wt = weight ? weight[r] : C(1), tl = tail ? tail[r] : -lg_inf(C());
     u64 i_bits = 0, z_bits = 0;
@@ -291,18 +290,18 @@ lg_distill_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, TeacherA
         z_bits = load_bits(tc.value, tc.value_dtype, r * k + tid);
     }
     if (r + ahead < x.n) {
-        if (tid == kLgThreads - 1) WideRow<T>(x, r + ahead, rank, per).prefetch();
+        if (tid == NT - 1) WideRow<T>(x, r + ahead, rank, per).prefetch();
         if (tid < k && (tid & 15) == 0) tc.prefetch((r + ahead) * k + tid);
     }
-    for (int i = tid; i < kClaims; i += kLgThreads) u.claim[i] = kLgMaxTop;
+    for (int i = tid; i < kClaims; i += NT) u.claim[i] = kLgMaxTop;
     if (tid == 0) s_next = 0;
     VecMax<T> most;
-    w.load(s, [&](const uint4& q) { most(q); });
+    w.template load<NT>(s, [&](const uint4& q) { most(q); });
     if (wt == C(0)) {  // the same for all blocks of the cluster
         if (tid == 0 && rank == 0) loss[r] = 0;
         const C zero[VE] = {};
         if (out)
-            for (int v = tid; v < w.nv; v += kLgThreads) put(v, zero);
+            for (int v = tid; v < w.nv; v += NT) put(v, zero);
         if (blocks > 1) cluster_wait();
         return;
     }
@@ -340,7 +339,7 @@ lg_distill_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, TeacherA
     __syncthreads();
     C top[2] = {red_max[0][0], red_max[1][0]};
 #pragma unroll
-    for (int i = 1; i < kLgWarps; ++i) {
+    for (int i = 1; i < kWarps; ++i) {
         top[0] = OpMax()(top[0], red_max[0][i]);
         top[1] = OpMax()(top[1], red_max[1][i]);
     }
@@ -350,7 +349,7 @@ lg_distill_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, TeacherA
     double sum[4] = {0.0, 0.0, 0.0, 0.0};  // s_rest, s_top, r_sum, cross
     auto add = [&](auto huge) {
 #pragma unroll 4
-        for (int v = tid; v < w.nv; v += kLgThreads) {
+        for (int v = tid; v < w.nv; v += NT) {
             C a[VE];
             unpack(s[v], a, T());
             here.template exps<decltype(huge)::value>(a);
@@ -373,7 +372,7 @@ lg_distill_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, TeacherA
     if (warp_id < 4) {
         double v = 0.0;
 #pragma unroll
-        for (int i = 0; i < kLgWarps; ++i) v += u.red[warp_id][lane + 32 * i];
+        for (int i = 0; i < kWarps; ++i) v += u.red[warp_id][lane + 32 * i];
         v = warp_sum(v, 32);
         if (lane < blocks) {
             DistillPart<C>* to = cluster.map_shared_rank(&parts[rank], lane);
@@ -399,7 +398,7 @@ lg_distill_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, TeacherA
         }
         __syncthreads();
     }
-    if (warp_id == kLgWarps - 1 && rank == 0) {  // and another the loss, while the others are at the second pass
+    if (warp_id == kWarps - 1 && rank == 0) {  // and another the loss, while the others are at the second pass
         const double v = distill_loss<C>(p, blocks, (double)wt, temp, (double)tl, sc);
         if (lane == 0) loss[r] = (C)v;
     }
@@ -437,13 +436,13 @@ lg_distill_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, TeacherA
                     }
                 }
             }
-            w.ends([&](int v) {
+            w.template ends<NT>([&](int v) {
                 C a[VE];
                 der(v, a);
                 put(v, a);
             });
         } else {
-            for (int v = tid; v < w.nv; v += kLgThreads) {
+            for (int v = tid; v < w.nv; v += NT) {
                 C a[VE];
                 der(v, a);
                 put(v, a);
@@ -466,9 +465,14 @@ int run_distill(const cbgpu_logits* x, const cbgpu_teacher* tc, const void* weig
     const Scale<C> sc(temp);
     const TeacherArgs ta{tc->index, tc->value, tc->index_bytes, tc->value_dtype, tc->k};
     if (is_wide(rows.n, rows.V)) {
-        const Wide w = wide_shape<T>(rows.n, rows.V);
-        return lg_launch_wide(who, lg_distill_wide_kernel<T>, rows.n, w, w.smem, st, w.ahead, rows, ta, (const C*)tc->tail,
-                              (const C*)weight, temp, sc, (C*)loss, (T*)der1, drs, dcs);
+        auto wide = [&](auto kernel, int threads, const Wide& w) {
+            return lg_launch_wide_n(who, kernel, rows.n, w, threads, w.smem, st, w.ahead, rows, ta, (const C*)tc->tail,
+                                    (const C*)weight, temp, sc, (C*)loss, (T*)der1, drs, dcs);
+        };
+        // a thread an entry; small rows by small blocks (20000 x 1000 f32: 119 us against 192)
+        if (tc->k <= 128 && (size_t)rows.V * sizeof(T) <= 16384)
+            return wide(lg_distill_wide_kernel<T, 128>, 128, wide_shape<T>(rows.n, rows.V));
+        return wide(lg_distill_wide_kernel<T, 256>, 256, wide_shape<T>(rows.n, rows.V));
     }
     auto narrow = [&](auto kernel, int lanes) {
         const bool direct = lanes == 1 && rows.class_stride > rows.row_stride && (!der1 || dcs > drs);
