@@ -378,14 +378,6 @@ struct Ranked {  // a class in the operators' order
         return key > o.key || (key == o.key && idx < o.idx);
     }
 };
-template <typename Team, typename Key>
-__device__ __forceinline__ Ranked<Key> team_first(const Team& t, Ranked<Key> v) {
-    Ranked<Key> r;
-    r.key = t.reduce(v.key, OpMax());
-    r.idx = t.reduce(v.key == r.key ? v.idx : 0xffffffffu, OpMin());
-    return r;
-}
-
 // ---- wide rows: a cluster of blocks holds a row in its shared memory --------------------------
 //
 // The row is cut into 16-byte vectors from the 16-byte boundary at or below
@@ -784,7 +776,7 @@ struct TopShared {
     uint32_t bound[16][2];  // of every block: its k-th and its ceil(k / blocks)-th largest thread maximum
     uint32_t flag[16];
     int base, vectors;
-    uint16_t hit[kHits];    // vectors that hold a class to collect
+    uint16_t hit[kHits];    // places of the classes that the sampler collected from this block
     u64 part[2][16][kGather];  // values that go round the cluster
     u64 warp_part[kGather][kLgWarps];
     int count;
@@ -1006,7 +998,7 @@ __device__ int wide_top(const ClusterInfo& cl, TopShared<typename Num<T>::Key>& 
     const int tid = threadIdx.x;
     const int share = (k + cl.blocks - 1) / cl.blocks;
     sh.idx[tid] = (uint32_t)(key_of(mine) >> kDrop);
-    if (tid == 0) sh.count = 0, sh.vectors = 0;
+    if (tid == 0) sh.count = 0;
     flag = __syncthreads_or(flag) != 0;
     if (tid < 64) {
         const uint32_t b = warp_bound(sh.idx, tid < 32 ? k : share);
@@ -1046,8 +1038,26 @@ __device__ int wide_top(const ClusterInfo& cl, TopShared<typename Num<T>::Key>& 
     constexpr int VE = WideRow<T>::VE;
     rest = -lg_inf(C());
     exact = false;
-    // vectors that hold one are noted, so that a warp does not go through their classes for each of them
-    auto open = [&](int v) {
+    // a thread's vectors that hold one are noted and gone through at the end, not one by one with the
+    // warp waiting; each thread its own, so that its sums are in the same order always
+    uint64_t hits = 0;
+    int round = 0;
+#pragma unroll 2
+    for (int v = tid; v < w.nv; v += kLgThreads, ++round) {
+        const uint4 q = s[v];
+        VecMax<T> m;
+        m(q);
+        if (m.get() < least) {
+            rest = OpMax()(rest, m.get());
+            C a[VE];
+            unpack(q, a, T());
+            see(a, least);
+        } else {
+            hits |= 1ull << round;  // at most 33 rounds (8193 vectors)
+        }
+    }
+    for (; hits; hits &= hits - 1) {
+        const int v = tid + (__ffsll((long long)hits) - 1) * kLgThreads;
         C a[VE];
         unpack(s[v], a, T());
         const int i = w.first(v);
@@ -1061,25 +1071,7 @@ __device__ int wide_top(const ClusterInfo& cl, TopShared<typename Num<T>::Key>& 
             }
         }
         see(a, least);
-    };
-#pragma unroll 2
-    for (int v = tid; v < w.nv; v += kLgThreads) {
-        const uint4 q = s[v];
-        VecMax<T> m;
-        m(q);
-        if (m.get() < least) {
-            rest = OpMax()(rest, m.get());
-            C a[VE];
-            unpack(q, a, T());
-            see(a, least);
-        } else {
-            const int p = atomicAdd(&sh.vectors, 1);
-            if (p < kHits) sh.hit[p] = (uint16_t)v;
-            else open(v);
-        }
     }
-    __syncthreads();
-    for (int p = tid; p < sh.vectors && p < kHits; p += kLgThreads) open(sh.hit[p]);
     hand_over();
     const int n = cl.of(&sh, 0)->count;
     if (n >= k && n <= kTopCap) return n;
@@ -1117,6 +1109,12 @@ int check_logits(const char* who, const cbgpu_logits* x) {
     if (x->n > 0 && !x->data) return lfail(CBGPU_ERR_INVALID, "%s: logits.data is NULL", who);
     if ((uintptr_t)x->data % dtype_size(x->dtype) != 0)
         return lfail(CBGPU_ERR_INVALID, "%s: logits.data is not aligned to its type", who);
+    return CBGPU_OK;
+}
+
+// An array that a kernel reads or writes by elements of `size` bytes.
+int check_aligned(const char* who, const char* name, const void* p, size_t size) {
+    if ((uintptr_t)p % size != 0) return lfail(CBGPU_ERR_INVALID, "%s: %s is not aligned to its type", who, name);
     return CBGPU_OK;
 }
 

@@ -18,6 +18,9 @@ namespace {
 // teacher's exponentials and R their sum, the loss is
 //   w T^2 [ (sum r_j (z_j - z_max - a_j + m) / T + r_t (tail - z_max / T - ln s_t)) / R - ln R + ln s ]:
 // no difference of logarithms of rounded sums but ln (s / R), taken in 64 bits.
+// Where the others lie far below m (s_t < kFar), their exponentials and s_t are taken relative to the
+// largest of the others instead: Q ln s_t and Q / s_t need s_t by itself, not beside s.
+constexpr double kFar = 1e-20;
 
 template <typename C>
 struct RowOut {  // what turns a row's logits into its loss and derivative
@@ -28,19 +31,19 @@ struct RowOut {  // what turns a row's logits into its loss and derivative
 
 template <typename C>
 __device__ __forceinline__ RowOut<C> distill_finish(double w, double t, double s_top, double s_rest, double r_sum,
-                                                    double r_tail, double tail_rel, double cross) {
+                                                    double r_tail, double tail_rel, double cross, double rest_ln) {  // rest_ln: logarithm of s_rest's unit
     RowOut<C> o{};
-    const double s = s_top + s_rest;
+    const double unit = rest_ln == 0.0 ? 1.0 : exp(rest_ln), s = s_top + s_rest * unit;
     o.zero = s == 0.0 || r_sum == 0.0;  // every class masked (m is 0 then), or a teacher without an entry
     if (o.zero) return o;
     double kl = cross;
-    if (r_tail > 0.0 || r_tail != r_tail) kl += r_tail * (tail_rel - log(s_rest));
+    if (r_tail > 0.0 || r_tail != r_tail) kl += r_tail * (tail_rel - log(s_rest) - rest_ln);
     const double per_r = 1.0 / r_sum, per_s = 1.0 / s, wt = w * t;
     o.loss = wt * t * (kl * per_r + log(s * per_r));
     o.q_scale = (C)(wt * per_r);
     o.c_top = (C)(wt * per_s);
     const double q = r_tail * per_r;
-    o.c_rest = (C)(wt * (per_s - (q != 0.0 && s_rest != 0.0 ? q / s_rest : (q != q ? q : 0.0))));
+    o.c_rest = (C)(wt * (per_s * unit - (q != 0.0 && s_rest != 0.0 ? q / s_rest : (q != q ? q : 0.0))));
     return o;
 }
 
@@ -165,11 +168,27 @@ lg_distill_narrow_kernel(Rows<T> x, TeacherArgs tc, const typename Num<T>::C* __
             }
             a[it] = e;
         }
-        const double s_top = t.reduce((double)sum_top, OpSum()), s_rest = t.reduce((double)sum_rest, OpSum());
+        const double s_top = t.reduce((double)sum_top, OpSum());
+        double s_rest = t.reduce((double)sum_rest, OpSum()), rest_ln = 0.0;
         r_sum = t.reduce(r_sum, OpSum());
         cross = t.reduce(cross, OpSum());
         const double r_tail = (double)row_exp((C)(tl - z_max), table);
-        RowOut<C> o = distill_finish<C>(w, temp, s_top, s_rest, r_sum + r_tail, r_tail, tl - z_max, cross);
+        if (s_rest < kFar && r_tail > 0.0) {  // the same for a row's lanes
+            auto logit = [&](int i) { return to_c(direct ? g[r * x.row_stride + (int64_t)i * x.class_stride] : row[i]); };
+            C mr = -lg_inf(C());
+            LG_EACH(it) if (mine.has(it) && !((top >> it) & 1)) mr = OpMax()(mr, logit(mine.first + it));
+            mr = t.reduce(mr, OpMax());
+            if (mr != -lg_inf(C())) {
+                C sum = 0;
+                LG_EACH(it) if (mine.has(it) && !((top >> it) & 1)) {
+                    a[it] = row_exp(logit(mine.first + it) - mr, sc, table);
+                    sum += a[it];
+                }
+                s_rest = t.reduce((double)sum, OpSum());
+                rest_ln = ((double)mr - (double)m) * sc.inv_t;
+            }
+        }
+        RowOut<C> o = distill_finish<C>(w, temp, s_top, s_rest, r_sum + r_tail, r_tail, tl - z_max, cross, rest_ln);
         if (w == 0.0) {
             o = RowOut<C>{};
             o.zero = true;
@@ -202,14 +221,16 @@ lg_distill_narrow_kernel(Rows<T> x, TeacherArgs tc, const typename Num<T>::C* __
 template <typename C>
 struct DistillPart {  // sums relative to the block's own maxima: m of its logits, z of its entries' z / T
     double s_rest, s_top, r_sum, cross;
-    C m, z;
+    C m, z, m_rest;  // m_rest: what s_rest is relative to, m or (far below it) the largest of the others
+    __device__ C rest() const { return s_rest == 0.0 ? -lg_inf(C()) : m_rest; }
 };
 
 constexpr int kClaims = 1024;  // places where entries claim their index
 
 template <typename C>
 struct DistillJoin {  // for the second pass, from the joined parts
-    C base, c_rest, q_scale, c_top;  // an entry: der1 = q_scale * r - c_top * e, both relative to this block's maxima
+    C base, c_rest;     // the others: der1 = -c_rest * e, relative to base
+    C q_scale, c_top;   // an entry: der1 = q_scale * r - c_top * e, both relative to this block's maxima
     bool zero;
 };
 
@@ -218,16 +239,19 @@ template <typename C>
 __device__ DistillJoin<C> distill_join(const DistillPart<C>& p, int rank, int blocks, C w, C tl, const Scale<C>& sc) {
     const Base<C> base(floor_max(warp_max(p.m)), sc);
     const C z_max = floor_max(OpMax()(warp_max(p.z), tl));
-    const C f = Base<C>(floor_max(p.m), sc).shift(base);
+    const C rest_max = warp_max(p.rest());
+    const Base<C> rest(floor_max(rest_max), sc);
+    const C f = Base<C>(floor_max(p.m), sc).shift(base), h = Base<C>(floor_max(p.m_rest), sc).shift(rest);
+    const C unit = rest_max == -lg_inf(C()) ? C(0) : rest.shift(base);
     const C g = part_exp(floor_max(p.z) - z_max), r_tail = part_exp(tl - z_max);
-    const C s_rest = warp_sum(p.s_rest == 0.0 ? C(0) : (C)p.s_rest * f, blocks);
-    const C s = s_rest + warp_sum(p.s_top == 0.0 ? C(0) : (C)p.s_top * f, blocks);
+    const C s_rest = warp_sum(p.s_rest == 0.0 ? C(0) : (C)p.s_rest * h, blocks);
+    const C s = s_rest * unit + warp_sum(p.s_top == 0.0 ? C(0) : (C)p.s_top * f, blocks);
     const C r_sum = r_tail + warp_sum(p.r_sum == 0.0 ? C(0) : (C)p.r_sum * g, blocks);
     const C q = r_tail / r_sum, per_s = C(1) / s;
     DistillJoin<C> j;
-    j.base = base.m;
+    j.base = rest.m;
     j.zero = s == C(0) || r_sum == C(0);  // every class masked, or a teacher without an entry
-    j.c_rest = w * (q != q ? q : (q != C(0) && s_rest != C(0) ? per_s - q / s_rest : per_s));
+    j.c_rest = w * (q != q ? q : (q != C(0) && s_rest != C(0) ? per_s * unit - q / s_rest : per_s * unit));
     j.q_scale = __shfl_sync(0xffffffffu, w / r_sum * g, rank);
     j.c_top = __shfl_sync(0xffffffffu, w * per_s * f, rank);
     return j;
@@ -240,12 +264,16 @@ __device__ double distill_loss(const DistillPart<C>& p, int blocks, double w, do
     const double z_max = floor_max(fmax((double)warp_max(p.z), tl));
     const double ln_f = Base<C>(floor_max(p.m), sc).ln_shift(base), f = exp(ln_f);
     const double ln_g = (double)floor_max(p.z) - z_max, g = exp(ln_g);
-    const double s_rest = warp_sum(p.s_rest == 0.0 ? 0.0 : p.s_rest * f, blocks);
+    const C rest_max = warp_max(p.rest());
+    const Base<C> rest(floor_max(rest_max), sc);
+    const double s_rest =
+        warp_sum(p.s_rest == 0.0 ? 0.0 : p.s_rest * exp(Base<C>(floor_max(p.m_rest), sc).ln_shift(rest)), blocks);
+    const double rest_ln = rest_max == -lg_inf(C()) ? 0.0 : rest.ln_shift(base);
     const double s_top = warp_sum(p.s_top == 0.0 ? 0.0 : p.s_top * f, blocks);
     const double r_sum = warp_sum(p.r_sum == 0.0 ? 0.0 : p.r_sum * g, blocks);
     const double cross = warp_sum(p.r_sum == 0.0 ? 0.0 : g * (p.cross + p.r_sum * (ln_g - ln_f)), blocks);
     const double r_tail = exp(tl - z_max);
-    return distill_finish<double>(w, t, s_top, s_rest, r_sum + r_tail, r_tail, tl - z_max, cross).loss;
+    return distill_finish<double>(w, t, s_top, s_rest, r_sum + r_tail, r_tail, tl - z_max, cross, rest_ln).loss;
 }
 
 template <typename T, int NT>
@@ -366,7 +394,28 @@ lg_distill_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, TeacherA
     const double e_own = sum[1], r_own = sum[2];
 #pragma unroll
     for (int i = 0; i < 4; ++i) u.red[i][tid] = sum[i];
-    __syncthreads();
+    C m_rest = top[0];
+    if (!__syncthreads_or(!(sum[0] < kFar)) && tl > -lg_inf(C())) {  // the block's others lie far below
+        most = VecMax<T>();
+        for (int v = tid; v < w.nv; v += NT) most(s[v]);
+        const C m = warp_max(most.get());
+        if (lane == 0) red_max[0][warp_id] = m;
+        __syncthreads();
+        m_rest = red_max[0][0];
+#pragma unroll
+        for (int i = 1; i < kWarps; ++i) m_rest = OpMax()(m_rest, red_max[0][i]);
+        const Base<C> rest(floor_max(m_rest), sc);
+        double own = 0.0;
+        for (int v = tid; v < w.nv; v += NT) {
+            C a[VE];
+            unpack(s[v], a, T());
+            if (rest.huge) rest.template exps<true>(a);
+            else rest.template exps<false>(a);
+            own += Base<C>::total(a);
+        }
+        u.red[0][tid] = own;
+        __syncthreads();
+    }
     // a warp for each of the four sums, which it gives to all blocks of the cluster
     if (blocks > 1) cluster_wait();  // every block runs: its shared memory can be written
     if (warp_id < 4) {
@@ -376,7 +425,7 @@ lg_distill_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, TeacherA
         v = warp_sum(v, 32);
         if (lane < blocks) {
             DistillPart<C>* to = cluster.map_shared_rank(&parts[rank], lane);
-            if (warp_id == 0) to->s_rest = v, to->m = top[0], to->z = top[1];
+            if (warp_id == 0) to->s_rest = v, to->m = top[0], to->z = top[1], to->m_rest = m_rest;
             else if (warp_id == 1) to->s_top = v;
             else if (warp_id == 2) to->r_sum = v;
             else to->cross = v;
@@ -389,7 +438,7 @@ lg_distill_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, TeacherA
     } else {
         __syncthreads();
     }
-    DistillPart<C> p{0.0, 0.0, 0.0, 0.0, -lg_inf(C()), -lg_inf(C())};
+    DistillPart<C> p{0.0, 0.0, 0.0, 0.0, -lg_inf(C()), -lg_inf(C()), -lg_inf(C())};
     if (lane < blocks) p = parts[lane];
     if (out) {  // one warp works out what the second pass needs
         if (warp_id == 0) {
@@ -505,13 +554,19 @@ int cbgpu_distill(const cbgpu_logits* x, const cbgpu_teacher* t, const void* wei
     if ((rc = check_temperature("distill", temperature, false))) return rc;
     if (x->n == 0) return CBGPU_OK;
     if (!t->index || !t->value || !loss) return lfail(CBGPU_ERR_INVALID, "distill: index, value or loss is NULL");
+    const size_t wide = x->dtype == CBGPU_F64 ? 8 : 4;
+    if ((rc = check_aligned("distill", "index", t->index, (size_t)t->index_bytes)) ||
+        (rc = check_aligned("distill", "value", t->value, dtype_size(t->value_dtype))) ||
+        (rc = check_aligned("distill", "tail", t->tail, wide)) ||
+        (rc = check_aligned("distill", "weight", weight, wide)) || (rc = check_aligned("distill", "loss", loss, wide)))
+        return rc;
     if (der1) {
         const int64_t n = x->n, V = x->n_classes, rs = der1_row_stride, cs = der1_class_stride;
         if (rs < 0 || cs < 0) return lfail(CBGPU_ERR_INVALID, "distill: negative strides");
         const bool apart = (n == 1 && V == 1) || (n == 1 && cs >= 1) || (V == 1 && rs >= 1) ||
                            (cs >= 1 && rs > cs * (V - 1)) || (rs >= 1 && cs > rs * (n - 1));
         if (!apart) return lfail(CBGPU_ERR_INVALID, "distill: elements of der1 share memory");
-        const size_t es = dtype_size(x->dtype), wide = x->dtype == CBGPU_F64 ? 8 : 4;
+        const size_t es = dtype_size(x->dtype);
         if ((uintptr_t)der1 % es != 0) return lfail(CBGPU_ERR_INVALID, "distill: der1 is not aligned to its type");
         const Span d = span_of(der1, es, n, (int)V, rs, cs);
         const bool same = der1 == x->data && (n == 1 || rs == x->row_stride) && (V == 1 || cs == x->class_stride);

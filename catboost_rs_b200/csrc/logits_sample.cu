@@ -802,5 +802,12 @@ int cbgpu_sample_classes(const cbgpu_logits* x, const cbgpu_sampling* s, int32_t
         return lfail(CBGPU_ERR_INVALID, "sample_classes: min_p %g is outside 0..1", s->min_p);
     if (x->n == 0) return CBGPU_OK;
     if (!s->uniform || !index) return lfail(CBGPU_ERR_INVALID, "sample_classes: uniform or index is NULL");
+    if ((rc = check_aligned("sample_classes", "uniform", s->uniform, dtype_size(s->uniform_dtype))) ||
+        (rc = check_aligned("sample_classes", "index", index, 4)) ||
+        (rc = check_aligned("sample_classes", "temperature_rows", s->temperature_rows, 4)) ||
+        (rc = check_aligned("sample_classes", "top_p_rows", s->top_p_rows, 4)) ||
+        (rc = check_aligned("sample_classes", "min_p_rows", s->min_p_rows, 4)) ||
+        (rc = check_aligned("sample_classes", "top_k_rows", s->top_k_rows, 4)))
+        return rc;
     return LG_BY_DTYPE(x->dtype, run_sample, x, s, index, (cudaStream_t)stream);
 }

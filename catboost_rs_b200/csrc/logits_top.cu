@@ -363,6 +363,10 @@ int cbgpu_top_logits(const cbgpu_logits* x, int32_t k, double temperature, void*
                      x->n_classes);
     if ((rc = check_temperature("top_logits", temperature, false))) return rc;
     if (x->n > 0 && (!value || !index)) return lfail(CBGPU_ERR_INVALID, "top_logits: value or index is NULL");
+    const size_t wide = x->dtype == CBGPU_F64 ? 8 : 4;
+    if ((rc = check_aligned("top_logits", "value", value, dtype_size(x->dtype))) ||
+        (rc = check_aligned("top_logits", "index", index, 4)) || (rc = check_aligned("top_logits", "tail", tail, wide)))
+        return rc;
     if (x->n == 0) return CBGPU_OK;
     return LG_BY_DTYPE(x->dtype, run_top, x, k, temperature, value, index, tail, (cudaStream_t)stream);
 }

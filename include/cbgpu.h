@@ -531,9 +531,13 @@ CBGPU_API int cbgpu_apply_oblivious(const float* features_fm, int64_t n, int32_t
  * stream) and the call returns without waiting.  The calls allocate nothing,
  * hold no state and share no workspace, so they may overlap on any streams
  * and be captured into graphs.  Arithmetic and the "wide" outputs are f64 for
- * CBGPU_F64 logits and f32 for the other types; sums are taken in 64 bits.
- * The same call gives the same bits again; rows in another layout may be
- * summed in another grouping (the last bits of loss, der1 and tail).
+ * CBGPU_F64 logits and f32 for the other types, whose terms are added up in
+ * f32 for a few neighbouring classes (16 at most; a row of up to 512 or its
+ * tail: a thread's share) and in 64 bits from there.
+ * The same call gives the same bits again; rows in another layout or in a
+ * batch of another size may be summed in another grouping (the last bits of
+ * loss, der1 and tail).  Outputs may not overlap inputs or each other, but
+ * for der1 below.
  * Classes are ordered by logit, larger first, equal logits (-0 == +0) by
  * lower index, NaN last.  Limits: 1..262144 classes, n < 2^31 rows; n = 0 is
  * a call that does nothing. */
@@ -555,7 +559,8 @@ typedef struct {
  *  value        [n][k] of the logits' dtype;  index [n][k];
  *  tail         [n] wide: ln sum of exp(a_i / temperature) over the classes
  *               not in the row's k; -inf where they are none or all masked
- *               (-inf); NaN where the row holds a NaN; or NULL. */
+ *               (-inf); NaN where the row holds a NaN or the others a +inf; or
+ *               NULL. */
 CBGPU_API int cbgpu_top_logits(const cbgpu_logits* logits, int32_t k, double temperature, void* value,
                                int32_t* index, void* tail, void* stream);
 

@@ -61,7 +61,8 @@ def distill(row, index, value, tail, weight, temperature):
         log_rest = logsumexp(log_p[rest]) if rest.any() else -np.inf
         loss += q[-1] * (log_q[-1] - log_rest)
         if log_rest > -np.inf:
-            target[rest] = q[-1] * np.exp(log_p[rest] - log_rest)
+            # from the logits: log_p of a class 20000 below the others is rounded to 2e-12
+            target[rest] = q[-1] * np.exp(log_softmax(row[rest] / T))
     return weight * T * T * loss, weight * T * (target - p), p, target
 
 

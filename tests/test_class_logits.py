@@ -102,6 +102,19 @@ def test_bad_teacher_is_refused(change, text):
     refused(L.cbgpu_distill(C.byref(x), C.byref(teacher(**change)), None, 1.0, SOME, None, 0, 0, None), text)
 
 
+def test_unaligned_arrays_are_refused():
+    L, x, odd = _lib.load(), logits(), SOME + 4098
+    far = SOME << 4
+    for v, i, t in ((odd, far, None), (far, odd, None), (far, far, odd)):
+        refused(L.cbgpu_top_logits(C.byref(x), 1, 1.0, v, i, t, None), "aligned")
+    for t, w, loss in ((teacher(index=odd), None, far), (teacher(value=odd), None, far), (teacher(tail=odd), None, far),
+                       (teacher(index=far + 4, index_bytes=8), None, far), (teacher(), odd, far), (teacher(), None, odd)):
+        refused(L.cbgpu_distill(C.byref(x), C.byref(t), w, 1.0, loss, None, 0, 0, None), "aligned")
+    for name in ("uniform", "temperature_rows", "top_p_rows", "min_p_rows", "top_k_rows"):
+        refused(L.cbgpu_sample_classes(C.byref(x), C.byref(sampling(**{name: odd})), far, None), "aligned")
+    refused(L.cbgpu_sample_classes(C.byref(x), C.byref(sampling()), odd, None), "aligned")
+
+
 def test_no_rows_is_no_work():
     # needs no device: nothing is launched
     L, x = _lib.load(), logits(n=0, data=None)

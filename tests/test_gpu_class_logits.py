@@ -127,9 +127,84 @@ def test_top_logits_ties_masks_and_nan(V, dtype):
     assert got.tail is None
 
 
+@pytest.mark.parametrize("n", [6, 40000])
+@pytest.mark.parametrize("V", [14, 100, 400, 700, 5000])
+@pytest.mark.parametrize("dtype", ["f64", "f32"])
+def test_tails_far_below_and_infinite(V, dtype, n):
+    # the rest lies 300 (e^-300 is below any f32) to 30000 under the first k; with infinite logits the first
+    # k may be those alone, or leave one to the rest
+    if n > 6 and V > 100:
+        pytest.skip("as with few rows")
+    rs = np.random.RandomState(V)
+    a = rs.standard_normal((6, V))
+    at = rs.permutation(V)[:7]
+    for r, lift in enumerate((300.0, 3000.0, 30000.0, np.inf, -np.inf, 60.0)):
+        a[r, at] += lift if lift > 0 else 0.0
+        if lift < 0:
+            a[r, np.delete(np.arange(V), at)] = -np.inf
+    x = put(np.tile(a, (-(-n // 6), 1))[:n], dtype)
+    same = torch.arange(n, device="cuda") % 6
+    for k in (7, 8):
+        check_top(x[:6].contiguous(), k, 1.0, dtype)
+        few, many = cb.top_logits(x[:6].contiguous(), k), cb.top_logits(x, k)
+        assert torch.equal(many.index, few.index[same]) and torch.equal(many.value, few.value[same])
+        fine, u = torch.isfinite(few.tail), unit(dtype)
+        assert torch.equal(torch.isfinite(many.tail), fine[same])
+        # each within u (3 reach + 4) + 3 u |tail| of the 64-bit value, reach at most 40
+        bound = 2 * u * (124 + 3 * few.tail[fine].abs())
+        assert ((many.tail[:6] - few.tail)[fine].abs() <= bound).all()
+    tail = cb.top_logits(x, 5).tail  # of row 3 two infinite ones are left
+    assert torch.isnan(tail[3]) and not torch.isnan(tail[:3]).any()
+
+
+@pytest.mark.parametrize("V", [9, 300, 6000])
+def test_rows_and_classes_that_share_memory(V):
+    # strides of 0 are allowed for what is read
+    one = make(1, V, "f32", "rows", 3)
+    t, u = make_teacher(1, V, 4, "f32", 5, True), torch.full((50,), 0.4, device="cuda")
+    many = cb.TopLogits(*(v.repeat_interleave(50, 0) for v in (t.index, t.value, t.tail)))
+    x = one.expand(50, V)
+    out = torch.empty((50, V), device="cuda")
+    d = cb.distill_derivatives(x, many, out=out)
+    for got, want in ((d.der1, cb.distill_derivatives(one.repeat(50, 1), many).der1),
+                      (cb.top_logits(x, 3).tail, cb.top_logits(one.repeat(50, 1), 3).tail),
+                      (cb.sample_classes(x, u, top_p=0.8), cb.sample_classes(one.repeat(50, 1), u, top_p=0.8))):
+        assert torch.equal(got, want)
+    same = one[:, :1].expand(50, V)  # every class one number
+    top = cb.top_logits(same, 3)
+    assert (top.index == torch.arange(3, device="cuda")).all() and (top.value == one[0, 0]).all()
+    assert (cb.sample_classes(same, u) == int(np.float32(0.4) * np.float64(V))).all()
+    with pytest.raises(cb.CbGpuError):
+        cb.distill_derivatives(x, many, out=x)
+
+
+def test_calls_that_overlap_on_streams():
+    # nothing is shared between calls: as many at a time as the streams allow
+    sets = [batch(V, dtype, n) for V, dtype, n in
+            ((10, "f64", 4000), (100, "f32", 4000), (1000, "bf16", 900), (40000, "bf16", 60), (131071, "f32", 4))]
+
+    def call(x, t, u):
+        d = cb.distill_derivatives(x, t, temperature=1.5)
+        top = cb.top_logits(x, 7)
+        return d.loss, d.der1, top.value, top.index, top.tail, cb.sample_classes(x, u, top_p=0.9), \
+            cb.sample_classes(x, u, top_k=6)
+
+    want = [call(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = []
+    for turn in range(4):
+        for s, st in zip(sets, streams):
+            with torch.cuda.stream(st):
+                got.append(call(*s))
+    torch.cuda.synchronize()
+    for i, g in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(g, want[i % len(sets)]))
+
+
 # ---- distillation -------------------------------------------------------------------
 
-def check_distill(x, teacher, weight, temperature, dtype, out=None):
+def check_distill(x, teacher, weight, temperature, dtype, out=None, lost=0.0):
     u, V = unit(dtype), x.shape[1]
     a = host(x)
     loss_only = host(cb.distill_loss(x, teacher, weight=weight, temperature=temperature))
@@ -156,7 +231,7 @@ def check_distill(x, teacher, weight, temperature, dtype, out=None):
         if np.isnan(wd).any():
             assert np.isnan(der1[r]).all()
             continue
-        bound = abs(w[r]) * temperature * rel * 2 * (p + q) + rounding(dtype) * np.abs(wd) + small
+        bound = abs(w[r]) * temperature * rel * 2 * (p + q) + rounding(dtype) * np.abs(wd) + small + abs(w[r]) * temperature * lost
         off = np.abs(der1[r] - wd) - bound
         assert off.max() <= 0, (r, int(off.argmax()), der1[r][off.argmax()], wd[off.argmax()])
     return got
@@ -221,6 +296,32 @@ def test_distill_edges(V, dtype):
                          torch.tensor(val, dtype=DTYPES[dtype], device="cuda"),
                          torch.tensor(tail, dtype=wide, device="cuda"))
         check_distill(x, t, torch.tensor(w, dtype=wide, device="cuda"), 1.0, dtype)
+
+
+@pytest.mark.parametrize("V", [9, 14, 60, 400, 900, 6000, 40000])
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_distill_others_far_below(V, dtype):
+    # the student's other classes lie so far below the teacher's that their exponentials beside them are 0 or
+    # nearly so, all of them or those of a part of the row; the teacher's others weigh something
+    rs = np.random.RandomState(V)
+    a = rs.standard_normal((8, V))
+    at = np.stack([rs.permutation(V)[:5] for _ in a])
+    for r, lift in enumerate((40.0, 60.0, 85.0, 100.0, 300.0, 1000.0, 20000.0, 100.0)):
+        a[r, at[r]] += lift
+    a[7, np.delete(np.arange(V), at[7])] -= np.linspace(0, 400, V - 5)
+    a[6, V // 2] = -np.inf  # (an entry for some V: a loss of +inf)
+    wide = torch.float64 if dtype == "f64" else torch.float32
+    t = cb.TopLogits(torch.tensor(at, dtype=torch.int32, device="cuda"),
+                     torch.tensor(rs.standard_normal((8, 5)), dtype=DTYPES[dtype], device="cuda"),
+                     torch.tensor(rs.uniform(-1, 2, 8), dtype=wide, device="cuda"))
+    # in f32 an exponential below 2^-126 of its unit is 0.  The others' sum s is at least 1e-20 in that unit (or
+    # the unit is their largest, and s >= 1), so Q e / s and e / (s and the rest) lose at most 2^-126 1e20 each
+    lost = 0.0 if dtype == "f64" else 2 * 2.0 ** -126 * 1e20
+    for layout in ("rows", "dims"):
+        x = put(a, dtype, layout)
+        got = check_distill(x, t, None, 1.0, dtype, lost=lost)
+        assert torch.isfinite(got.loss[:6]).all() and (got.der1.double().max(1).values > 0).all()
+        check_distill(x, t, None, 1.0, dtype, out=x, lost=lost)
 
 
 @pytest.mark.parametrize("V", [10, 100, 1000, 5000])
@@ -478,6 +579,21 @@ def test_same_results_again_on_another_stream_and_in_a_graph(V):
     g.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(held, [v.clone() for v in call()]))
+
+
+@pytest.mark.parametrize("V", [100, 3000, 40000])
+def test_the_same_bits_every_time(V):
+    # f64 sums show an order that changes; rows with the largest classes side by side and spread
+    x = make(64, V, "f64", "rows", 9)
+    x[::2, :90] += 12.0
+    t = cb.top_logits(x.flip(0).contiguous(), 33)
+    first = None
+    for _ in range(20):
+        top = cb.top_logits(x, 40)
+        d = cb.distill_derivatives(x, t)
+        got = (top.tail, top.index, d.loss, d.der1)
+        first = first or got
+        assert all(torch.equal(a, b) for a, b in zip(got, first))
 
 
 def test_empty_batches_and_refusals():
