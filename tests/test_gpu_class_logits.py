@@ -541,6 +541,29 @@ def test_top_logits_of_very_many_rows(V, layout, dtype):
         assert cb.top_logits(x, k, tail=False).tail is None
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("V", [17, 33, 75, 90, 100, 127, 128])
+def test_top_logits_of_many_rows_in_every_layout(V, dtype):
+    # rows that start on 16, 8, 4 and 2 bytes, rows by the class and with gaps; every row against a stable sort
+    n, u = 148 * 64 + 7, unit(dtype)
+    a = np.random.RandomState(V).standard_normal((n, V)) * 3
+    a[::3] = np.round(a[::3])  # ties, also across the k-th
+    a[1::50, 5:] = -np.inf
+    for layout in LAYOUTS:
+        x = put(a, dtype, layout)
+        wide = x.double()
+        value, order = torch.sort(wide, dim=1, descending=True, stable=True)
+        for k in (1, 2, 4, 7, 8):
+            got = cb.top_logits(x, k, temperature=0.6)
+            assert torch.equal(got.index.long(), order[:, :k])
+            assert torch.equal(got.value.double(), value[:, :k])
+            want = torch.logsumexp(value[:, k:] / 0.6, dim=1)
+            fine = torch.isfinite(want)
+            assert torch.equal(got.tail[~fine].double(), want[~fine])
+            # u (3 reach + 4), reach at most 40, as in check_top
+            assert ((got.tail.double() - want)[fine].abs() <= u * (124 + 3 * want[fine].abs())).all()
+
+
 # ---- how they are called ---------------------------------------------------------------
 
 def batch(V, dtype="bf16", n=130):
