@@ -8,9 +8,9 @@
 // are bound by that traffic, so one launch does all of an operator.
 //
 // Two shapes of kernel:
-//   narrow (<= kLgNarrow classes)  a block stages a tile of rows in shared memory, then 1, 8 or 32
-//                                  lanes work on each row;
-//   wide                           a cluster of blocks holds one row in its shared memory.
+//   narrow  a block stages a tile of rows in shared memory, then 1, 8 or 32 lanes work on each row:
+//           up to kLgNarrow classes, where there are few rows kLgFew (is_wide; the sampler has its own rule);
+//   wide    a cluster of blocks holds one row in its shared memory.
 // Order of classes: larger logit first, equal logits by lower index, NaN last.
 #pragma once
 
@@ -1225,10 +1225,10 @@ int lg_launch_wide(const char* who, K kernel, int64_t n, const Wide& w, size_t s
     return lg_launch_wide_n(who, kernel, n, w, kLgThreads, smem, st, args...);
 }
 
-// Rows above kLgFew classes are wide when there are few of them: a block of 256 threads a row
-// instead of a warp (8 rows of 1000 f32, derivatives: 5 us against 22; at 20000 rows 193 against 391
-// before the warp's loops stopped at its classes).
-bool is_wide(int64_t n, int V) { return V > kLgNarrow || (V > kLgFew && n <= 148 * 8); }
+// Rows above kLgFew classes are wide when there are few of them: a block of 256 threads a row instead of a
+// warp (f32 rows of 256: 300 of them 10 us against 12 for derivatives and top 16; 4000 27 and 41 against 16
+// and 23).
+bool is_wide(int64_t n, int V) { return V > kLgNarrow || (V > kLgFew && n <= 148 * 2); }
 
 unsigned tiles_of(int64_t n, int rows) { return (unsigned)((n + rows - 1) / rows); }
 

@@ -532,8 +532,8 @@ CBGPU_API int cbgpu_apply_oblivious(const float* features_fm, int64_t n, int32_t
  * hold no state and share no workspace, so they may overlap on any streams
  * and be captured into graphs.  Arithmetic and the "wide" outputs are f64 for
  * CBGPU_F64 logits and f32 for the other types, whose terms are added up in
- * f32 for a few neighbouring classes (16 at most; a row of up to 512 or its
- * tail: a thread's share) and in 64 bits from there.
+ * f32 for up to 16 classes at a time and in 64 bits from there (der1's two
+ * factors join the sums of a row's up to 16 blocks in f32).
  * The same call gives the same bits again; rows in another layout or in a
  * batch of another size may be summed in another grouping (the last bits of
  * loss, der1 and tail).  Outputs may not overlap inputs or each other, but
