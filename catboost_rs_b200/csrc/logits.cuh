@@ -615,32 +615,23 @@ __device__ __forceinline__ float ex2(float x) {  // within 2 ulp; a result below
     return e;
 }
 
-// exp((a - m) / T) as 2^(a c - m c), one fused multiply-add and one ex2 an
-// element.  The rounding of m c is the same for all classes of a base, so it
-// cancels in every ratio; ln() gives the logarithm that belongs to it.  Where m c has no room (rows of the
-// type's lowest value, infinities) `huge` takes the difference first.
+// exp((a - m) / T) as 2^((a - m) c): the difference first, so that an exponential is at most 1 however far from 0
+// the logits lie beside T (2^(a c - round(m c)) is one operation less, but its factor 2^(m c - round(m c)) is
+// infinite from |m / T| of some 1e9 on: masks of -1e10, temperatures of 1e-6).
 template <typename C>
 struct Base;
 template <>
 struct Base<float> {
-    float c, m, mc;
-    bool huge;
-    __device__ Base(float m_, const Scale<float>& sc) : c(sc.c), m(m_), mc(m_ * sc.c) {
-        huge = !(fabsf(mc) < 1e30f);
-    }
-    template <bool kHuge>
-    __device__ float exp(float a) const {
-        return ex2(kHuge ? (a - m) * c : fmaf(a, c, -mc));
-    }
+    float c, m;
+    __device__ Base(float m_, const Scale<float>& sc) : c(sc.c), m(m_) {}
+    __device__ float exp(float a) const { return ex2((a - m) * c); }
     // a vector: each class to its exponential
-    template <bool kHuge, int N>
+    template <int N>
     __device__ void exps(float (&a)[N]) const {
-        const u64 c2 = f2(c, c), k2 = kHuge ? f2(-m, -m) : f2(-mc, -mc);
+        const u64 c2 = f2(c, c), m2 = f2(-m, -m);
 #pragma unroll
         for (int j = 0; j < N; j += 2) {
-            u64 x = f2(a[j], a[j + 1]);
-            x = kHuge ? f2_mul(f2_add(x, k2), c2) : f2_fma(x, c2, k2);
-            f2_split(x, a[j], a[j + 1]);
+            f2_split(f2_mul(f2_add(f2(a[j], a[j + 1]), m2), c2), a[j], a[j + 1]);
             a[j] = ex2(a[j]), a[j + 1] = ex2(a[j + 1]);
         }
     }
@@ -659,41 +650,27 @@ struct Base<float> {
 #pragma unroll
         for (int j = 0; j < N; j += 2) f2_split(f2_mul(f2(e[j], e[j + 1]), k2), e[j], e[j + 1]);
     }
-    __device__ float exp(float a) const { return huge ? exp<true>(a) : exp<false>(a); }
-    __device__ double ln(float a) const {
-        const double x = huge ? ((double)a - (double)m) * (double)c : (double)a * (double)c - (double)mc;
-        return x * 0.6931471805599453;
-    }
-    __device__ float shift(const Base& to) const {  // turns this base's sums into `to`'s
-        return ex2(huge || to.huge ? (m - to.m) * c : mc - to.mc);
-    }
-    __device__ double ln_shift(const Base& to) const {  // the logarithm of that, in 64 bits
-        return 0.6931471805599453 *
-               (huge || to.huge ? ((double)m - (double)to.m) * (double)c : (double)mc - (double)to.mc);
-    }
+    __device__ double ln(float a) const { return ((double)a - (double)m) * (double)c * 0.6931471805599453; }
+    __device__ float shift(const Base& to) const { return ex2((m - to.m) * c); }  // turns this base's sums into `to`'s
+    __device__ double ln_shift(const Base& to) const { return to.ln(m); }  // the logarithm of that, in 64 bits
 };
 template <>
 struct Base<double> {
-    double c, m, mc;
-    bool huge;
-    __device__ Base(double m_, const Scale<double>& sc) : c(sc.c), m(m_), mc(m_ * sc.c) { huge = !(fabs(mc) < 1e300); }
-    template <bool kHuge>
-    __device__ double exp(double a) const {
-        return ::exp(kHuge ? (a - m) * c : fma(a, c, -mc));
-    }
-    template <bool kHuge, int N>
+    double c, m;
+    __device__ Base(double m_, const Scale<double>& sc) : c(sc.c), m(m_) {}
+    __device__ double exp(double a) const { return ::exp((a - m) * c); }
+    template <int N>
     __device__ void exps(double (&a)[N]) const {
 #pragma unroll
-        for (int j = 0; j < N; ++j) a[j] = exp<kHuge>(a[j]);
+        for (int j = 0; j < N; ++j) a[j] = exp(a[j]);
     }
     template <int N>
     __device__ static double total(const double (&e)[N]) { return e[0] + e[1]; }
     template <int N>
     __device__ static void times(double (&e)[N], double k) { e[0] *= k, e[1] *= k; }
-    __device__ double exp(double a) const { return huge ? exp<true>(a) : exp<false>(a); }
-    __device__ double ln(double a) const { return huge ? (a - m) * c : fma(a, c, -mc); }
+    __device__ double ln(double a) const { return (a - m) * c; }
     __device__ double shift(const Base& to) const { return ::exp(ln_shift(to)); }
-    __device__ double ln_shift(const Base& to) const { return huge || to.huge ? (m - to.m) * c : mc - to.mc; }
+    __device__ double ln_shift(const Base& to) const { return to.ln(m); }
 };
 
 constexpr int kLgWarps = kLgThreads / 32;

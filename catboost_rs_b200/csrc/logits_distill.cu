@@ -1,7 +1,5 @@
 // logits_distill.cu -- cbgpu_distill: the Kullback-Leibler loss of a student's rows against a teacher's
 // top logits, and its derivative.
-#include <type_traits>
-
 #include "logits.cuh"
 
 namespace {
@@ -381,17 +379,13 @@ lg_distill_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, TeacherA
     const double z_here = (double)floor_max(top[1]);
 
     double sum[4] = {0.0, 0.0, 0.0, 0.0};  // s_rest, s_top, r_sum, cross
-    auto add = [&](auto huge) {
 #pragma unroll 4
-        for (int v = tid; v < w.nv; v += NT) {
-            C a[VE];
-            unpack(s[v], a, T());
-            here.template exps<decltype(huge)::value>(a);
-            sum[0] += Base<C>::total(a);
-        }
-    };
-    if (here.huge) add(std::true_type());
-    else add(std::false_type());
+    for (int v = tid; v < w.nv; v += NT) {
+        C a[VE];
+        unpack(s[v], a, T());
+        here.exps(a);
+        sum[0] += Base<C>::total(a);
+    }
     if (at >= 0) {
         sum[1] = (double)here.exp(a_own);
         sum[2] = exp(z - z_here);
@@ -415,8 +409,7 @@ lg_distill_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, TeacherA
         for (int v = tid; v < w.nv; v += NT) {
             C a[VE];
             unpack(s[v], a, T());
-            if (rest.huge) rest.template exps<true>(a);
-            else rest.template exps<false>(a);
+            rest.exps(a);
             own += Base<C>::total(a);
         }
         u.red[0][tid] = own;
@@ -459,53 +452,49 @@ lg_distill_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, TeacherA
     }
     if (!out) return;
     const Base<C> base(join.base, sc);
-    auto write = [&](auto huge) {
-        const C c = join.zero ? C(0) : -join.c_rest;
-        auto der = [&](int v, C(&a)[VE]) {
-            unpack(s[v], a, T());
-            base.template exps<decltype(huge)::value>(a);
-            Base<C>::times(a, c);
-        };
-        if (vec_out) {
-            uint4* g = reinterpret_cast<uint4*>(out + ((int64_t)w.v0 * VE - w.head));
-            const int lo = w.whole_lo(), hi = w.whole_hi();
-            constexpr int kRun = 4;  // warps take runs of vectors as they come, since one is late by the loss
-            for (;;) {
-                int v = 0;
-                if (lane == 0) v = atomicAdd(&s_next, kRun * 32);
-                v = lo + __shfl_sync(0xffffffffu, v, 0);
-                if (v >= hi) break;
-                v += lane;
-                if (v - lane + kRun * 32 <= hi) {
+    const C c = join.zero ? C(0) : -join.c_rest;
+    auto der = [&](int v, C(&a)[VE]) {
+        unpack(s[v], a, T());
+        base.exps(a);
+        Base<C>::times(a, c);
+    };
+    if (vec_out) {
+        uint4* g = reinterpret_cast<uint4*>(out + ((int64_t)w.v0 * VE - w.head));
+        const int lo = w.whole_lo(), hi = w.whole_hi();
+        constexpr int kRun = 4;  // warps take runs of vectors as they come, since one is late by the loss
+        for (;;) {
+            int v = 0;
+            if (lane == 0) v = atomicAdd(&s_next, kRun * 32);
+            v = lo + __shfl_sync(0xffffffffu, v, 0);
+            if (v >= hi) break;
+            v += lane;
+            if (v - lane + kRun * 32 <= hi) {
 #pragma unroll
-                    for (int u = 0; u < kRun; ++u) {
-                        C a[VE];
-                        der(v + 32 * u, a);
-                        __stcs(g + v + 32 * u, pack(a, T()));
-                    }
-                } else {
-                    for (; v < hi; v += 32) {
-                        C a[VE];
-                        der(v, a);
-                        __stcs(g + v, pack(a, T()));
-                    }
+                for (int u = 0; u < kRun; ++u) {
+                    C a[VE];
+                    der(v + 32 * u, a);
+                    __stcs(g + v + 32 * u, pack(a, T()));
+                }
+            } else {
+                for (; v < hi; v += 32) {
+                    C a[VE];
+                    der(v, a);
+                    __stcs(g + v, pack(a, T()));
                 }
             }
-            w.template ends<NT>([&](int v) {
-                C a[VE];
-                der(v, a);
-                put(v, a);
-            });
-        } else {
-            for (int v = tid; v < w.nv; v += NT) {
-                C a[VE];
-                der(v, a);
-                put(v, a);
-            }
         }
-    };
-    if (base.huge) write(std::true_type());
-    else write(std::false_type());
+        w.template ends<NT>([&](int v) {
+            C a[VE];
+            der(v, a);
+            put(v, a);
+        });
+    } else {
+        for (int v = tid; v < w.nv; v += NT) {
+            C a[VE];
+            der(v, a);
+            put(v, a);
+        }
+    }
     __syncthreads();  // the entries' classes over the zeros just written
     if (at >= 0)
         out[(int64_t)own * dcs] = from_c<T>(join.zero ? C(0) : join.q_scale * (C)r_own - join.c_top * (C)e_own);

@@ -417,8 +417,7 @@ lg_top_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, int k, Scale
         if (!tail) return;
         ref = floor_max(least);
         const Base<C> at(ref, sc);
-        if (at.huge) at.template exps<true>(a);
-        else at.template exps<false>(a);
+        at.exps(a);
         sum += Base<C>::total(a);
     });
     if (tail) {
@@ -437,8 +436,7 @@ lg_top_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, int k, Scale
             for (int v = tid; v < w.nv; v += kLgThreads) {
                 C a[VE];
                 unpack(s[v], a, T());
-                if (at.huge) at.template exps<true>(a);
-                else at.template exps<false>(a);
+                at.exps(a);
                 part += Base<C>::total(a);
             }
             part = warp_sum(part, 32);

@@ -1,0 +1,129 @@
+"""Class-logit operators at the ends of their ranges: finite masks, very small and very large
+temperatures, parts of a row that weigh nothing, against the plain 64-bit forms.
+
+Tolerances.  u is the unit roundoff (2^-24 for 16- and 32-bit logits, 2^-53 for f64).  An exponential's
+argument is a difference that is rounded, times a scale that is rounded, rounded again: off by at most 3u times
+its size, which counts up to 40 (behind it the exponential is below u).  With 2 ulp of its own an exponential
+is off by 3u 40 + 4u of itself and a probability, two of them, by REL = 2 u 124.  A loss holds two logarithms of
+sums (2 REL), the scaled differences that it adds up, whose rounding is 3u of their size each, and the q that
+it weighs its terms with, each off by REL of itself: REL sum q |ln q / p|, of which the negative terms are
+at most sum p (1 / e) in all, so it is at most REL (loss / T^2 + 2 / e) T^2.  Results that are below 2^-126 of
+their unit are 0 in f32; numbers above the largest of a type are its infinity.
+"""
+import numpy as np
+import pytest
+
+import catboost_rs_b200 as cb
+from tests import logits_reference as ref
+from tests import test_gpu_class_logits as base
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+DTYPES = base.DTYPES
+
+
+@pytest.fixture(scope="module", autouse=True)
+def cuda():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+
+
+def teacher_of(index, value, tail, dtype):
+    wide = torch.float64 if dtype == "f64" else torch.float32
+    return cb.TopLogits(torch.tensor(np.asarray(index), dtype=torch.int32, device="cuda"),
+                        torch.tensor(np.asarray(value, dtype=np.float64), dtype=DTYPES[dtype], device="cuda"),
+                        None if tail is None else torch.tensor(np.asarray(tail, dtype=np.float64), dtype=wide, device="cuda"))
+
+
+def check(x, teacher, T, dtype, out=None):
+    """Loss and derivatives against the definition, taken on rows from which their largest logit was
+    subtracted first (so that the 64-bit form keeps its bits when the logits are large beside T)."""
+    u, rel = base.unit(dtype), 2 * base.unit(dtype) * 124
+    a, idx, val = base.host(x), teacher.index.cpu().numpy(), base.host(teacher.value)
+    tail = np.full(len(a), -np.inf) if teacher.tail is None else base.host(teacher.tail)
+    alone = base.host(cb.distill_loss(x, teacher, temperature=T))
+    got = cb.distill_derivatives(x, teacher, temperature=T, out=out)
+    loss, der1 = base.host(got.loss), base.host(got.der1)
+    low = 0.0 if dtype == "f64" else 2.0 ** -126
+    small = float(torch.finfo(x.dtype).smallest_normal) * float(torch.finfo(x.dtype).eps)
+    wide = torch.finfo(torch.float64 if dtype == "f64" else torch.float32)
+    for r in range(len(a)):
+        row, z = a[r] - max(a[r].max(), np.finfo(np.float64).min), val[r]
+        valid = (idx[r] >= 0) & (idx[r] < x.shape[1])
+        top = z[valid].max() if valid.any() and z[valid].max() > -np.inf else 0.0
+        wl, wd, p, q = ref.distill(row, idx[r], z - top, tail[r] - top / T, 1.0, T)
+        scaled = np.concatenate([[0.0], row[idx[r][valid]], (z - top)[valid]]) / T
+        size = np.abs(scaled[np.isfinite(scaled)]).max()
+        for g in (loss[r], alone[r]):
+            if abs(wl) > float(wide.max):
+                assert g == wl or np.isinf(g), (r, g, wl)
+            elif np.isfinite(wl):
+                assert abs(g - wl) <= T * T * (3 * rel + 6 * u * size) + (rel + 4 * u) * abs(wl) + float(wide.tiny), (r, g, wl)
+            else:
+                assert np.array_equal(g, wl, equal_nan=True), (r, g, wl)
+        bound = T * rel * 2 * (p + q) + base.rounding(dtype) * np.abs(wd) + small + 2 * T * low
+        beyond = np.abs(wd) + bound > float(torch.finfo(x.dtype).max)
+        assert (np.isfinite(der1[r]) | beyond | np.isnan(wd)).all() and (der1[r] * np.sign(wd) >= 0)[beyond].all()
+        off = np.where(beyond, 0.0, np.abs(der1[r] - wd) - bound)
+        assert np.isnan(wd).any() or off.max() <= 0, (r, int(off.argmax()), der1[r][off.argmax()], wd[off.argmax()])
+        assert np.isnan(der1[r]).all() or not np.isnan(wd).any()
+    return got
+
+
+# ---- finite masks ---------------------------------------------------------------------------------
+
+MASKS = [("f64", -1e10), ("f64", -1e20), ("f64", -1e300), ("f32", -1e9), ("f32", -1e10), ("f32", -1e20), ("f32", -1e30),
+         ("bf16", -1e10), ("bf16", -1e20), ("f16", -65504.0)]
+
+
+@pytest.mark.parametrize("V", [14, 400, 513, 900, 6000, 40000, 131072])
+@pytest.mark.parametrize("dtype,mask", MASKS)
+def test_distill_under_finite_masks(V, dtype, mask):
+    rs = np.random.RandomState(V)
+    a = rs.standard_normal((6, V)) * 2
+    at = np.stack([rs.permutation(V // 2)[:5] + V // 2 for _ in a])  # the teacher's classes: in the second half
+    a[0, :V // 2] = mask                                 # a part of the row, whole blocks of it
+    keep = a[1, at[1]].copy()
+    a[1] = mask                                          # all but the teacher's classes
+    a[1, at[1]] = keep
+    a[2] = mask                                          # all of them
+    a[3, V // 2:] = mask                                 # the teacher's classes among them
+    a[4, at[4]] += 30.0
+    a[4, :V // 2] = mask
+    z = rs.standard_normal((6, 5))
+    for T in (1.0, 0.5, 2.0):
+        for tail in (rs.uniform(-1, 2, 6), None):
+            x, t = base.put(a, dtype), teacher_of(at, z, tail, dtype)
+            got = check(x, t, T, dtype)
+            assert not torch.isnan(got.loss).any() and not torch.isnan(got.der1).any()
+            check(x, t, T, dtype, out=x)
+
+
+@pytest.mark.parametrize("V", [14, 100, 400, 513, 900, 6000, 40000, 131072])
+@pytest.mark.parametrize("dtype,mask", MASKS)
+def test_top_logits_under_finite_masks(V, dtype, mask):
+    rs = np.random.RandomState(V)
+    a = rs.standard_normal((5, V)) * 2
+    for r, left in enumerate((3, 5, 7, 0)):  # unmasked classes
+        masked = np.ones(V, dtype=bool)
+        masked[rs.permutation(V)[:left]] = False
+        a[r, masked] = mask
+    a[4, :V // 2] = mask
+    x = base.put(a, dtype)
+    for T in (1.0, 0.5, 2.0):
+        base.check_top(x, 5, T, dtype)
+
+
+# ---- the ends of the temperature's range --------------------------------------------------------------
+
+@pytest.mark.parametrize("V", [14, 100, 400, 513, 900, 6000, 40000])
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("T,spread", [(1e-6, 1.0), (1e-6, 3000.0), (1e-6, 1e-6), (1e-3, 300.0), (1e6, 3.0), (1e6, 30000.0)])
+def test_ends_of_the_temperature(V, dtype, T, spread):
+    n = 3
+    x = base.put(np.random.RandomState(V).standard_normal((n, V)) * spread, dtype)
+    base.check_top(x, 5, T, dtype)
+    rs = np.random.RandomState(V + 1)  # a teacher whose logits are of the size of T
+    at, z = np.stack([rs.permutation(V)[:5] for _ in range(n)]), rs.standard_normal((n, 5)) * min(T, 100.0)
+    check(x, teacher_of(at, z, None, dtype), T, dtype)
