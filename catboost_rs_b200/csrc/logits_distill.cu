@@ -253,9 +253,13 @@ __device__ DistillJoin<C> distill_join(const DistillPart<C>& p, int rank, int bl
     const C r_sum = r_tail + warp_sum(p.r_sum == 0.0 ? C(0) : (C)p.r_sum * g, blocks);
     const C q = r_tail / r_sum, per_s = C(1) / s;
     DistillJoin<C> j;
-    j.base = rest.m;
+    // Without a tail nothing needs the others' sum by itself, and blocks whose others lie far below have not looked
+    // for their largest: the others are then relative to the row's maximum, beside which each is 1 at most.
+    const bool apart = tl > -lg_inf(C());
+    j.base = apart ? rest.m : base.m;
     j.zero = s == C(0) || r_sum == C(0);  // every class masked, or a teacher without an entry
-    j.c_rest = w * (q != q ? q : (q != C(0) && s_rest != C(0) ? per_s * unit - q / s_rest : per_s * unit));
+    const C per_e = apart ? per_s * unit : per_s;
+    j.c_rest = w * (q != q ? q : (q != C(0) && s_rest != C(0) ? per_e - q / s_rest : per_e));
     j.q_scale = __shfl_sync(0xffffffffu, w / r_sum * g, rank);
     j.c_top = __shfl_sync(0xffffffffu, w * per_s * f, rank);
     return j;

@@ -3,8 +3,11 @@ temperatures, parts of a row that weigh nothing, against the plain 64-bit forms.
 
 Tolerances.  u is the unit roundoff (2^-24 for 16- and 32-bit logits, 2^-53 for f64).  An exponential's
 argument is a difference that is rounded, times a scale that is rounded, rounded again: off by at most 3u times
-its size, which counts up to 40 (behind it the exponential is below u).  With 2 ulp of its own an exponential
-is off by 3u 40 + 4u of itself and a probability, two of them, by REL = 2 u 124.  A loss holds two logarithms of
+its size r, which in a sum counts up to 40 (behind it the exponential is below u).  With 2 ulp of its own an
+exponential is off by 3u r + 4u of itself, a sum by 124 u, a probability by u (3 r + 128), REL = 2 u 124 for those
+that count beside 1; one far below is small, but as a share of itself off by its own r (up to 800, where it is 0 in
+64 bits), and der1 of a class below shows it.  The 64-bit forms run on long doubles here: their differences
+of large logits keep the bits that the devices' 64-bit differences keep.  A loss holds two logarithms of
 sums (2 REL), the scaled differences that it adds up, whose rounding is 3u of their size each, and the q that
 it weighs its terms with, each off by REL of itself: REL sum q |ln q / p|, of which the negative terms are
 at most sum p (1 / e) in all, so it is at most REL (loss / T^2 + 2 / e) T^2.  Results that are below 2^-126 of
@@ -49,10 +52,12 @@ def check(x, teacher, T, dtype, out=None):
     small = float(torch.finfo(x.dtype).smallest_normal) * float(torch.finfo(x.dtype).eps)
     wide = torch.finfo(torch.float64 if dtype == "f64" else torch.float32)
     for r in range(len(a)):
-        row, z = a[r] - max(a[r].max(), np.finfo(np.float64).min), val[r]
+        row = a[r].astype(np.longdouble) - max(a[r].max(), np.finfo(np.float64).min)
+        z = val[r].astype(np.longdouble)
         valid = (idx[r] >= 0) & (idx[r] < x.shape[1])
         top = z[valid].max() if valid.any() and z[valid].max() > -np.inf else 0.0
-        wl, wd, p, q = ref.distill(row, idx[r], z - top, tail[r] - top / T, 1.0, T)
+        wl, wd, p, q = ref.distill(row, idx[r], z - top, tail[r] - top / T, 1.0, np.longdouble(T))
+        wl, wd = float(wl), wd.astype(np.float64)
         scaled = np.concatenate([[0.0], row[idx[r][valid]], (z - top)[valid]]) / T
         size = np.abs(scaled[np.isfinite(scaled)]).max()
         for g in (loss[r], alone[r]):
@@ -62,7 +67,8 @@ def check(x, teacher, T, dtype, out=None):
                 assert abs(g - wl) <= T * T * (3 * rel + 6 * u * size) + (rel + 4 * u) * abs(wl) + float(wide.tiny), (r, g, wl)
             else:
                 assert np.array_equal(g, wl, equal_nan=True), (r, g, wl)
-        bound = T * rel * 2 * (p + q) + base.rounding(dtype) * np.abs(wd) + small + 2 * T * low
+        own = np.maximum(rel, u * (3 * np.minimum(-row / T, 800.0) + 128))
+        bound = T * own * 2 * (p + q) + base.rounding(dtype) * np.abs(wd) + small + 2 * T * low
         beyond = np.abs(wd) + bound > float(torch.finfo(x.dtype).max)
         assert (np.isfinite(der1[r]) | beyond | np.isnan(wd)).all() and (der1[r] * np.sign(wd) >= 0)[beyond].all()
         off = np.where(beyond, 0.0, np.abs(der1[r] - wd) - bound)
@@ -127,3 +133,28 @@ def test_ends_of_the_temperature(V, dtype, T, spread):
     rs = np.random.RandomState(V + 1)  # a teacher whose logits are of the size of T
     at, z = np.stack([rs.permutation(V)[:5] for _ in range(n)]), rs.standard_normal((n, 5)) * min(T, 100.0)
     check(x, teacher_of(at, z, None, dtype), T, dtype)
+
+
+# ---- parts of a row that weigh nothing ------------------------------------------------------------------
+
+@pytest.mark.parametrize("V", [10, 14, 60, 400, 900, 6000, 40000, 131072])
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("T", [0.1, 1.0])
+def test_distill_others_far_below_without_a_tail(V, dtype, T):
+    # the others lie so far below the entries that their exponentials beside them are 0, and yet far above 0
+    # (88.7 T is where a 32-bit exponential of the logit itself ends, 709 T a 64-bit one), in the whole row or
+    # in one part of it while another part lies lower still
+    rs = np.random.RandomState(V)
+    a = rs.standard_normal((6, V)) * T
+    at = np.stack([rs.permutation(V // 2)[:5] for _ in a])  # in the first half
+    for r, (entries, others) in enumerate(((200, 100), (2000, 1000), (40000, 20000), (300, 0), (-100, -200), (120, 5))):
+        a[r] += others * T
+        a[r, at[r]] += (entries - others) * T
+    a[3, :V // 2] += 150 * T     # the others of the entries' half of the row far above those of the other half
+    a[5, V // 2:] += 90 * T      # and below them
+    z = rs.standard_normal((6, 5)) * T
+    for tail in (None, np.full(6, -np.inf), rs.uniform(-1, 2, 6)):
+        x, t = base.put(a, dtype), teacher_of(at, z, tail, dtype)
+        got = check(x, t, T, dtype)
+        assert not torch.isnan(got.der1).any() and not torch.isnan(got.loss).any()
+        check(x, t, T, dtype, out=x)
