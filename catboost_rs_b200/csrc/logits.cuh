@@ -113,8 +113,9 @@ __device__ __forceinline__ double lg_inf(double) { return __longlong_as_double(0
 __device__ __forceinline__ float lowest(float) { return __int_as_float((int)0xff7fffffu); }  // of the finite numbers
 __device__ __forceinline__ double lowest(double) { return __longlong_as_double((long long)0xffefffffffffffffull); }
 
-// exp((a - m) / T).  f32: 2^((a - m) c) with c = log2(e) / T rounded to f32 (a relative change of the
-// temperature by at most 2^-24, taken for teacher and student alike).
+// exp((a - m) / T).  f32: 2^((a - m) c) with c = log2(e) / T rounded to f32: a relative change of the
+// temperature by at most 2^-24, taken for differences of logits, of teacher and student alike.  A maximum, which
+// may be large beside T, meets a tail, which comes divided by T, in 64 bits and by T itself.
 __device__ __forceinline__ float lg_exp(float d, float c) { return exp2f(d * c); }
 __device__ __forceinline__ double lg_exp(double d, double c) { return exp(d * c); }
 template <typename C>
@@ -123,12 +124,14 @@ template <>
 struct Scale<float> {
     float c;
     double inv_t;  // the 1 / T that c stands for
-    __host__ explicit Scale(double t) : c((float)(1.4426950408889634 / t)), inv_t((double)c * 0.6931471805599453) {}
+    double t, by_t;  // T and 1 / T
+    __host__ explicit Scale(double t)
+        : c((float)(1.4426950408889634 / t)), inv_t((double)c * 0.6931471805599453), t(t), by_t(1.0 / t) {}
 };
 template <>
 struct Scale<double> {
-    double c, inv_t;
-    __host__ explicit Scale(double t) : c(1.0 / t), inv_t(1.0 / t) {}
+    double c, inv_t, t, by_t;
+    __host__ explicit Scale(double t) : c(1.0 / t), inv_t(c), t(t), by_t(c) {}
 };
 
 // A maximum that is subtracted: 0 where there is no class, so that the exponentials are 0 there.

@@ -20,6 +20,21 @@ namespace {
 // largest of the others instead: Q ln s_t and Q / s_t need s_t by itself, not beside s.
 constexpr double kFar = 1e-20;
 
+// The teacher's largest logit z_max and its tail: an entry's exponential is exp((z_j - z_max) / T - lift), the
+// tail's exp(tail), both at most 1.  Differences are taken before they are scaled, so that their rounding does not
+// grow with the logits.
+struct TeacherBase {
+    double z, tail, lift;
+    template <typename C>
+    __device__ TeacherBase(C z_max, double tl, const Scale<C>& sc) : z((double)floor_max(z_max)) {
+        tail = fma(tl, sc.t, -z) * sc.by_t;  // beside z_max: tl - z / T
+        if (tail == lg_inf(0.0) && tl < tail) tail = -lowest(0.0);  // out of range: the entries weigh nothing
+        lift = floor_max(fmax(z_max == -lg_inf(C()) ? -lg_inf(0.0) : 0.0, tail));
+        tail -= lift;
+    }
+    __device__ double entry(double zj, double inv_t) const { return fma(zj - z, inv_t, -lift); }
+};
+
 template <typename C>
 struct RowOut {  // what turns a row's logits into its loss and derivative
     double loss;
@@ -133,7 +148,7 @@ lg_distill_narrow_kernel(Rows<T> x, TeacherArgs tc, const typename Num<T>::C* __
         }
         m = floor_max(t.reduce(m, OpMax()));
         zm = t.reduce(zm, OpMax());
-        const double z_max = floor_max(fmax((double)zm * sc.inv_t, tl));
+        const TeacherBase z_base(zm, tl, sc);
         C sum_top = 0, sum_rest = 0;
         double r_sum = 0.0, cross = 0.0;
         if (by_entry) {  // a lane an entry: fewer steps in 64 bits than by class (for which a warp's rows differ)
@@ -141,7 +156,7 @@ lg_distill_narrow_kernel(Rows<T> x, TeacherArgs tc, const typename Num<T>::C* __
                 if (!((claimed >> (j0 / G)) & 1)) continue;
                 const int i = (int)tc.idx((r0 + r) * tc.k + j0 + t.rank);
                 const C ai = to_c(direct ? g[r * x.row_stride + (int64_t)i * x.class_stride] : row[i]);
-                const double d = (double)tgt[i] * sc.inv_t - z_max;
+                const double d = z_base.entry((double)tgt[i], sc.inv_t);
                 const C rj = row_exp((C)d, table);
                 r_sum += (double)rj;
                 if (rj != C(0)) cross += (double)rj * (d - ((double)ai - (double)m) * sc.inv_t);
@@ -157,7 +172,7 @@ lg_distill_narrow_kernel(Rows<T> x, TeacherArgs tc, const typename Num<T>::C* __
                     a[it] = e;
                     continue;
                 }
-                const double d = (double)tgt[mine.first + it] * sc.inv_t - z_max;
+                const double d = z_base.entry((double)tgt[mine.first + it], sc.inv_t);
                 const double rj = (double)row_exp((C)d, table);
                 r_sum += rj;
                 if (rj != 0.0) cross += rj * (d - ((double)a[it] - (double)m) * sc.inv_t);
@@ -171,7 +186,7 @@ lg_distill_narrow_kernel(Rows<T> x, TeacherArgs tc, const typename Num<T>::C* __
         double s_rest = t.reduce((double)sum_rest, OpSum()), rest_ln = 0.0;
         r_sum = t.reduce(r_sum, OpSum());
         cross = t.reduce(cross, OpSum());
-        const double r_tail = (double)row_exp((C)(tl - z_max), table);
+        const double r_tail = (double)row_exp((C)z_base.tail, table);
         if (s_rest < kFar && r_tail > 0.0) {  // the same for a row's lanes
             auto logit = [&](int i) { return to_c(direct ? g[r * x.row_stride + (int64_t)i * x.class_stride] : row[i]); };
             C mr = -lg_inf(C());
@@ -187,7 +202,7 @@ lg_distill_narrow_kernel(Rows<T> x, TeacherArgs tc, const typename Num<T>::C* __
                 rest_ln = ((double)mr - (double)m) * sc.inv_t;
             }
         }
-        RowOut<C> o = distill_finish<C>(w, temp, s_top, s_rest, r_sum + r_tail, r_tail, tl - z_max, cross, rest_ln);
+        RowOut<C> o = distill_finish<C>(w, temp, s_top, s_rest, r_sum + r_tail, r_tail, z_base.tail, cross, rest_ln);
         if (w == 0.0) {
             o = RowOut<C>{};
             o.zero = true;
@@ -223,7 +238,7 @@ lg_distill_narrow_kernel(Rows<T> x, TeacherArgs tc, const typename Num<T>::C* __
 // sums, exchange, of which three blocks an SM cover a part.  Rows held in registers instead were slower
 // (the unrolled passes leave the instruction cache), and so were 512 threads a block.
 template <typename C>
-struct DistillPart {  // sums relative to the block's own maxima: m of its logits, z of its entries' z / T
+struct DistillPart {  // sums relative to the block's own maxima: m of its logits, z of its entries' logits
     double s_rest, s_top, r_sum, cross;
     C m, z, m_rest;  // m_rest: what s_rest is relative to, m or (far below it) the largest of the others
     __device__ C rest() const { return s_rest == 0.0 ? -lg_inf(C()) : m_rest; }
@@ -242,12 +257,12 @@ struct DistillJoin {  // for the second pass, from the joined parts
 template <typename C>
 __device__ DistillJoin<C> distill_join(const DistillPart<C>& p, int rank, int blocks, C w, C tl, const Scale<C>& sc) {
     const Base<C> base(floor_max(warp_max(p.m)), sc);
-    const C z_max = floor_max(OpMax()(warp_max(p.z), tl));
+    const TeacherBase z_base(warp_max(p.z), (double)tl, sc);
     const C rest_max = warp_max(p.rest());
     const Base<C> rest(floor_max(rest_max), sc);
     const C f = Base<C>(floor_max(p.m), sc).shift(base), h = Base<C>(floor_max(p.m_rest), sc).shift(rest);
     const C unit = rest_max == -lg_inf(C()) ? C(0) : rest.shift(base);
-    const C g = part_exp(floor_max(p.z) - z_max), r_tail = part_exp(tl - z_max);
+    const C g = part_exp((C)z_base.entry((double)floor_max(p.z), sc.inv_t)), r_tail = part_exp((C)z_base.tail);
     const C s_rest = warp_sum(p.s_rest == 0.0 ? C(0) : (C)p.s_rest * h, blocks);
     const C s = s_rest * unit + warp_sum(p.s_top == 0.0 ? C(0) : (C)p.s_top * f, blocks);
     const C r_sum = r_tail + warp_sum(p.r_sum == 0.0 ? C(0) : (C)p.r_sum * g, blocks);
@@ -269,9 +284,9 @@ __device__ DistillJoin<C> distill_join(const DistillPart<C>& p, int rank, int bl
 template <typename C>
 __device__ double distill_loss(const DistillPart<C>& p, int blocks, double w, double t, double tl, const Scale<C>& sc) {
     const Base<C> base(floor_max(warp_max(p.m)), sc);
-    const double z_max = floor_max(fmax((double)warp_max(p.z), tl));
+    const TeacherBase z_base(warp_max(p.z), tl, sc);
     const double ln_f = Base<C>(floor_max(p.m), sc).ln_shift(base), f = exp(ln_f);
-    const double ln_g = (double)floor_max(p.z) - z_max, g = exp(ln_g);
+    const double ln_g = z_base.entry((double)floor_max(p.z), sc.inv_t), g = exp(ln_g);
     const C rest_max = warp_max(p.rest());
     const Base<C> rest(floor_max(rest_max), sc);
     const double s_rest =
@@ -279,9 +294,9 @@ __device__ double distill_loss(const DistillPart<C>& p, int blocks, double w, do
     const double rest_ln = rest_max == -lg_inf(C()) ? 0.0 : rest.ln_shift(base);
     const double s_top = warp_sum(p.s_top == 0.0 ? 0.0 : p.s_top * f, blocks);
     const double r_sum = warp_sum(p.r_sum == 0.0 ? 0.0 : p.r_sum * g, blocks);
-    const double cross = warp_sum(p.r_sum == 0.0 ? 0.0 : g * (p.cross + p.r_sum * (ln_g - ln_f)), blocks);
-    const double r_tail = exp(tl - z_max);
-    return distill_finish<double>(w, t, s_top, s_rest, r_sum + r_tail, r_tail, tl - z_max, cross, rest_ln).loss;
+    const double cross = warp_sum(p.r_sum == 0.0 || g == 0.0 ? 0.0 : g * (p.cross + p.r_sum * (ln_g - ln_f)), blocks);
+    const double r_tail = exp(z_base.tail);
+    return distill_finish<double>(w, t, s_top, s_rest, r_sum + r_tail, r_tail, z_base.tail, cross, rest_ln).loss;
 }
 
 template <typename T, int NT>
@@ -342,7 +357,7 @@ lg_distill_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, TeacherA
         return;
     }
     const int64_t idx = tid < k ? tc.of_idx_bits(i_bits) : -1;
-    double z = tid < k ? (double)(C)of_bits(z_bits, tc.value_dtype) * sc.inv_t : -lg_inf(0.0);
+    C z = tid < k ? (C)of_bits(z_bits, tc.value_dtype) : -lg_inf(C());
     const int own = idx >= 0 && idx < w.V ? (int)idx : -1;  // the class of this thread's entry
     if (tid < k) s_idx[tid] = own;
     __syncthreads();
@@ -366,10 +381,10 @@ lg_distill_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, TeacherA
         a_own = to_c(se[at]);
         se[at] = from_c<T>(-lg_inf(C()));
     } else {
-        z = -lg_inf(0.0);
+        z = -lg_inf(C());
     }
     {
-        const C m = warp_max(OpMax()(most.get(), a_own)), zm = warp_id * 32 < k ? warp_max((C)z) : -lg_inf(C());
+        const C m = warp_max(OpMax()(most.get(), a_own)), zm = warp_id * 32 < k ? warp_max(z) : -lg_inf(C());
         if (lane == 0) red_max[0][warp_id] = m, red_max[1][warp_id] = zm;
     }
     __syncthreads();
@@ -392,8 +407,9 @@ lg_distill_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, TeacherA
     }
     if (at >= 0) {
         sum[1] = (double)here.exp(a_own);
-        sum[2] = exp(z - z_here);
-        if (sum[2] != 0.0) sum[3] = sum[2] * (z - z_here - here.ln(a_own));
+        const double d = ((double)z - z_here) * sc.inv_t;
+        sum[2] = exp(d);
+        if (sum[2] != 0.0) sum[3] = sum[2] * (d - here.ln(a_own));
     }
     const double e_own = sum[1], r_own = sum[2];
 #pragma unroll

@@ -141,7 +141,7 @@ lg_top_narrow_kernel(Rows<T> x, int k, Scale<typename Num<T>::C> sc, int tile, T
             if (key[it] != 0) part += lg_exp(to_c(row[mine.first + it]) - m, sc.c);
         const double sum = t.reduce((double)part, OpSum());
         if (t.rank == 0) {
-            const double none = sum == 0.0 ? -lg_inf(0.0) : log(sum) + (double)m * sc.inv_t;
+            const double none = sum == 0.0 ? -lg_inf(0.0) : log(sum) + (double)m * sc.by_t;
             tail[r0 + r] = (C)(nan ? lg_inf(0.0) - lg_inf(0.0) : none);
         }
     }
@@ -374,7 +374,7 @@ lg_top_thread_kernel(Rows<T> x, int k, Scale<float> sc, int unit, T* __restrict_
                 sum += v < last ? (double)ex2((v - base) * sc.c) : 0.0;
             }
     }
-    const double none = sum == 0.0 ? -lg_inf(0.0) : log(sum) + (double)base * sc.inv_t;
+    const double none = sum == 0.0 ? -lg_inf(0.0) : log(sum) + (double)base * sc.by_t;
     tail[r] = (float)(ties > 0 && last == lg_inf(0.0f) ? nan : none);
 }
 
@@ -470,8 +470,8 @@ lg_top_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, int k, Scale
     sum = warp_sum(sum, 32);
     if (tid == 0) {
         const double nan = (double)lg_inf(C()) - (double)lg_inf(C());
-        // ln sum + the logarithm of the base's 1; a NaN among the first k (its key is 0) counts as one anywhere
-        tail[r] = sh.key[k - 1] == 0 ? (C)nan : (C)(sum == 0.0 ? -lg_inf(0.0) : log(sum) - base.ln(C(0)));
+        // ln sum + the base's logit scaled; a NaN among the first k (its key is 0) counts as one anywhere
+        tail[r] = sh.key[k - 1] == 0 ? (C)nan : (C)(sum == 0.0 ? -lg_inf(0.0) : log(sum) + (double)base.m * sc.by_t);
     }
 }
 

@@ -6,13 +6,15 @@ argument is a difference that is rounded, times a scale that is rounded, rounded
 its size r, which in a sum counts up to 40 (behind it the exponential is below u).  With 2 ulp of its own an
 exponential is off by 3u r + 4u of itself, a sum by 124 u, a probability by u (3 r + 128), REL = 2 u 124 for those
 that count beside 1; one far below is small, but as a share of itself off by its own r (up to 800, where it is 0 in
-64 bits), and der1 of a class below shows it.  The 64-bit forms run on long doubles here: their differences
-of large logits keep the bits that the devices' 64-bit differences keep.  A loss holds two logarithms of
+64 bits), and der1 of a class below shows it.  The 64-bit forms run on long doubles for f64 rows: their differences
+of large logits keep the bits that the device's 64-bit differences keep.  A loss holds two logarithms of
 sums (2 REL), the scaled differences that it adds up, whose rounding is 3u of their size each, and the q that
 it weighs its terms with, each off by REL of itself: REL sum q |ln q / p|, of which the negative terms are
 at most sum p (1 / e) in all, so it is at most REL (loss / T^2 + 2 / e) T^2.  Results that are below 2^-126 of
 their unit are 0 in f32; numbers above the largest of a type are its infinity.
 """
+from fractions import Fraction
+
 import numpy as np
 import pytest
 
@@ -51,12 +53,19 @@ def check(x, teacher, T, dtype, out=None):
     low = 0.0 if dtype == "f64" else 2.0 ** -126
     small = float(torch.finfo(x.dtype).smallest_normal) * float(torch.finfo(x.dtype).eps)
     wide = torch.finfo(torch.float64 if dtype == "f64" else torch.float32)
+    real = np.longdouble if dtype == "f64" else np.float64
     for r in range(len(a)):
-        row = a[r].astype(np.longdouble) - max(a[r].max(), np.finfo(np.float64).min)
-        z = val[r].astype(np.longdouble)
+        row = a[r].astype(real) - max(a[r].max(), np.finfo(np.float64).min)
+        z = val[r].astype(real)
         valid = (idx[r] >= 0) & (idx[r] < x.shape[1])
         top = z[valid].max() if valid.any() and z[valid].max() > -np.inf else 0.0
-        wl, wd, p, q = ref.distill(row, idx[r], z - top, tail[r] - top / T, 1.0, np.longdouble(T))
+        # (tail T - z) / T exactly: the product has at most 106 bits
+        beside_top = real(tail[r])
+        if np.isfinite(tail[r]):
+            exact = (Fraction(float(tail[r])) * Fraction(T) - Fraction(float(top))) / Fraction(T)
+            most = Fraction(np.finfo(np.float64).max)
+            beside_top = real(float(max(-most, min(most, exact))))
+        wl, wd, p, q = ref.distill(row, idx[r], z - top, beside_top, 1.0, real(T))
         wl, wd = float(wl), wd.astype(np.float64)
         scaled = np.concatenate([[0.0], row[idx[r][valid]], (z - top)[valid]]) / T
         size = np.abs(scaled[np.isfinite(scaled)]).max()
@@ -133,6 +142,49 @@ def test_ends_of_the_temperature(V, dtype, T, spread):
     rs = np.random.RandomState(V + 1)  # a teacher whose logits are of the size of T
     at, z = np.stack([rs.permutation(V)[:5] for _ in range(n)]), rs.standard_normal((n, 5)) * min(T, 100.0)
     check(x, teacher_of(at, z, None, dtype), T, dtype)
+
+
+# ---- teachers' logits that are large beside the temperature -----------------------------------------------
+
+@pytest.mark.parametrize("V", [14, 100, 400, 513, 900, 6000, 40000])
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("T,spread", [(1e-6, 1.0), (1e-6, 3000.0), (1e-3, 300.0), (0.3, 20000.0), (1.0, 60000.0), (1e6, 30000.0)])
+def test_teachers_logits_large_beside_the_temperature(V, dtype, T, spread):
+    x = base.put(np.random.RandomState(V).standard_normal((3, V)) * T, dtype)
+    # (within the 16-bit type's range)
+    y = base.put(np.clip(np.random.RandomState(V + 1).standard_normal((3, V)) * spread, -6e4, 6e4), dtype)
+    y[:, V // 2] = y[:, 0] = y.max()  # several of much the same weight
+    t = cb.top_logits(y, 5, temperature=T)
+    check(x, t, T, dtype)
+    check(x, cb.TopLogits(t.index, t.value), T, dtype)
+    # the same by the logits of the teacher as they are: its entries lie where the tail puts them
+    check(y, t, T, dtype)
+
+
+@pytest.mark.parametrize("V", [14, 100, 400, 513, 900, 6000, 40000])
+@pytest.mark.parametrize("dtype,mask", MASKS)
+def test_teachers_under_finite_masks(V, dtype, mask):
+    # entries of a teacher's masked classes: a few, all of them beside a tail, all without one (they share it)
+    rs = np.random.RandomState(V)
+    x = base.put(rs.standard_normal((4, V)), dtype)
+    at = np.stack([rs.permutation(V)[:5] for _ in range(4)])
+    z = rs.standard_normal((4, 5))
+    z[0, 3:], z[1] = mask, mask
+    z[2] = float(torch.finfo(DTYPES[dtype]).min)
+    for T in (1.0, 0.5, 2.0, 0.7):
+        for tail in (None, np.array([0.3, 0.1, -0.5, 1.0]), np.array([0.3, mask / T, 0.3, 0.3])):
+            t = teacher_of(at, z, tail, dtype)
+            got = check(x, t, T, dtype)
+            assert torch.isfinite(got.loss).all() and torch.isfinite(got.der1).all()
+    # the teacher's top logits of rows that are masked but for some
+    a = rs.standard_normal((4, V))
+    for r, left in enumerate((3, 5, 0, V // 2)):
+        masked = np.ones(V, dtype=bool)
+        masked[rs.permutation(V)[:left]] = False
+        a[r, masked] = mask
+    t = cb.top_logits(base.put(a, dtype), 5)
+    got = check(x, t, 1.0, dtype)
+    assert torch.isfinite(got.loss).all() and torch.isfinite(got.der1).all()
 
 
 # ---- parts of a row that weigh nothing ------------------------------------------------------------------
