@@ -260,12 +260,15 @@ __device__ DistillJoin<C> distill_join(const DistillPart<C>& p, int rank, int bl
     const TeacherBase z_base(warp_max(p.z), (double)tl, sc);
     const C rest_max = warp_max(p.rest());
     const Base<C> rest(floor_max(rest_max), sc);
-    const C f = Base<C>(floor_max(p.m), sc).shift(base), h = Base<C>(floor_max(p.m_rest), sc).shift(rest);
+    // (a part of weight 0 may have no maximum: relative to 0 instead, its factor can be infinite)
+    const C f = p.s_top == 0.0 ? C(0) : Base<C>(floor_max(p.m), sc).shift(base);
+    const C h = p.s_rest == 0.0 ? C(0) : Base<C>(floor_max(p.m_rest), sc).shift(rest);
     const C unit = rest_max == -lg_inf(C()) ? C(0) : rest.shift(base);
-    const C g = part_exp((C)z_base.entry((double)floor_max(p.z), sc.inv_t)), r_tail = part_exp((C)z_base.tail);
-    const C s_rest = warp_sum(p.s_rest == 0.0 ? C(0) : (C)p.s_rest * h, blocks);
-    const C s = s_rest * unit + warp_sum(p.s_top == 0.0 ? C(0) : (C)p.s_top * f, blocks);
-    const C r_sum = r_tail + warp_sum(p.r_sum == 0.0 ? C(0) : (C)p.r_sum * g, blocks);
+    const C g = p.r_sum == 0.0 ? C(0) : part_exp((C)z_base.entry((double)floor_max(p.z), sc.inv_t));
+    const C r_tail = part_exp((C)z_base.tail);
+    const C s_rest = warp_sum((C)p.s_rest * h, blocks);
+    const C s = s_rest * unit + warp_sum((C)p.s_top * f, blocks);
+    const C r_sum = r_tail + warp_sum((C)p.r_sum * g, blocks);
     const C q = r_tail / r_sum, per_s = C(1) / s;
     DistillJoin<C> j;
     // Without a tail nothing needs the others' sum by itself, and blocks whose others lie far below have not looked

@@ -210,3 +210,28 @@ def test_distill_others_far_below_without_a_tail(V, dtype, T):
         got = check(x, t, T, dtype)
         assert not torch.isnan(got.der1).any() and not torch.isnan(got.loss).any()
         check(x, t, T, dtype, out=x)
+
+
+@pytest.mark.parametrize("V", [10, 14, 60, 400, 900, 6000, 40000, 131072])
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("T", [0.1, 1.0])
+def test_distill_entries_of_no_weight_in_rows_far_below_0(V, dtype, T):
+    # a part of the row whose entries the teacher rules out (-inf), or whose classes the student masks (-inf), has no
+    # maximum of its own: beside maxima of -200 T (-1500 T in 64 bits) nothing may be taken relative to 0
+    rs = np.random.RandomState(V)
+    a = rs.standard_normal((5, V)) * T - 200 * T
+    at = np.concatenate([np.stack([rs.permutation(V // 2)[:3] for _ in a]),
+                         np.stack([rs.permutation(V // 2)[:2] + V // 2 for _ in a])], axis=1)
+    z = rs.standard_normal((5, 5)) * T - 200 * T
+    z[0, :3] = -np.inf                       # the entries of the first half
+    a[1, :V // 2], z[1, :3] = -np.inf, -np.inf   # and the student masks that half
+    a[2, :V // 2] = -np.inf                  # the student alone: loss +inf, der1 finite
+    z[3, :4] = -np.inf
+    a[4, V // 2:], z[4, 3:] = -np.inf, -np.inf
+    lower = 1300 * T if dtype == "f64" else 0.0
+    for tail in (None, rs.uniform(-1, 2, 5) - 200 - lower / T):
+        x, t = base.put(a - lower, dtype), teacher_of(at, z - lower, tail, dtype)
+        got = check(x, t, T, dtype)
+        assert not torch.isnan(got.der1).any() and not torch.isnan(got.loss).any()
+        assert torch.isinf(got.loss).tolist() == [False, False, True, False, False]
+        check(x, t, T, dtype, out=x)
