@@ -334,6 +334,16 @@ lg_distill_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, TeacherA
         for (int j = 0; j < VE; ++j)
             if (i + j >= 0 && i + j < w.V) out[(int64_t)(i + j) * dcs] = from_c<T>(d[j]);
     };
+    auto put_zeros = [&] {  // whatever the row holds
+        const C zero[VE] = {};
+        if (vec_out) {
+            uint4* g = reinterpret_cast<uint4*>(out + ((int64_t)w.v0 * VE - w.head));
+            for (int v = w.whole_lo() + tid; v < w.whole_hi(); v += NT) __stcs(g + v, make_uint4(0, 0, 0, 0));
+            w.template ends<NT>([&](int v) { put(v, zero); });
+        } else {
+            for (int v = tid; v < w.nv; v += NT) put(v, zero);
+        }
+    };
     if (blocks > 1) cluster_arrive<false>();
 
     // the row's own numbers are asked for before its logits and used after them
@@ -353,9 +363,7 @@ lg_distill_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, TeacherA
     w.template load<NT>(s, [&](const uint4& q) { most(q); });
     if (wt == C(0)) {  // the same for all blocks of the cluster
         if (tid == 0 && rank == 0) loss[r] = 0;
-        const C zero[VE] = {};
-        if (out)
-            for (int v = tid; v < w.nv; v += NT) put(v, zero);
+        if (out) put_zeros();
         if (blocks > 1) cluster_wait();
         return;
     }
@@ -474,8 +482,12 @@ lg_distill_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, TeacherA
         if (lane == 0) loss[r] = (C)v;
     }
     if (!out) return;
+    if (join.zero) {
+        put_zeros();
+        return;
+    }
     const Base<C> base(join.base, sc);
-    const C c = join.zero ? C(0) : -join.c_rest;
+    const C c = -join.c_rest;
     auto der = [&](int v, C(&a)[VE]) {
         unpack(s[v], a, T());
         base.exps(a);
@@ -520,7 +532,7 @@ lg_distill_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, TeacherA
     }
     __syncthreads();  // the entries' classes over the zeros just written
     if (at >= 0)
-        out[(int64_t)own * dcs] = from_c<T>(join.zero ? C(0) : join.q_scale * (C)r_own - join.c_top * (C)e_own);
+        out[(int64_t)own * dcs] = from_c<T>(join.q_scale * (C)r_own - join.c_top * (C)e_own);
 }
 
 template <typename T>

@@ -137,7 +137,7 @@ def test_top_logits_under_finite_masks(V, dtype, mask):
 @pytest.mark.parametrize("T,spread", [(1e-6, 1.0), (1e-6, 3000.0), (1e-6, 1e-6), (1e-3, 300.0), (1e6, 3.0), (1e6, 30000.0)])
 def test_ends_of_the_temperature(V, dtype, T, spread):
     n = 3
-    x = base.put(np.random.RandomState(V).standard_normal((n, V)) * spread, dtype)
+    x = base.put(np.clip(np.random.RandomState(V).standard_normal((n, V)) * spread, -6e4, 6e4), dtype)
     base.check_top(x, 5, T, dtype)
     rs = np.random.RandomState(V + 1)  # a teacher whose logits are of the size of T
     at, z = np.stack([rs.permutation(V)[:5] for _ in range(n)]), rs.standard_normal((n, 5)) * min(T, 100.0)
@@ -235,3 +235,19 @@ def test_distill_entries_of_no_weight_in_rows_far_below_0(V, dtype, T):
         assert not torch.isnan(got.der1).any() and not torch.isnan(got.loss).any()
         assert torch.isinf(got.loss).tolist() == [False, False, True, False, False]
         check(x, t, T, dtype, out=x)
+
+
+@pytest.mark.parametrize("V", [6, 60, 400, 900, 6000, 40000])
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_a_teacher_without_an_entry_gives_0_whatever_the_row_holds(V, dtype):
+    a = np.random.RandomState(V).standard_normal((6, V))
+    a[0, V // 2], a[1, 0], a[2, V - 1], a[3, 1] = np.nan, np.inf, np.nan, -np.inf
+    a[4] = np.nan
+    index, value = np.full((6, 3), -1), np.zeros((6, 3))
+    for tail in (None, np.full(6, -np.inf)):
+        for i, z in ((index, value), (np.tile([0, 1, 2], (6, 1)), np.full((6, 3), -np.inf))):
+            for layout in base.LAYOUTS:
+                x, t = base.put(a, dtype, layout), teacher_of(i, z, tail, dtype)
+                for out in (None, x):
+                    got = cb.distill_derivatives(x, t, out=out)
+                    assert (got.loss == 0).all() and (got.der1 == 0).all()
