@@ -127,7 +127,8 @@ __device__ int sample_row(const LaneTeam<G>& t, const Items<G, ITEMS>& mine, con
             hi = m;
             int n_hi = n;
             C low = m;
-            LG_EACH(it) if ((stay >> it) & 1) low = a[it] < low ? a[it] : low;
+            // (masked classes, -inf, weigh nothing, and towards them an interval of 16-bit logits cannot be halved)
+            LG_EACH(it) if (((stay >> it) & 1) && a[it] > -lg_inf(C())) low = a[it] < low ? a[it] : low;
             low = t.reduce(low, OpMin());
             lo = (C)((double)m - reach);
             lo = low > lo ? low : lo;

@@ -251,3 +251,21 @@ def test_a_teacher_without_an_entry_gives_0_whatever_the_row_holds(V, dtype):
                 for out in (None, x):
                     got = cb.distill_derivatives(x, t, out=out)
                     assert (got.loss == 0).all() and (got.der1 == 0).all()
+
+
+# ---- draws ----------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("V", [14, 30, 100, 400, 513, 1000, 5000])
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("T", [1e4, 1e6])
+def test_cuts_of_masked_rows_at_large_temperatures(V, dtype, T):
+    # many distinct logits of nearly the same weight, some classes masked: cuts in the middle of them, by count
+    # and by mass, with classes by index in no order
+    n = 40
+    a = np.random.RandomState(V).standard_normal((n, V)) * 1000.0
+    a[::2, ::3] = -np.inf
+    a[1::4, 5] = float(torch.finfo(DTYPES[dtype]).min)
+    x = base.put(a, dtype)
+    u = (torch.arange(n, device="cuda") + 0.5) / n
+    for kw in (dict(top_k=max(2, V // 5)), dict(top_p=0.5), dict(top_k=20, top_p=0.5), dict(top_k=9), dict(top_p=0.05)):
+        base.check_sample(x, u, temperature=T, **kw)
