@@ -538,7 +538,8 @@ lg_sample_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, SampleArg
         // behind it a weight is below a quarter of the last bit: 0
         const float reach = (float)((double)(shift + 2) * 0.6931471805599453 / rs.inv_t);
         const float range = fminf((float)(m + ends[1]), reach);
-        const float per_bin = range > 0.0f && range < lg_inf(0.0f) ? (float)(kBins - 1) / range : 0.0f;
+        // (0: one bin for all that is not masked; a range of some 1e-36 has no reciprocal to scale by)
+        const float per_bin = range > 3e-35f && range < lg_inf(0.0f) ? (float)(kBins - 1) / range : 0.0f;
         auto bin_of = [&](C v) {  // larger logits have lower bins
             if (weigh.infinite) return v == m ? 0 : kBins - 1;
             const float d = fminf((float)(m - v) * per_bin, (float)(kBins - 1));

@@ -269,3 +269,26 @@ def test_cuts_of_masked_rows_at_large_temperatures(V, dtype, T):
     u = (torch.arange(n, device="cuda") + 0.5) / n
     for kw in (dict(top_k=max(2, V // 5)), dict(top_p=0.5), dict(top_k=20, top_p=0.5), dict(top_k=9), dict(top_p=0.05)):
         base.check_sample(x, u, temperature=T, **kw)
+
+
+@pytest.mark.parametrize("V", [14, 100, 700, 1500, 5000, 140000])
+@pytest.mark.parametrize("dtype", ["f64", "f32", "bf16"])
+def test_draws_at_temperatures_next_to_0(V, dtype):
+    # row temperatures down to the smallest f32: what is below the largest logit weighs nothing, equal ones
+    # share, and are cut by index
+    T = [1e-3, 1e-20, 1e-36, 1e-37, 1e-38, 1.4e-45][::1 if V < 10000 else 2]
+    rs = np.random.RandomState(V)
+    a = np.floor(rs.uniform(0, 3, (2 * len(T), V)))  # a third of the classes each
+    a[1::4] = 1.0
+    x = base.put(a, dtype)
+    t = torch.tensor(np.repeat(T, 2), dtype=torch.float32, device="cuda")
+    for u0 in (0.1, 0.9)[:2 if V < 10000 else 1]:
+        u = torch.full((len(a),), u0, device="cuda")
+        for kw in (dict(), dict(top_k=3), dict(top_k=max(2, min(V // 4, 300))), dict(top_p=0.5), dict(top_k=min(V, 400), top_p=0.5),
+                   dict(min_p=0.3)):
+            base.check_sample(x, u, temperature=t, **kw)
+    # logits that are such numbers themselves: a spread of 1e-38
+    x = base.put(rs.uniform(-1e-38, 0, (3, V)), "f32" if dtype == "bf16" else dtype)
+    u = torch.rand((3,), generator=torch.Generator("cuda").manual_seed(V), device="cuda")
+    for kw in (dict(top_k=min(V, 300)), dict(top_p=0.5), dict(top_k=min(V, 400), top_p=0.5)):
+        base.check_sample(x, u, **kw)
