@@ -146,7 +146,8 @@ struct OpMax {
 };
 // exp of a non-positive number by the table-driven method of P. T. P. Tang (ACM TOMS 15, 1989): with
 // x log2(e) = (n + r) / 64, |r| <= 1/2, it is 2^(n / 64), from a table of 64 and an exponent, times a polynomial
-// in r ln2 / 64 (below 0.0055), of which degree 4 leaves 4e-14 and degree 5 4e-17.  10 or 11 operations in 64
+// in r ln2 / 64 (below 0.0055), of which degree 5 leaves 4e-17 (degree 4 leaves 4e-14, some 180 units of a draw's
+// last bit, for 1 to 2 % of the time of draws that are bound by it).  11 operations in 64
 // bits, where exp() with its range checks takes two to three times as many instructions, and f64 rows and the
 // sampler's masses are bound by them (draws 64 x 131071 f32: 55 us against 35).
 struct ExpTable {
@@ -158,7 +159,7 @@ struct ExpTable {
     }
     // 2^(y / 64) for y <= 0.  Below 2^-1020, -inf included, it is 0, and a NaN stays one, with kExact;
     // else it is 2^-1020, for those who round it to 0 anyway.
-    template <int kDegree, bool kExact>
+    template <bool kExact>
     __device__ double exp(double y) const {
         const uint32_t hi = (uint32_t)__double2hiint(y);  // of negative numbers the larger is further down
         const bool none = kExact && hi > 0xc0efdfffu && hi <= 0xfff00000u;  // y <= -65280, -inf; not a NaN
@@ -168,7 +169,7 @@ struct ExpTable {
         const int n = __double2loint(t);
         const double r = x - (t - 6755399441055744.0);
         constexpr double c = 0.6931471805599453 / kSize;
-        double p = kDegree == 5 ? fma(r, c * c * c * c * c / 120.0, c * c * c * c / 24.0) : c * c * c * c / 24.0;
+        double p = fma(r, c * c * c * c * c / 120.0, c * c * c * c / 24.0);
         p = fma(r, p, c * c * c / 6.0);
         p = fma(r, p, c * c / 2.0);
         p = fma(r, p, c);

@@ -64,10 +64,10 @@ __device__ __forceinline__ float part_exp(float x) { return __expf(x); }
 __device__ __forceinline__ double part_exp(double x) { return exp(x); }
 // exp(x) for x <= 0 of a narrow row
 __device__ __forceinline__ float row_exp(float x, const ExpTable&) { return __expf(x); }
-__device__ __forceinline__ double row_exp(double x, const ExpTable& t) { return t.exp<5, true>(x * ExpTable::kPerUnit); }
+__device__ __forceinline__ double row_exp(double x, const ExpTable& t) { return t.exp<true>(x * ExpTable::kPerUnit); }
 __device__ __forceinline__ float row_exp(float d, const Scale<float>& sc, const ExpTable&) { return ex2(d * sc.c); }
 __device__ __forceinline__ double row_exp(double d, const Scale<double>& sc, const ExpTable& t) {
-    return t.exp<5, true>(d * sc.c * ExpTable::kPerUnit);
+    return t.exp<true>(d * sc.c * ExpTable::kPerUnit);
 }
 
 constexpr uint32_t kAbsent32 = 0xffffffffu;  // a NaN no arithmetic gives

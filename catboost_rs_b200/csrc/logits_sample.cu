@@ -9,9 +9,10 @@ namespace {
 //
 // e_i = exp((a_i - max) / T) is taken in 64 bits and held as the integer
 // w_i = rint(e_i 2^s), with 2^s V <= 2^62, so that every sum of weights is exact
-// whatever its order: the draw does not depend on the launch's shape, and a
-// class is drawn as the 64-bit definition draws it unless the drawn number lies
-// within V 2^-s of a border.
+// whatever its order: the draw does not depend on the launch's shape.  A weight
+// is off by less than 4 of its last bit (half of it by rint, the rest by the
+// exponential and its argument), so a class is drawn as the definition draws it
+// unless the drawn number lies within 8 V 2^-s of a border.
 //   top-k   the first k classes in order
 //   top-p   a class stays while the mass before it is below p times the mass top-k left
 //   min-p   a class stays while e_i >= min_p
@@ -98,7 +99,7 @@ __device__ int sample_row(const LaneTeam<G>& t, const Items<G, ITEMS>& mine, con
     LG_EACH(it) {
         w[it] = 0;
         if (!mine.has(it)) continue;
-        const double e = a[it] == m ? 1.0 : table.exp<4, false>(((double)a[it] - (double)m) * per64);
+        const double e = a[it] == m ? 1.0 : table.exp<false>(((double)a[it] - (double)m) * per64);
         w[it] = whole_mass(e, scale);
         stay |= 1u << it;
         if (e < rs.min_p) small |= 1u << it;
@@ -291,7 +292,7 @@ struct Weigh {
     __device__ Weigh(C m_, double inv_t_, int shift, const ExpTable* t)
         : m(m_), inv_t(inv_t_), scale(power_of_2(shift)), min_p(0.0), last{0, 0xffffffffu}, cut(false),
           infinite(m_ == lg_inf(C())), table(t), per64(inv_t_ * ExpTable::kPerUnit) {}
-    __device__ double finite_share(C a) const { return table->template exp<4, false>(((double)a - (double)m) * per64); }
+    __device__ double finite_share(C a) const { return table->template exp<false>(((double)a - (double)m) * per64); }
     // infinite logits share the mass among themselves
     __device__ double share(C a) const { return infinite ? (a == m ? 1.0 : 0.0) : finite_share(a); }
     __device__ u64 whole(double e) const { return whole_mass(e, scale); }

@@ -620,9 +620,10 @@ typedef struct {
  *          largest.
  * Drawn is the first class by INDEX whose running sum of kept probabilities
  * exceeds uniform times their sum.  Weights are held as integers of
- * min(52, 62 - ceil(log2 n_classes)) bits, so the sums are exact; a class
+ * b = min(52, 62 - ceil(log2 n_classes)) bits, so the sums are exact; a class
  * whose probability is below half of the last bit of the largest is never
- * drawn.  Among +inf logits the draw is uniform.
+ * drawn, and a uniform within 8 n_classes 2^-b of a border may go to either
+ * side.  Among +inf logits the draw is uniform.
  *  index  [n]; -1 where the row holds a NaN or masks every class (-inf). */
 CBGPU_API int cbgpu_sample_classes(const cbgpu_logits* logits, const cbgpu_sampling* sampling, int32_t* index,
                                    void* stream);

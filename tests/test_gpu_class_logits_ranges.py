@@ -292,3 +292,24 @@ def test_draws_at_temperatures_next_to_0(V, dtype):
     u = torch.rand((3,), generator=torch.Generator("cuda").manual_seed(V), device="cuda")
     for kw in (dict(top_k=min(V, 300)), dict(top_p=0.5), dict(top_k=min(V, 400), top_p=0.5)):
         base.check_sample(x, u, **kw)
+
+
+@pytest.mark.parametrize("V", [2, 3, 10, 16, 30, 100, 500])
+@pytest.mark.parametrize("layout", ["rows", "dims"])
+def test_numbers_next_to_a_border(V, layout):
+    # a weight of V <= 512 classes is a multiple of 2^-52, off by half of it for its rounding; the exponential's
+    # argument by 3 roundings (3 |x| e^x <= 1.2 of 2^-53) and its table and polynomial by 2 ulp at most (2 of
+    # 2^-52): below 4 2^-52 in all, so a border moves by less than 8 V 2^-52 of the mass (border and mass).  What is
+    # drawn beside it is what the definition draws.
+    n = 64
+    rs = np.random.RandomState(V)
+    x = base.put(rs.standard_normal((n, V)) * 2, "f64", layout)
+    a = base.host(x)
+    share = np.exp((a - a.max(1, keepdims=True)).astype(np.longdouble))
+    upto = np.cumsum(share, axis=1) / share.sum(1, keepdims=True)
+    at = rs.randint(0, V - 1, n)
+    for side in (-1, 1):
+        u = (upto[np.arange(n), at] + side * (8 * V * 2.0 ** -52 + 2.0 ** -53)).astype(np.float64)
+        got = cb.sample_classes(x, torch.from_numpy(u).cuda()).cpu().numpy()
+        want = np.array([np.searchsorted(upto[r], u[r], side="right") for r in range(n)])
+        assert (got == want).all(), (side, int((got != want).sum()))
