@@ -2323,9 +2323,11 @@ namespace {
 template <typename T>
 int mdalloc(T** p, size_t count) {
     cudaError_t e = cudaMalloc((void**)p, sizeof(T) * (count ? count : 1));
-    if (e != cudaSuccess)
+    if (e != cudaSuccess) {
+        cudaGetLastError();  // not the next launch's
         return mfail(e == cudaErrorMemoryAllocation ? CBGPU_ERR_OOM : CBGPU_ERR_CUDA, "cudaMalloc(%zu bytes): %s",
                      sizeof(T) * count, cudaGetErrorString(e));
+    }
     return CBGPU_OK;
 }
 
@@ -3425,22 +3427,29 @@ int cbgpu_multi_set_teacher(cbgpu_multi_session* s, const int32_t* index, const 
             return mfail(CBGPU_ERR_INVALID, "multi_set_teacher: tail %g at row %lld", tail[i], (long long)i);
     }
     MCU(cudaSetDevice(s->device));
-    // (an earlier teacher, or one that found no memory, gives way)
-    cudaFree(s->d_tindex);
-    cudaFree(s->d_tvalue);
-    cudaFree(s->d_ttail);
-    cudaFree(s->d_tloss);
-    s->d_tindex = nullptr;
-    s->d_tvalue = s->d_ttail = s->d_tloss = nullptr;
-    s->t_k = 0;
-    MDA(s->d_tindex, (size_t)n * k);
-    MDA(s->d_tvalue, (size_t)n * k);
-    MDA(s->d_tloss, n);
-    if (tail) MDA(s->d_ttail, n);
-    MCU(cudaMemcpyAsync(s->d_tindex, index, sizeof(int32_t) * (size_t)n * k, cudaMemcpyHostToDevice, s->st));
-    MCU(cudaMemcpyAsync(s->d_tvalue, value, sizeof(double) * (size_t)n * k, cudaMemcpyHostToDevice, s->st));
-    if (tail) MCU(cudaMemcpyAsync(s->d_ttail, tail, sizeof(double) * (size_t)n, cudaMemcpyHostToDevice, s->st));
+    // an earlier teacher gives way once this one is on the device: a call that fails leaves the session as it was
+    struct Arrays {
+        int32_t* index = nullptr;
+        double *value = nullptr, *tail = nullptr, *loss = nullptr;
+        ~Arrays() {
+            cudaFree(index);
+            cudaFree(value);
+            cudaFree(tail);
+            cudaFree(loss);
+        }
+    } now;
+    MDA(now.index, (size_t)n * k);
+    MDA(now.value, (size_t)n * k);
+    MDA(now.loss, n);
+    if (tail) MDA(now.tail, n);
+    MCU(cudaMemcpyAsync(now.index, index, sizeof(int32_t) * (size_t)n * k, cudaMemcpyHostToDevice, s->st));
+    MCU(cudaMemcpyAsync(now.value, value, sizeof(double) * (size_t)n * k, cudaMemcpyHostToDevice, s->st));
+    if (tail) MCU(cudaMemcpyAsync(now.tail, tail, sizeof(double) * (size_t)n, cudaMemcpyHostToDevice, s->st));
     MCU(cudaStreamSynchronize(s->st));
+    std::swap(s->d_tindex, now.index);
+    std::swap(s->d_tvalue, now.value);
+    std::swap(s->d_ttail, now.tail);
+    std::swap(s->d_tloss, now.loss);
     // |w der1| <= max|w| T: the leaf sums' fixed point gives way by T's exponent
     int e = 0;
     std::frexp(std::max(temperature, 1.0), &e);
