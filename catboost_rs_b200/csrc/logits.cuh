@@ -1131,13 +1131,20 @@ constexpr int kLgSmemMost = 200 * 1024;
 
 template <typename K, typename... A>
 int lg_launch_n(const char* who, K kernel, unsigned grid, int threads, size_t smem, cudaStream_t st, A... args) {
-    if (smem > 20 * 1024) {  // with the kernels' static arrays (up to 25 KB) above the 48 KB that need no asking
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kLgSmemMost);
-        if (e != cudaSuccess) return lfail(CBGPU_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
+    cudaError_t e = cudaSuccess;
+    if (smem > 20 * 1024)  // with the kernels' static arrays (up to 25 KB) above the 48 KB that need no asking
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kLgSmemMost);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    // (the launch's own error: the thread's last one may be another call's)
+    if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, kernel, args...);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return lfail(CBGPU_ERR_CUDA, "%s: launch failed: %s", who, cudaGetErrorString(e));
     }
-    kernel<<<grid, (unsigned)threads, smem, st>>>(args...);
-    const cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return lfail(CBGPU_ERR_CUDA, "%s: launch failed: %s", who, cudaGetErrorString(e));
     return CBGPU_OK;
 }
 template <typename K, typename... A>

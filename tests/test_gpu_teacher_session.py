@@ -77,3 +77,23 @@ def test_a_replaced_teacher_counts():
         want.append(grow(rt, K))
         rt.end_device_training()
     assert want[0][0] == want[1][0] and np.array_equal(want[0][1], want[1][1])
+
+
+@pytest.mark.parametrize("V", [10, 100, 700])
+def test_an_error_of_another_call_is_not_a_launchs(V):
+    x, u = torch.randn((8, V), device="cuda"), torch.full((8,), 0.5, device="cuda")
+    few = torch.randn((10000, 100), device="cuda")
+    top = cb.top_logits(x, 3)
+    calls = [lambda: cb.top_logits(x, 3), lambda: cb.top_logits(few, 8), lambda: cb.distill_derivatives(x, top),
+             lambda: cb.sample_classes(x, u)]
+    for call in calls:
+        call()
+    n = 60 << 20  # a prediction that needs 720 MB of device memory
+    model = (np.zeros(1, np.uint32), np.zeros(1), np.array([0, 1], np.uint32), np.zeros(2), np.array([0, 2], np.uint32))
+    held = all_device_memory_but(256 << 20)
+    for call in calls:
+        with pytest.raises(cb.CbGpuError, match="out of memory"):
+            cb.apply_oblivious(np.zeros((1, n), np.float32), model)
+        call()
+    del held
+    torch.cuda.empty_cache()
