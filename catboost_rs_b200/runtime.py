@@ -450,9 +450,12 @@ class B200MultiRuntime(B200Runtime):
         classes (-1: no entry), value [n, k] logits, tail [n] the log-sum-exp
         of its other classes at the temperature.  Before the first tree; the
         grow calls then take no target.  False when the session declines."""
+        with np.errstate(invalid="ignore"):
+            i = np.ascontiguousarray(index, dtype=np.int32)
+        if not np.array_equal(i, index):  # a class of 64 bits would wrap into another one
+            raise _lib.CbGpuError(_lib.ERR_INVALID, "set_teacher: an index is no whole number of 32 bits")
         if not self._s:
             raise _lib.CbGpuError(_lib.ERR_INVALID, "no session")
-        i = np.ascontiguousarray(index, dtype=np.int32)
         v = np.ascontiguousarray(value, dtype=np.float64)
         t = None if tail is None else np.ascontiguousarray(tail, dtype=np.float64)
         if i.ndim != 2 or i.shape[0] != self.n or v.shape != i.shape or (t is not None and t.shape != (self.n,)):
