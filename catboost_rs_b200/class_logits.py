@@ -66,6 +66,12 @@ def _bad(msg: str):
     return _lib.CbGpuError(_lib.ERR_INVALID, msg)
 
 
+def _plain(who, name, x):
+    # memory that stands for its negative (the imaginary part of a conjugate view) would be read as it is
+    if x.is_neg():
+        raise _bad(f"{who}: {name} is a negated view, pass {name}.resolve_neg()")
+
+
 def _logits(who, x):
     torch = _torch or _t()
     if not isinstance(x, torch.Tensor):
@@ -81,6 +87,7 @@ def _logits(who, x):
         raise _bad(f"{who}: {V} classes, outside 1..{MAX_CLASSES}")
     if n > 0x7fffffff:
         raise _bad(f"{who}: {n} rows, at most 2^31 - 1")
+    _plain(who, "logits", x)
     if not x.is_cuda:
         raise _bad(f"{who}: logits must be on a CUDA device")
     rs, cs = x.stride()
@@ -95,6 +102,7 @@ def _side(who, name, v, x, shape, dtypes):
         raise _bad(f"{who}: {name} has dtype {v.dtype}, expected {' or '.join(str(d) for d in dtypes)}")
     if v.shape != shape:
         raise _bad(f"{who}: LengthMismatch: {name} is {tuple(v.shape)}, expected {shape}")
+    _plain(who, name, v)
     return v if v.is_contiguous() else v.contiguous()
 
 
@@ -163,6 +171,7 @@ def _distill(who, logits, teacher, weight, temperature, der1, d=None):
             raise _bad(f"{who}: out must be a {logits.dtype} tensor on the logits' device")
         if der1.shape != logits.shape:
             raise _bad(f"{who}: LengthMismatch: out is {tuple(der1.shape)}, expected {tuple(logits.shape)}")
+        _plain(who, "out", der1)
     loss = logits.new_empty(n, dtype=wide)
     t = _lib.Teacher(index.data_ptr(), value.data_ptr(), None if rest is None else rest.data_ptr(),
                      index.element_size(), _dtypes[value.dtype], shape[1])
