@@ -335,14 +335,8 @@ lg_distill_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, TeacherA
             if (i + j >= 0 && i + j < w.V) out[(int64_t)(i + j) * dcs] = from_c<T>(d[j]);
     };
     auto put_zeros = [&] {  // whatever the row holds
-        const C zero[VE] = {};
-        if (vec_out) {
-            uint4* g = reinterpret_cast<uint4*>(out + ((int64_t)w.v0 * VE - w.head));
-            for (int v = w.whole_lo() + tid; v < w.whole_hi(); v += NT) __stcs(g + v, make_uint4(0, 0, 0, 0));
-            w.template ends<NT>([&](int v) { put(v, zero); });
-        } else {
-            for (int v = tid; v < w.nv; v += NT) put(v, zero);
-        }
+        const int end = w.first(w.nv) < w.V ? w.first(w.nv) : w.V;
+        for (int i = (w.first(0) > 0 ? w.first(0) : 0) + tid; i < end; i += NT) out[(int64_t)i * dcs] = from_c<T>(C(0));
     };
     if (blocks > 1) cluster_arrive<false>();
 
