@@ -1141,10 +1141,7 @@ int lg_launch_n(const char* who, K kernel, unsigned grid, int threads, size_t sm
     cfg.stream = st;
     // (the launch's own error: the thread's last one may be another call's)
     if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, kernel, args...);
-    if (e != cudaSuccess) {
-        cudaGetLastError();
-        return lfail(CBGPU_ERR_CUDA, "%s: launch failed: %s", who, cudaGetErrorString(e));
-    }
+    if (e != cudaSuccess) return lfail(CBGPU_ERR_CUDA, "%s: launch failed: %s", who, cudaGetErrorString(e));
     return CBGPU_OK;
 }
 template <typename K, typename... A>
@@ -1202,10 +1199,7 @@ int lg_launch_wide_n(const char* who, K kernel, int64_t n, const Wide& w, int th
         cfg.gridDim = dim3((unsigned)((n - r0 < step ? n - r0 : step) * w.blocks));
         e = cudaLaunchKernelEx(&cfg, kernel, r0, w.per, args...);
     }
-    if (e != cudaSuccess) {
-        cudaGetLastError();
-        return lfail(CBGPU_ERR_CUDA, "%s: launch failed: %s", who, cudaGetErrorString(e));
-    }
+    if (e != cudaSuccess) return lfail(CBGPU_ERR_CUDA, "%s: launch failed: %s", who, cudaGetErrorString(e));
     return CBGPU_OK;
 }
 template <typename K, typename... A>

@@ -2323,11 +2323,9 @@ namespace {
 template <typename T>
 int mdalloc(T** p, size_t count) {
     cudaError_t e = cudaMalloc((void**)p, sizeof(T) * (count ? count : 1));
-    if (e != cudaSuccess) {
-        cudaGetLastError();  // not the next launch's
+    if (e != cudaSuccess)
         return mfail(e == cudaErrorMemoryAllocation ? CBGPU_ERR_OOM : CBGPU_ERR_CUDA, "cudaMalloc(%zu bytes): %s",
                      sizeof(T) * count, cudaGetErrorString(e));
-    }
     return CBGPU_OK;
 }
 

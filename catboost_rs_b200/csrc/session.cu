@@ -32,6 +32,8 @@ int fail(int code, const char* fmt, ...) {
     vsnprintf(buf, sizeof buf, fmt, ap);
     va_end(ap);
     g_last_error = buf;
+    // the runtime keeps an error until it is asked for: a call that failed leaves none for the next one's launch
+    if (code == CBGPU_ERR_CUDA || code == CBGPU_ERR_OOM || code == CBGPU_ERR_NO_DEVICE) cudaGetLastError();
     return code;
 }
 

@@ -97,3 +97,27 @@ def test_an_error_of_another_call_is_not_a_launchs(V):
         call()
     del held
     torch.cuda.empty_cache()
+
+
+def test_a_call_that_fails_leaves_no_error_for_the_next():
+    n, K = 2000, 3
+    X, borders, rs = columns(n, 3, 7)
+    y = rs.randint(0, K, n)
+    model = (np.zeros(1, np.uint32), np.zeros(1), np.array([0, 1], np.uint32), np.zeros(2), np.array([0, 2], np.uint32))
+    scalar = cb.FitParams(loss="RMSE", depth=3, iterations=2, bootstrap_type="No", random_seed=1)
+    cols = [c.copy() for c in X.T]
+
+    def multi():
+        rt = session(X, borders, K)
+        grow(rt, K, y)
+        rt.end_device_training()
+
+    for call in (lambda: cb.fit(cols, borders, X[:, 0].astype(np.float64), scalar), multi,
+                 lambda: cb.select_borders([cols[0]], 16), lambda: cb.apply_oblivious(np.zeros((1, 64), np.float32), model)):
+        call()
+        held = all_device_memory_but(512 << 20)
+        with pytest.raises(cb.CbGpuError, match="out of memory"):
+            cb.apply_oblivious(np.zeros((1, 120 << 20), np.float32), model)
+        call()
+        del held
+        torch.cuda.empty_cache()
