@@ -82,7 +82,8 @@ __device__ __forceinline__ double plain_nan(double v) {
 }
 
 // Narrow rows: the student's exponentials stay in registers; tgt[i] = the
-// teacher's logit of class i, or absent, and then its exponential.  Bound by issue (1000003 x 10 f64, class by
+// teacher's logit of class i, or absent, and then its exponential.  32-bit rows take the teacher's by __expf, off
+// by 2 ulp and one more for each unit of the argument: by 40 ulp where it weighs e^-34.  Bound by issue (1000003 x 10 f64, class by
 // class, k 4: 94 us at 74 % of the slots; floor 36; 64-bit exponentials from a table, 165 us with exp()).
 template <typename T, int G, int ITEMS>
 __global__ void __launch_bounds__(kLgThreads, 4)
@@ -232,11 +233,14 @@ lg_distill_narrow_kernel(Rows<T> x, TeacherArgs tc, const typename Num<T>::C* __
 // of the cluster exchange their maxima and sums once through each other's
 // shared memory, then each writes its part of der1.  der1 may be the logits'
 // own memory: all reads are before the exchange.
-// Measured: derivatives of 4096 x 64000 bf16 265 us, 4.0 TB/s of a row's one read and one write (floor 163 us);
-// losses of 512 x 131072 f32 92 us (floor 42).  Both passes are bound by the exponentials' pipe, which is 50 %
-// busy over the whole, with one exponential a class and pass; the rest is the chain of a block, copy, maximum,
-// sums, exchange, of which three blocks an SM cover a part.  Rows held in registers instead were slower
+// Measured: derivatives of 4096 x 64000 bf16 266 us, 3.9 TB/s of a row's one read and one write (floor 163 us);
+// losses of 512 x 131072 f32 92 us (floor 42).  No pipe is full: the exponentials', one a class and pass, is busy
+// 51 % of the time (loss: 25 %), and the chain of a block, copy, maximum, sums, exchange, is what the rest waits
+// for; three blocks an SM cover a part of it.  Rows held in registers instead were slower
 // (the unrolled passes leave the instruction cache), and so were 512 threads a block.
+// Roundings to fewer bits than 64 for 32- and 16-bit rows: exponentials (ex2.approx, within 2 ulp) and sums of up
+// to 16 of them; a teacher's 64-bit logits, which become f32 as the student's are; the join for der1, whose
+// per_e - q / s_rest cancels where the student agrees with the teacher, to 2^-24 of the probabilities.
 template <typename C>
 struct DistillPart {  // sums relative to the block's own maxima: m of its logits, z of its entries' logits
     double s_rest, s_top, r_sum, cross;

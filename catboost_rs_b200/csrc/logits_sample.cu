@@ -68,7 +68,7 @@ __device__ __forceinline__ u64 whole_mass(double e, double scale) {
 // Narrow rows: logits and masses in registers, the classes that stay as bits.
 // A thread that has a row to itself counts for each class what comes before
 // it; a team finds the cut by halving an interval of logits.  Bound by issue: 100000 x 10 f64, top-k and
-// top-p, 16 us at 61 % of the slots, of which 64-bit arithmetic is a fifth; with exp() instead of the
+// top-p, 15 us at 60 % of the slots, of which 64-bit arithmetic is a fifth; with exp() instead of the
 // table 37 us.
 template <typename T, int G, int ITEMS>
 __device__ int sample_row(const LaneTeam<G>& t, const Items<G, ITEMS>& mine, const typename Num<T>::C (&a)[ITEMS], int V,
@@ -270,14 +270,18 @@ lg_sample_narrow_kernel(Rows<T> x, SampleArgs a, int shift, int tile, int direct
 // ---- wide rows -------------------------------------------------------------------------------
 //
 // top-k up to kLgMaxTop: the first block collects the first k classes and does the rest alone.
-// Else each class is weighed once.  Where top-p or a larger top-k cuts, a
+// Else each class is weighed once, or again where the cut was not in the bin
+// it was looked for in.  Where top-p or a larger top-k cuts, a
 // histogram of the logits shows in which bin the cut lies (a bin's classes weigh nearly the same, so
 // counts are enough: f32 masses added in shared memory took three times as long); the
 // bin's classes and its neighbours' are collected and sorted, and the cut is then taken
 // with exact masses, which also show whether the bin was the right one.
 // Measured: 64 x 131071 f32 without cuts 32 us, where 64-bit exponentials take a fifth of their pipe and the
 // rest is a block's chain of copy, maximum, masses and draw, three cluster barriers long; 256 x 128000
-// bf16 with top-k 50 by row 37 us (1.8 TB/s); one row of 32000, top-p, 18 us on the device.
+// bf16 with top-k 50 by row 37 us (1.8 TB/s); one row of 32000, top-p, 18 us on the device.  Cuts over many
+// rows are far from their floor (256 x 128000 bf16, 10 us): top-k 1000 with top-p 0.95 184 us, through the four
+// passes over shared memory; top-p 0.95 alone over normal logits 1290 us, where three bins hold more classes
+// than the list (kTopCap) and the cut is found bit by bit.
 
 template <typename T>
 struct Weigh {

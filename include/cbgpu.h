@@ -533,7 +533,10 @@ CBGPU_API int cbgpu_apply_oblivious(const float* features_fm, int64_t n, int32_t
  * and be captured into graphs.  Arithmetic and the "wide" outputs are f64 for
  * CBGPU_F64 logits and f32 for the other types, whose terms are added up in
  * f32 for up to 16 classes at a time and in 64 bits from there (der1's two
- * factors join the sums of a row's up to 16 blocks in f32).
+ * factors join the sums of a row's up to 16 blocks in f32).  32-bit
+ * exponentials are within a few units of 2^-24 of themselves; differences of
+ * logits are scaled by an f32 log2(e) / temperature, and a teacher's f64
+ * logits are rounded to f32 beside f32 or 16-bit rows.
  * The same call gives the same bits again; rows in another layout or in a
  * batch of another size may be summed in another grouping (the last bits of
  * loss, der1 and tail).  Outputs may not overlap inputs or each other, but
