@@ -35,6 +35,16 @@ struct TeacherBase {
     __device__ double entry(double zj, double inv_t) const { return fma(zj - z, inv_t, -lift); }
 };
 
+// The least d whose exp(d) is more than 0 in 64 bits: a bucket has a weight if its exponential there has one, also
+// where the 32-bit one is 0.
+constexpr double kNoWeight = -745.0;
+
+// An entry's part of the loss' first sum: r = exp(d), ln_a = the student's (a - m) / T.
+__device__ __forceinline__ double cross_part(double r, double d, double ln_a) {
+    if (ln_a == -lg_inf(0.0)) return d > kNoWeight ? lg_inf(0.0) : 0.0;
+    return r != 0.0 ? r * (d - ln_a) : 0.0;
+}
+
 template <typename C>
 struct RowOut {  // what turns a row's logits into its loss and derivative
     double loss;
@@ -51,6 +61,7 @@ __device__ __forceinline__ RowOut<C> distill_finish(double w, double t, double s
     if (o.zero) return o;
     double kl = cross;
     if (r_tail > 0.0 || r_tail != r_tail) kl += r_tail * (tail_rel - log(s_rest) - rest_ln);
+    else if (s_rest == 0.0 && tail_rel > kNoWeight) kl = lg_inf(0.0);
     const double per_r = 1.0 / r_sum, per_s = 1.0 / s, wt = w * t;
     o.loss = wt * t * (kl * per_r + log(s * per_r));
     o.q_scale = (C)(wt * per_r);
@@ -160,7 +171,7 @@ lg_distill_narrow_kernel(Rows<T> x, TeacherArgs tc, const typename Num<T>::C* __
                 const double d = z_base.entry((double)tgt[i], sc.inv_t);
                 const C rj = row_exp((C)d, table);
                 r_sum += (double)rj;
-                if (rj != C(0)) cross += (double)rj * (d - ((double)ai - (double)m) * sc.inv_t);
+                cross += cross_part((double)rj, d, ((double)ai - (double)m) * sc.inv_t);
                 tgt[i] = rj;
             }
             t.sync();
@@ -176,7 +187,7 @@ lg_distill_narrow_kernel(Rows<T> x, TeacherArgs tc, const typename Num<T>::C* __
                 const double d = z_base.entry((double)tgt[mine.first + it], sc.inv_t);
                 const double rj = (double)row_exp((C)d, table);
                 r_sum += rj;
-                if (rj != 0.0) cross += rj * (d - ((double)a[it] - (double)m) * sc.inv_t);
+                cross += cross_part(rj, d, ((double)a[it] - (double)m) * sc.inv_t);
                 tgt[mine.first + it] = (C)rj;
             } else {
                 sum_rest += e;

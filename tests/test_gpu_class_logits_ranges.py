@@ -313,3 +313,25 @@ def test_numbers_next_to_a_border(V, layout):
         got = cb.sample_classes(x, torch.from_numpy(u).cuda()).cpu().numpy()
         want = np.array([np.searchsorted(upto[r], u[r], side="right") for r in range(n)])
         assert (got == want).all(), (side, int((got != want).sum()))
+
+
+@pytest.mark.parametrize("V", [6, 10, 16, 30, 100, 200, 400, 900, 6000, 40000])
+@pytest.mark.parametrize("dtype", ["f64", "f32", "bf16"])
+@pytest.mark.parametrize("n", [4, 400])
+def test_weights_below_32_bits_on_masked_classes(V, dtype, n):
+    # a class that the student masks and the teacher does not gives +inf however little the teacher gives it (down
+    # to e^-745, where it is 0 in 64 bits too), an entry as well as all others beside a tail
+    rs = np.random.RandomState(V)
+    below = [20.0, 80.0, 90.0, 150.0, 600.0, 900.0]
+    a = rs.standard_normal((2 * len(below), V))
+    index, value, tail = np.tile([0, 1, 2], (len(a), 1)), np.zeros((len(a), 3)), np.full(len(a), -np.inf)
+    for r, d in enumerate(below):
+        a[r, 1], value[r, 1] = -np.inf, -d
+        a[len(below) + r, 3:], tail[len(below) + r] = -np.inf, -d
+    want = np.array([d < 745 for d in below] * 2)
+    at = np.arange(max(n, len(a))) % len(a)
+    got = cb.distill_derivatives(base.put(a[at], dtype), teacher_of(index[at], value[at], tail[at], dtype))
+    loss = base.host(got.loss)
+    assert (loss[want[at]] == np.inf).all() and np.isfinite(loss[~want[at]]).all()
+    assert torch.isfinite(got.der1).all()
+    assert torch.equal(got.loss, cb.distill_loss(base.put(a[at], dtype), teacher_of(index[at], value[at], tail[at], dtype)))
