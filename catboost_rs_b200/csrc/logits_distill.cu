@@ -35,14 +35,11 @@ struct TeacherBase {
     __device__ double entry(double zj, double inv_t) const { return fma(zj - z, inv_t, -lift); }
 };
 
-// The least d whose exp(d) is more than 0 in 64 bits: a bucket has a weight if its exponential there has one, also
-// where the 32-bit one is 0.
-constexpr double kNoWeight = -745.0;
-
-// An entry's part of the loss' first sum: r = exp(d), ln_a = the student's (a - m) / T.
-__device__ __forceinline__ double cross_part(double r, double d, double ln_a) {
-    if (ln_a == -lg_inf(0.0)) return d > kNoWeight ? lg_inf(0.0) : 0.0;
-    return r != 0.0 ? r * (d - ln_a) : 0.0;
+// A teacher's exponential r = exp(d) for the loss.  Where the 32-bit one is 0 (from -87 on) the 64-bit one is taken:
+// the student's logarithm beside it may be as large as it is small, or infinite.  (64-bit ones end at -707.)
+template <typename C>
+__device__ __forceinline__ double loss_weight(C r, double d) {
+    return sizeof(C) == 4 && r == C(0) && d > -745.0 ? exp(d) : (double)r;
 }
 
 template <typename C>
@@ -61,7 +58,6 @@ __device__ __forceinline__ RowOut<C> distill_finish(double w, double t, double s
     if (o.zero) return o;
     double kl = cross;
     if (r_tail > 0.0 || r_tail != r_tail) kl += r_tail * (tail_rel - log(s_rest) - rest_ln);
-    else if (s_rest == 0.0 && tail_rel > kNoWeight) kl = lg_inf(0.0);
     const double per_r = 1.0 / r_sum, per_s = 1.0 / s, wt = w * t;
     o.loss = wt * t * (kl * per_r + log(s * per_r));
     o.q_scale = (C)(wt * per_r);
@@ -163,17 +159,29 @@ lg_distill_narrow_kernel(Rows<T> x, TeacherArgs tc, const typename Num<T>::C* __
         const TeacherBase z_base(zm, tl, sc);
         C sum_top = 0, sum_rest = 0;
         double r_sum = 0.0, cross = 0.0;
+        constexpr bool kNone = sizeof(C) == 4;
+        u64 none = 0;  // which of this lane's entries have a teacher's 32-bit exponential of 0
+        auto logit = [&](int i) { return to_c(direct ? g[r * x.row_stride + (int64_t)i * x.class_stride] : row[i]); };
+        // their part of `cross`, for which they keep their logit until here
+        auto small = [&](int i) {
+            const double d = z_base.entry((double)tgt[i], sc.inv_t), rj = loss_weight(C(0), d);
+            if (rj != 0.0) cross += rj * (d - ((double)logit(i) - (double)m) * sc.inv_t);
+            tgt[i] = C(0);
+        };
         if (by_entry) {  // a lane an entry: fewer steps in 64 bits than by class (for which a warp's rows differ)
             for (int j0 = 0; j0 < tc.k; j0 += G) {
                 if (!((claimed >> (j0 / G)) & 1)) continue;
                 const int i = (int)tc.idx((r0 + r) * tc.k + j0 + t.rank);
-                const C ai = to_c(direct ? g[r * x.row_stride + (int64_t)i * x.class_stride] : row[i]);
+                const C ai = logit(i);
                 const double d = z_base.entry((double)tgt[i], sc.inv_t);
                 const C rj = row_exp((C)d, table);
                 r_sum += (double)rj;
-                cross += cross_part((double)rj, d, ((double)ai - (double)m) * sc.inv_t);
-                tgt[i] = rj;
+                if (rj != C(0)) cross += (double)rj * (d - ((double)ai - (double)m) * sc.inv_t);
+                if (kNone && rj == C(0)) none |= 1ull << (j0 / G);
+                else tgt[i] = rj;
             }
+            for (; none != 0; none &= none - 1)
+                small((int)tc.idx((r0 + r) * tc.k + (__ffsll((long long)none) - 1) * G + t.rank));
             t.sync();
         }
         LG_EACH(it) {
@@ -187,20 +195,21 @@ lg_distill_narrow_kernel(Rows<T> x, TeacherArgs tc, const typename Num<T>::C* __
                 const double d = z_base.entry((double)tgt[mine.first + it], sc.inv_t);
                 const double rj = (double)row_exp((C)d, table);
                 r_sum += rj;
-                cross += cross_part(rj, d, ((double)a[it] - (double)m) * sc.inv_t);
-                tgt[mine.first + it] = (C)rj;
+                if (rj != 0.0) cross += rj * (d - ((double)a[it] - (double)m) * sc.inv_t);
+                if (kNone && rj == 0.0) none |= 1ull << it;
+                else tgt[mine.first + it] = (C)rj;
             } else {
                 sum_rest += e;
             }
             a[it] = e;
         }
+        for (; none != 0; none &= none - 1) small(mine.first + __ffsll((long long)none) - 1);
         const double s_top = t.reduce((double)sum_top, OpSum());
         double s_rest = t.reduce((double)sum_rest, OpSum()), rest_ln = 0.0;
         r_sum = t.reduce(r_sum, OpSum());
         cross = t.reduce(cross, OpSum());
-        const double r_tail = (double)row_exp((C)z_base.tail, table);
+        const double r_tail = loss_weight(row_exp((C)z_base.tail, table), z_base.tail);
         if (s_rest < kFar && r_tail > 0.0) {  // the same for a row's lanes
-            auto logit = [&](int i) { return to_c(direct ? g[r * x.row_stride + (int64_t)i * x.class_stride] : row[i]); };
             C mr = -lg_inf(C());
             LG_EACH(it) if (mine.has(it) && !((top >> it) & 1)) mr = OpMax()(mr, logit(mine.first + it));
             mr = t.reduce(mr, OpMax());

@@ -594,7 +594,9 @@ typedef struct {
  *          other array of the call.
  * A row whose classes are all masked (-inf), or whose teacher has no entry
  * left, gives 0; NaN or +inf among a row's logits or entries gives NaN; a
- * class the student masks but the teacher does not gives loss +inf. */
+ * class the student masks but the teacher does not gives loss +inf (one whose
+ * weight exp((z - z_max) / T) is below 2^-1020 may count as masked), and so
+ * may a loss beyond 1e300 (f64 rows masked by numbers near the lowest). */
 CBGPU_API int cbgpu_distill(const cbgpu_logits* logits, const cbgpu_teacher* teacher, const void* weight,
                             double temperature, void* loss, void* der1, int64_t der1_row_stride,
                             int64_t der1_class_stride, void* stream);

@@ -41,7 +41,7 @@ def teacher_of(index, value, tail, dtype):
                         None if tail is None else torch.tensor(np.asarray(tail, dtype=np.float64), dtype=wide, device="cuda"))
 
 
-def check(x, teacher, T, dtype, out=None):
+def check(x, teacher, T, dtype, out=None, lost=0.0):
     """Loss and derivatives against the definition, taken on rows from which their largest logit was
     subtracted first (so that the 64-bit form keeps its bits when the logits are large beside T)."""
     u, rel = base.unit(dtype), 2 * base.unit(dtype) * 124
@@ -77,7 +77,7 @@ def check(x, teacher, T, dtype, out=None):
             else:
                 assert np.array_equal(g, wl, equal_nan=True), (r, g, wl)
         own = np.maximum(rel, u * (3 * np.minimum(-row / T, 800.0) + 128))
-        bound = T * own * 2 * (p + q) + base.rounding(dtype) * np.abs(wd) + small + 2 * T * low
+        bound = T * own * 2 * (p + q) + base.rounding(dtype) * np.abs(wd) + small + 2 * T * max(low, lost)
         beyond = np.abs(wd) + bound > float(torch.finfo(x.dtype).max)
         assert (np.isfinite(der1[r]) | beyond | np.isnan(wd)).all() and (der1[r] * np.sign(wd) >= 0)[beyond].all()
         off = np.where(beyond, 0.0, np.abs(der1[r] - wd) - bound)
@@ -335,3 +335,31 @@ def test_weights_below_32_bits_on_masked_classes(V, dtype, n):
     assert (loss[want[at]] == np.inf).all() and np.isfinite(loss[~want[at]]).all()
     assert torch.isfinite(got.der1).all()
     assert torch.equal(got.loss, cb.distill_loss(base.put(a[at], dtype), teacher_of(index[at], value[at], tail[at], dtype)))
+
+
+@pytest.mark.parametrize("V", [10, 16, 30, 100, 200, 400, 900, 6000, 40000])
+@pytest.mark.parametrize("dtype,far", [("f64", -1e10), ("f64", -1e200), ("f32", -300.0), ("f32", -1e10), ("f32", -1e38),
+                                       ("bf16", -1e30), ("f16", -6e4)])
+@pytest.mark.parametrize("n", [16, 400])
+def test_weights_below_32_bits_on_classes_far_below(V, dtype, far, n):
+    # as much below as the weight is small: their product is the loss, finite, of an entry and of all others
+    rs = np.random.RandomState(V)
+    below = [20.0, 80.0, 90.0, 150.0, 600.0, 700.0]
+    a = rs.standard_normal((2 * len(below), V))
+    index, value, tail = np.tile([0, 1, 2], (len(a), 1)), np.zeros((len(a), 3)), np.full(len(a), -np.inf)
+    for r, d in enumerate(below):
+        a[r, 1], value[r, 1] = far, -d
+        a[len(below) + r, 3:], tail[len(below) + r] = far, -d
+    at = np.arange(n) % len(a)
+    x, t = base.put(a[at], dtype), teacher_of(index[at], value[at], tail[at], dtype)
+    loss = cb.distill_loss(x, t)
+    same = torch.from_numpy(at).cuda() if n > len(a) else None
+    few = cb.TopLogits(*(v[:len(a)] for v in (t.index, t.value, t.tail)))
+    lost = 0.0 if dtype == "f64" else 2.0 ** -126 * 1e20  # der1 beside a tail, as in test_distill_others_far_below
+    got = check(x[:len(a)].contiguous(), few, 1.0, dtype, lost=lost)
+    assert torch.isfinite(got.loss).all()
+    if same is not None:  # both kernels are within the bound of check
+        off = (loss.double() - got.loss.double()[same]).abs()
+        u = base.unit(dtype)
+        size = -far + 1000.0
+        assert (off <= 2 * (3 * 248 * u + 252 * u * loss.double().abs() + 6 * u * size * (size < 1e6))).all()
