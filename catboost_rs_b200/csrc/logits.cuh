@@ -425,9 +425,8 @@ struct WideRow {
     }
     // Copies this block's part to s; see(vector) is called for each vector on
     // the way.  kAhead loads a thread are under way at a time.
-    template <int NT = kLgThreads, typename See>
+    template <int NT = kLgThreads, int kAhead = 8, typename See>
     __device__ void load(uint4* s, See see) const {
-        constexpr int kAhead = 8;
         const int lo = whole_lo(), hi = whole_hi();
         const uint4* g = reinterpret_cast<const uint4*>(row + ((int64_t)v0 * VE - head));
         int v = lo + threadIdx.x;

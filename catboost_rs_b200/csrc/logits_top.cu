@@ -384,8 +384,11 @@ lg_top_thread_kernel(Rows<T> x, int k, Scale<float> sc, int unit, T* __restrict_
 // sum is taken in the same second look.  2048 x 64000 bf16, k 64: 141 us (floor 41), with the
 // exponentials' pipe 29 % busy and 41 % of the issue slots; the rest is a block's chain of copy, bound,
 // collection, hand-over and sort with their barriers.  8 x 131071 f32, k 128: 12 us on the device.
-template <typename T>
-__global__ void __launch_bounds__(kLgThreads)
+// kBlocks: what an SM holds at least.  Five, of 48 registers, for rows of up to 16 KB (20000 x 700 f32, k 16: 184 us
+// against 207 with 62 registers; bf16 203 against 225); above, where shared memory leaves three, registers count
+// (512 x 131072 f32: 131 us against 143; 2048 x 64000 bf16 143 against 147).
+template <typename T, int kBlocks>
+__global__ void __launch_bounds__(kLgThreads, kBlocks)
 lg_top_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, int k, Scale<typename Num<T>::C> sc,
                    T* __restrict__ value, int32_t* __restrict__ index, typename Num<T>::C* __restrict__ tail) {
     typedef typename Num<T>::C C;
@@ -407,7 +410,7 @@ lg_top_wide_kernel(int64_t row0, int per, int64_t ahead, Rows<T> x, int k, Scale
     if (cl.blocks > 1) cluster_arrive<false>();
     if (tid == 0 && r + ahead < x.n) WideRow<T>(x, r + ahead, cl.rank, per).prefetch();
     VecMax<T> most;
-    w.load(s, [&](const uint4& q) { most(q); });
+    w.template load<kLgThreads, kBlocks == 5 && sizeof(T) == 4 ? 4 : 8>(s, [&](const uint4& q) { most(q); });
     if (cl.blocks > 1) cluster_wait();  // every block runs
     int turn = 0;
     C rest, ref = C(0);
@@ -484,8 +487,12 @@ int run_top(const cbgpu_logits* x, int k, double temp, void* value, int32_t* ind
     const Scale<C> sc(temp);
     if (is_wide(rows.n, rows.V)) {
         const Wide w = wide_shape<T>(rows.n, rows.V);
-        return lg_launch_wide(who, lg_top_wide_kernel<T>, rows.n, w, w.smem, st, w.ahead, rows, k, sc, (T*)value, index,
-                              (C*)tail);
+        auto wide = [&](auto kernel) {
+            return lg_launch_wide(who, kernel, rows.n, w, w.smem, st, w.ahead, rows, k, sc, (T*)value, index, (C*)tail);
+        };
+        if constexpr (sizeof(T) < 8)
+            if (w.smem <= 16384) return wide(lg_top_wide_kernel<T, 5>);
+        return wide(lg_top_wide_kernel<T, 4>);
     }
     auto narrow = [&](auto kernel, int lanes) {
         const Tile t = narrow_tile(rows.n, rows.V, sizeof(T), kLgThreads / lanes);
