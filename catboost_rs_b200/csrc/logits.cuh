@@ -733,7 +733,7 @@ __device__ __forceinline__ void block_reduce(V (&v)[N], V (*scratch)[kLgWarps], 
 // too many (or NaN too few), the exact bound (logit, index) is found bit by
 // bit over the cluster instead, at some 50 passes over shared memory.  16-bit rows of 1025 to some 2050 classes have
 // fewer vectors than threads: a k above their number (129 at least) leaves no bound, and the exact way is the only
-// one (20000 x 1500 bf16, 188 vectors: 385 us at k 129, 1880 at k 200).
+// one (20000 x 1500 bf16, 188 vectors: 393 us at k 129, 1950 at k 200).
 
 constexpr int kTopCap = 1024;  // classes the first block can collect
 

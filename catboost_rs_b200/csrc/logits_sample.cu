@@ -279,8 +279,8 @@ lg_sample_narrow_kernel(Rows<T> x, SampleArgs a, int shift, int tile, int direct
 // Measured: 64 x 131071 f32 without cuts 32 us, where 64-bit exponentials take a fifth of their pipe and the
 // rest is a block's chain of copy, maximum, masses and draw, three cluster barriers long; 256 x 128000
 // bf16 with top-k 50 by row 37 us (1.8 TB/s); one row of 32000, top-p, 18 us on the device.  Cuts over many
-// rows are far from their floor (256 x 128000 bf16, 10 us): top-k 1000 with top-p 0.95 184 us, through the four
-// passes over shared memory; top-p 0.95 alone over normal logits 1290 us, where three bins hold more classes
+// rows are far from their floor (256 x 128000 bf16, 10 us): top-k 1000 with top-p 0.95 186 us, through the four
+// passes over shared memory; top-p 0.95 alone over normal logits 1300 us and more, where three bins hold more classes
 // than the list (kTopCap) and the cut is found bit by bit.
 
 template <typename T>

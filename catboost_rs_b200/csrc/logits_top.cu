@@ -381,7 +381,7 @@ lg_top_thread_kernel(Rows<T> x, int k, Scale<float> sc, int unit, T* __restrict_
 
 // Wide rows: the maxima that the threads keep while they copy their part give a bound that a few more
 // than k classes reach (logits.cuh, wide_top); those go to the first block, which sorts them, and the tail's
-// sum is taken in the same second look.  2048 x 64000 bf16, k 64: 141 us (floor 41), with the
+// sum is taken in the same second look.  2048 x 64000 bf16, k 64: 138 us (floor 41), with the
 // exponentials' pipe 29 % busy and 41 % of the issue slots; the rest is a block's chain of copy, bound,
 // collection, hand-over and sort with their barriers.  8 x 131071 f32, k 128: 12 us on the device.
 // kBlocks: what an SM holds at least.  Five, of 48 registers, for rows of up to 16 KB (20000 x 700 f32, k 16: 184 us
